@@ -280,16 +280,14 @@ def _own_attend(s):
                   "dv": torch.empty_like(s["v"])}
             if s["bias"] is not None:
                 r["dbias"] = torch.empty(c["buckets"], H, device=dev)
-        full = r["out"] if c["dtype"] == "f32" else torch.empty(s["total_q"], H * D, device=dev) if c["train"] else None
-        s["call"] = (a, torch.empty(max(1, size.value), dtype=torch.uint8, device=dev), full, torch.zeros(2, dtype=torch.int32, device=dev), r)
-    a, space, full, status, r = s["call"]
+        s["call"] = (a, torch.empty(max(1, size.value), dtype=torch.uint8, device=dev), torch.zeros(2, dtype=torch.int32, device=dev), r)
+    a, space, status, r = s["call"]
     p, st = capi.ptr, capi.current_stream()
     ins = (C.byref(a), p(s["q"]), H * D, p(s["k"]), Hk * D, p(s["v"]), Hk * D, p(s["q_offsets"]), p(s["k_offsets"]), p(s["q_start"]),
            p(s["keep"]), p(s["bias"]))
-    capi.check(lib.dctr_cross_attention_fwd(*ins, p(r["out"]), H * D, None if full is r["out"] else p(full), H * D, p(r.get("lse")), p(status),
-                                            p(space), space.numel(), st))
+    capi.check(lib.dctr_cross_attention_fwd(*ins, p(r["out"]), H * D, p(r.get("lse")), p(status), p(space), space.numel(), st))
     if c["train"]:
-        capi.check(lib.dctr_cross_attention_bwd(*ins, p(full), H * D, p(r["lse"]), p(s["dout"]), H * D, p(r["dq"]), H * D, p(r["dk"]), Hk * D,
+        capi.check(lib.dctr_cross_attention_bwd(*ins, p(r["out"]), H * D, p(r["lse"]), p(s["dout"]), H * D, p(r["dq"]), H * D, p(r["dk"]), Hk * D,
                                                 p(r["dv"]), Hk * D, p(r.get("dbias")), p(space), space.numel(), st))
     return r
 
