@@ -18,8 +18,10 @@ LIB = os.path.join(LIBDIR, "libdeepctr_hip.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+# -packed-fp32-ops: hipcc -O3 forms v_pk_add/mul/fma_f32 from ordinary float code, some forms of which have given wrong results on this
+# chip now and then (the host pass warns that it does not know the feature: harmless)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function", "-Wno-unused-value", "-Wno-unused-result",
-         "-I", INCLUDE]
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", INCLUDE]
 
 
 # per-file flags.  gemm_dr3.hip, gemm_ts.hip: hipcc's SLP pass pairs the split's f32 subtractions into v_pk_add_f32, slower beside MFMAs than two
@@ -44,7 +46,7 @@ def sources_hash() -> str:
 
 
 def _headers_mtime():
-    m = os.path.getmtime(os.path.join(INCLUDE, "deepctr_hip.h"))
+    m = max(os.path.getmtime(os.path.join(INCLUDE, "deepctr_hip.h")), os.path.getmtime(os.path.abspath(__file__)))     # (the flags live here)
     for f in os.listdir(CSRC):
         if f.endswith(".h"):
             m = max(m, os.path.getmtime(os.path.join(CSRC, f)))
