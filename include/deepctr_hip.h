@@ -425,6 +425,67 @@ int dctr_dcn_cross_bwd(const float* d_xs, const float* d_xlw, const float* d_w, 
                        int B, int D, int L, float* d_dx0, int dx0_ld, float* d_dw, float* d_db,
                        float* d_workspace, size_t workspace_bytes, void* stream);
 
+/* ---- sequence operators: attention over another sequence's states, and the softmax loss over a vocabulary ---------------------------
+ * Beyond DIN's sigmoid-scored pooling of a behaviour list (DIN.py:152-172) and the binary loss heads: multi-head softmax attention of any
+ * number of queries per example (candidate ads, a sequence's own steps, one new event) over that example's history, with a learned bias per
+ * bucket of the distance between them, and the cross entropy of rows against every row of an item table.  Types: F32, or BF16 with all
+ * sums, softmax statistics, biases, their gradients and losses in f32. */
+enum { DCTR_TYPE_F32 = 0, DCTR_TYPE_BF16 = 1 };
+#define DCTR_MAX_REL_BUCKETS 128
+#define DCTR_MAX_REL_SPAN 1024         /* last boundary - first boundary */
+#define DCTR_MAX_POSITION (1 << 28)
+typedef struct dctr_attention {
+    int32_t dtype;                     /* DCTR_TYPE_* of q, k, v, out and their gradients                                     */
+    int32_t n_seg;                     /* examples: segment b = rows [q_offsets[b], q_offsets[b+1]) x [k_offsets[b], k_offsets[b+1]) */
+    int32_t heads, kv_heads;           /* query head h reads key head h / (heads / kv_heads)                                  */
+    int32_t head_dim;                  /* a multiple of 8, 8..128; head h of a row is columns [h*head_dim, (h+1)*head_dim)     */
+    int32_t max_q, max_k;              /* no segment has more rows (the launches are sized by them)                           */
+    int32_t causal;                    /* 1: a query sees the keys at positions <= its own only                               */
+    int64_t total_q, total_k;          /* rows of the q / k, v arrays: offsets stay within them                               */
+    float   scale;                     /* of the scores, e.g. 1/sqrt(head_dim)                                                */
+    int32_t n_buckets;                 /* rows of the relative bias; 0: none                                                  */
+    int32_t boundaries[DCTR_MAX_REL_BUCKETS - 1];  /* ascending; bucket(d) = how many are <= d (tf.feature_column.bucketized_column's rule),
+                                                    * d = key position - query position                                       */
+} dctr_attention;
+/* Key j of a segment is at position j, query i at d_q_start[b] + i (d_q_start null: at i).  Scores
+ *     s_ij = scale <q_i, k_j> + d_rel_bias[bucket(j - q_start - i), h]      over the keys with d_key_keep[row] != 0 (null: all) that a causal
+ * query sees; out_i = sum_j softmax(s)_ij v_j, d_lse[row, h] = log sum_j exp(s_ij) (may be null).  A query that sees no key: out 0, lse -inf.
+ * Rows outside every segment are neither read nor written; what a key that is not kept holds (inf, NaN) reaches nothing.
+ *   d_q [total_q, heads * head_dim], d_k / d_v [total_k, kv_heads * head_dim]; row strides *_ld in elements; rows 16-byte aligned
+ *   d_q_offsets / d_k_offsets int32 [n_seg + 1]; d_q_start int32 [n_seg] or null; d_rel_bias f32 [n_buckets, heads]
+ *   d_status int32[2] or null: [0] = 1, [1] = b if segment b's offsets leave the arrays, descend, or hold more than max_q / max_k rows
+ *              (or its q_start is beyond +-DCTR_MAX_POSITION): such a segment is cut to what is within
+ *   d_workspace: dctr_cross_attention_workspace_bytes(a, backward = 0 / 1) bytes, 16-byte aligned, overwritten; calls that may run at the same
+ *              time (streams, captured graphs) need one each.  A handful of queries per segment (serving) splits long histories over blocks. */
+int dctr_cross_attention_workspace_bytes(const dctr_attention* a, int backward, int64_t* bytes);
+int dctr_cross_attention_fwd(const dctr_attention* a, const void* d_q, int q_ld, const void* d_k, int k_ld, const void* d_v, int v_ld,
+                             const int32_t* d_q_offsets, const int32_t* d_k_offsets, const int32_t* d_q_start, const uint8_t* d_key_keep,
+                             const float* d_rel_bias, void* d_out, int out_ld, float* d_lse, int32_t* d_status,
+                             void* d_workspace, size_t workspace_bytes, void* stream);
+/* gradients of the same call: d_dout = dL/dout in; dL/dq, dL/dk, dL/dv (shared key heads: summed over their query heads) and dL/d rel_bias
+ * [n_buckets, heads] f32 (null: not wanted) overwritten -- 0 where nothing contributes.  d_out, d_lse: the forward's.  Sums
+ * run in a fixed order: the same call gives the same bits. */
+int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld, const void* d_k, int k_ld, const void* d_v, int v_ld,
+                             const int32_t* d_q_offsets, const int32_t* d_k_offsets, const int32_t* d_q_start, const uint8_t* d_key_keep,
+                             const float* d_rel_bias, const void* d_out, int out_ld, const float* d_lse, const void* d_dout,
+                             int dout_ld, void* d_dq, int dq_ld, void* d_dk, int dk_ld, void* d_dv, int dv_ld, float* d_drel_bias,
+                             void* d_workspace, size_t workspace_bytes, void* stream);
+/* Softmax cross entropy of N rows against a vocabulary's table, without the [N, V] logits: z = x w^T + b (d_b f32 [V] or null),
+ *     d_loss[n] = lse_n - z[n, label_n]      d_lse[n] = log sum_v exp(z_nv) (may be null)
+ * d_labels int32 [N]; a negative label = a row without one: loss 0, no gradient; one >= V is treated the same and flagged in d_status
+ * (int32[2] or null: [0] = 1, [1] = the label).  Gradients are of  sum_n scale * d_row_scale[n] * loss_n  (d_row_scale f32 [N] or null = 1;
+ * scale = 1/batch for a mean).  d_x [N, D], d_w [V, D] and the gradients in `dtype`, rows 16-byte aligned, D a multiple of 8, 8..256.
+ *   fwd: loss, lse and, d_dx not null, dL/dx [N, dx_ld] from the same pass over the table
+ *   bwd_weights: dL/dw [V, dw_ld] and (may be null) dL/db f32 [V], overwritten; d_lse: the forward's
+ * d_workspace: dctr_vocab_softmax_workspace_bytes(dtype, N, V, D, train) bytes (train = 0: fwd without dx), as above. */
+int dctr_vocab_softmax_workspace_bytes(int dtype, int N, int64_t V, int D, int train, int64_t* bytes);
+int dctr_vocab_softmax_fwd(int dtype, const void* d_x, int x_ld, const void* d_w, int w_ld, const float* d_b, const int32_t* d_labels, int N,
+                           int64_t V, int D, const float* d_row_scale, float scale, float* d_loss, float* d_lse, void* d_dx, int dx_ld,
+                           int32_t* d_status, void* d_workspace, size_t workspace_bytes, void* stream);
+int dctr_vocab_softmax_bwd_weights(int dtype, const void* d_x, int x_ld, const void* d_w, int w_ld, const float* d_b, const int32_t* d_labels, int N,
+                                   int64_t V, int D, const float* d_row_scale, float scale, const float* d_lse, void* d_dw, int dw_ld,
+                                   float* d_db, void* d_workspace, size_t workspace_bytes, void* stream);
+
 /* ---- K7: loss head.  y = bias + y_w + y_v + y_d (DeepFM.py:174-175, terms may be NULL);
  * prob = sigmoid(y) (DeepFM.py:176); loss = mean xent (DeepFM.py:188, [TF-1.4] stable form);
  * d_dy = (prob - label)*inv_batch (inv_batch = 1/global batch).  d_loss_sum accumulates sum_b xent (caller zeroes, divides by B). */

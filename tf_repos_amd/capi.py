@@ -51,6 +51,17 @@ class Config(C.Structure):
     ]
 
 
+DTYPES = {"f32": 0, "bf16": 1}            # DCTR_TYPE_*: element types of the sequence operators
+MAX_REL_BUCKETS = 128
+
+
+class Attention(C.Structure):
+    """dctr_attention: the sizes of a ragged cross attention and the bucket boundaries of its relative bias."""
+    _fields_ = [("dtype", C.c_int32), ("n_seg", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("max_q", C.c_int32), ("max_k", C.c_int32), ("causal", C.c_int32), ("total_q", C.c_int64), ("total_k", C.c_int64),
+                ("scale", C.c_float), ("n_buckets", C.c_int32), ("boundaries", C.c_int32 * (MAX_REL_BUCKETS - 1))]
+
+
 class SlotSpec(C.Structure):
     _fields_ = [("ids_feature", C.c_char_p), ("vals_feature", C.c_char_p), ("fixed_len", C.c_int32)]
 
@@ -209,6 +220,14 @@ _SIGS["dctr_pairs_fc_bwd_weights_gate_split"] = ([_P, C.c_int, C.c_int, _P, _P, 
                                                   _P, C.c_size_t, _P], C.c_int)
 _SIGS["dctr_fc_bwd_data_gate_split"] = ([_P, C.c_int, _P, _P, _P, _P, _P, C.c_int, C.c_int64, C.c_int, C.c_int, _P, _P], C.c_int)
 _SIGS["dctr_set_stat_sync"] = ([_P, ALL_REDUCE_F32_FN, _P, C.c_int], C.c_int)
+_ATT_INS = [C.POINTER(Attention), _P, C.c_int, _P, C.c_int, _P, C.c_int, _P, _P, _P, _P, _P]
+_SIGS["dctr_cross_attention_workspace_bytes"] = ([C.POINTER(Attention), C.c_int, C.POINTER(C.c_int64)], C.c_int)
+_SIGS["dctr_cross_attention_fwd"] = (_ATT_INS + [_P, C.c_int, _P, _P, _P, C.c_size_t, _P], C.c_int)
+_SIGS["dctr_cross_attention_bwd"] = (_ATT_INS + [_P, C.c_int, _P, _P, C.c_int, _P, C.c_int, _P, C.c_int, _P, C.c_int, _P, _P, C.c_size_t, _P], C.c_int)
+_VS_INS = [C.c_int, _P, C.c_int, _P, C.c_int, _P, _P, C.c_int, C.c_int64, C.c_int, _P, C.c_float]
+_SIGS["dctr_vocab_softmax_workspace_bytes"] = ([C.c_int, C.c_int, C.c_int64, C.c_int, C.c_int, C.POINTER(C.c_int64)], C.c_int)
+_SIGS["dctr_vocab_softmax_fwd"] = (_VS_INS + [_P, _P, _P, C.c_int, _P, _P, C.c_size_t, _P], C.c_int)
+_SIGS["dctr_vocab_softmax_bwd_weights"] = (_VS_INS + [_P, _P, C.c_int, _P, _P, C.c_size_t, _P], C.c_int)
 
 DECLARED_SYMBOLS = tuple(_SIGS)
 

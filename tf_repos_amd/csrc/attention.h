@@ -1,0 +1,72 @@
+// Ragged multi-head attention of queries over another sequence's keys, with a learned bias per bucket of the distance between them:
+// what the entry points check once and the kernels of attention*.hip share.
+//
+// Segment b owns query rows [q_offsets[b], q_offsets[b+1]) and key rows [k_offsets[b], k_offsets[b+1]); query i of it stands at
+// position q_start[b] + i among the keys 0, 1, 2, ...  With h a query head and g = h / (heads / kv_heads) the key head it reads:
+//     s_ij = scale <q_i, k_j> + T[bucket(j - q_start[b] - i), h]         bucket(d) = number of boundaries <= d
+//     p_ij = softmax over the keys j that query i sees (key_keep[j] != 0; j <= q_start[b] + i when causal)
+//     o_i  = sum_j p_ij v_j                lse_i = log sum_j exp(s_ij)   (no key seen: o_i = 0, lse_i = -inf)
+// and for the gradient do of o:
+//     dv_j = sum_ih p_ij do_i     ds_ij = p_ij (<do_i, v_j> - <do_i, o_i>)      dT[u, h] = sum over the pairs of bucket u of ds_ij
+//     dq_i = scale sum_j ds_ij k_j                dk_j = scale sum_ih ds_ij q_i
+#pragma once
+#include <hip/hip_bf16.h>
+
+#include "common.h"
+
+namespace dctr {
+
+struct RelBuckets {                                     // passed by value: a captured graph keeps what it was captured with
+    int32_t n;                                          // 0: no bias
+    int32_t edge[DCTR_MAX_REL_BUCKETS - 1];             // ascending; bucket(d) = #{u : edge[u] <= d}
+};
+
+struct AttnView {
+    const void *q, *k, *v;
+    int64_t q_ld, k_ld, v_ld;                           // row strides in elements
+    const int32_t *q_off, *k_off, *q_start;             // q_start may be null (0)
+    const uint8_t* keep;                                // may be null (every key)
+    const float* bias;                                  // [n_buckets, heads]
+    int64_t total_q, total_k;
+    int32_t n_seg, heads, group, dim, max_q, max_k, causal;
+    float scale;
+    RelBuckets rel;
+};
+
+struct Segment { int64_t q0, k0; int nq, nk, start; };
+
+// A segment's rows, kept inside the arrays whatever the offsets say (the forward reports the ones that had to be cut, see flag_segment).
+__device__ __forceinline__ Segment load_segment(const AttnView& a, int b) {
+    Segment s;
+    auto cut = [](int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); };
+    s.q0 = cut(a.q_off[b], 0, a.total_q);
+    s.k0 = cut(a.k_off[b], 0, a.total_k);
+    s.nq = (int)cut(cut(a.q_off[b + 1], s.q0, a.total_q) - s.q0, 0, a.max_q);
+    s.nk = (int)cut(cut(a.k_off[b + 1], s.k0, a.total_k) - s.k0, 0, a.max_k);
+    s.start = a.q_start != nullptr ? (int)cut(a.q_start[b], -DCTR_MAX_POSITION, DCTR_MAX_POSITION) : 0;
+    return s;
+}
+
+__device__ __forceinline__ bool segment_is_bad(const AttnView& a, int b) {
+    const int q0 = a.q_off[b], q1 = a.q_off[b + 1], k0 = a.k_off[b], k1 = a.k_off[b + 1];
+    const int st = a.q_start != nullptr ? a.q_start[b] : 0;
+    return q0 < 0 || q1 < q0 || q1 > a.total_q || (int64_t)q1 - q0 > a.max_q || k0 < 0 || k1 < k0 || k1 > a.total_k ||
+           (int64_t)k1 - k0 > a.max_k || st < -DCTR_MAX_POSITION || st > DCTR_MAX_POSITION;
+}
+
+__device__ __forceinline__ int bucket_of(const RelBuckets& r, int d) {
+    int lo = 0, hi = r.n - 1;                           // number of edges <= d
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (r.edge[mid] <= d) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__hip_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float x) { return __float2bfloat16(x); }   // nearest even
+
+}  // namespace dctr
