@@ -10,9 +10,9 @@
 //     dv_j = sum_ih p_ij do_i     ds_ij = p_ij (<do_i, v_j> - <do_i, o_i>)      dT[u, h] = sum over the pairs of bucket u of ds_ij
 //     dq_i = scale sum_j ds_ij k_j                dk_j = scale sum_ih ds_ij q_i
 #pragma once
-#include <hip/hip_bf16.h>
+#include <algorithm>
 
-#include "common.h"
+#include "seq_mma.h"
 
 namespace dctr {
 
@@ -63,10 +63,33 @@ __device__ __forceinline__ int bucket_of(const RelBuckets& r, int d) {
     return lo;
 }
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__hip_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T from_f32(float x);
-template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <> __device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float x) { return __float2bfloat16(x); }   // nearest even
+// The bias of one tile of scores.  Distances below the first boundary all share bucket 0, those from the last boundary on the last bucket: only
+// a tile that reaches between the two ("near") looks values up, any other adds one number.  Tables hold log2(e) x the bias (the kernels'
+// exponents are base 2) and reach REL_PAD distances past either boundary, so that a near tile's lookups need no clamp.
+constexpr int REL_PAD = 128;                            // > keys + queries of a tile
+
+__device__ __forceinline__ bool near_tile(const RelBuckets& r, int dmin, int dmax) { return r.n > 1 && dmax >= r.edge[0] && dmin < r.edge[r.n - 2]; }
+// bucket of every distance of a tile that is not near
+__device__ __forceinline__ int far_bucket(const RelBuckets& r, int dmin) { return r.n > 1 && dmin >= r.edge[r.n - 2] ? r.n - 1 : 0; }
+
+// number of the r.n - 1 edges (staged in shared memory: kernel arguments are not indexed by lanes) that are <= d
+__device__ __forceinline__ int bucket_of(const int32_t* edges, int n, int d) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (edges[mid] <= d) lo = mid + 1; else hi = mid;
+    }
+    return lo;
+}
+
+inline int rel_reach(const dctr_attention* a) {         // entries of a table over distances
+    return a->n_buckets > 1 ? a->boundaries[a->n_buckets - 2] - a->boundaries[0] + 2 * REL_PAD : 0;
+}
+
+// ---- launchers (attention_fwd.hip, attention_bwd.hip): DP = 32, 64 or 128 by head_dim
+struct AttnSplit { int row_blocks, splits; };           // the forward's form for few query rows a key head (splits = 0: the other form)
+AttnSplit attn_split(const dctr_attention* a);
+int64_t attn_fwd_workspace(const dctr_attention* a);      // bytes
+int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st);
 
 }  // namespace dctr

@@ -42,46 +42,6 @@ __global__ void attn_check_kernel(AttnView a, int32_t* status) {
     if (b < a.n_seg && segment_is_bad(a, b)) { status[0] = 1; status[1] = b; }
 }
 
-// item = (segment, query row i < max_q, head)
-template <typename T>
-__global__ __launch_bounds__(64 * WAVES) void attn_fwd_kernel(AttnView a, T* out, int64_t out_ld, float* lse) {
-    const int64_t item = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, h = (int)(item % a.heads);
-    const int64_t r = item / a.heads;
-    const int i = (int)(r % a.max_q), b = (int)(r / a.max_q);
-    if (b >= a.n_seg) return;
-    const Segment s = load_segment(a, b);
-    if (i >= s.nq) return;
-    const T* qi = (const T*)a.q + (s.q0 + i) * a.q_ld + (int64_t)h * a.dim;
-    const T* K = (const T*)a.k + s.k0 * a.k_ld + (int64_t)(h / a.group) * a.dim;
-    const T* V = (const T*)a.v + s.k0 * a.v_ld + (int64_t)(h / a.group) * a.dim;
-    float m = -INFINITY, l = 0.f, acc0 = 0.f, acc1 = 0.f;
-    for (int j0 = 0; j0 < s.nk; j0 += 64) {
-        const int j = j0 + lane;
-        const bool on = key_seen(a, s, i, j);
-        const float z = on ? score(a, s, qi, K + j * a.k_ld, i, j, h) : -INFINITY;
-        const float top = fmaxf(m, wave_max(z)), base = top == -INFINITY ? 0.f : top;
-        const float p = expf(z - base), shrink = expf(m - base);
-        l = l * shrink + wave_sum(p);
-        acc0 *= shrink; acc1 *= shrink;
-        const uint64_t seen = __ballot(on);
-        for (int t = 0; t < 64; ++t) {
-            const float w = __shfl(p, t);
-            if (!(seen >> t & 1)) continue;
-            const T* v = V + (j0 + t) * a.v_ld;
-            if (lane < a.dim) acc0 = fmaf(w, to_f32(v[lane]), acc0);
-            if (64 + lane < a.dim) acc1 = fmaf(w, to_f32(v[64 + lane]), acc1);
-        }
-        m = top;
-    }
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
-    if (lse != nullptr && lane == 0) lse[(s.q0 + i) * a.heads + h] = m == -INFINITY ? -INFINITY : m + logf(l);
-    for (int d = lane; d < a.dim; d += 64) {
-        const float o = (d < 64 ? acc0 : acc1) * inv;
-        out[(s.q0 + i) * out_ld + (int64_t)h * a.dim + d] = from_f32<T>(o);
-    }
-}
-
 // dq, and this row's share of the bias gradient: part[(q0 + i), h, bucket]
 template <typename T>
 __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(AttnView a, const float* lse, const T* dout, int64_t dout_ld, T* dq, int64_t dq_ld, float* part) {
@@ -123,7 +83,7 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_q_kernel(AttnView a, cons
             if (u == 64 + lane) bin1 += w;
         }
     }
-    for (int d = lane; d < a.dim; d += 64) dq[row * dq_ld + hd + d] = from_f32<T>((d < 64 ? acc0 : acc1) * a.scale);
+    for (int d = lane; d < a.dim; d += 64) dq[row * dq_ld + hd + d] = (T)((d < 64 ? acc0 : acc1) * a.scale);
     if (part != nullptr)
         for (int u = lane; u < a.rel.n; u += 64) part[(row * a.heads + h) * a.rel.n + u] = u < 64 ? bin0 : bin1;
 }
@@ -192,8 +152,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_bwd_kv_kernel(AttnView a, con
         }
     }
     for (int d = lane; d < a.dim; d += 64) {
-        dk[row * dk_ld + gd + d] = from_f32<T>((d < 64 ? k0 : k1) * a.scale);
-        dv[row * dv_ld + gd + d] = from_f32<T>(d < 64 ? v0 : v1);
+        dk[row * dk_ld + gd + d] = (T)((d < 64 ? k0 : k1) * a.scale);
+        dv[row * dv_ld + gd + d] = (T)(d < 64 ? v0 : v1);
     }
 }
 
@@ -245,7 +205,7 @@ static int make_view(const dctr_attention* a, const void* q, int q_ld, const voi
 }
 
 static int64_t workspace_bytes(const dctr_attention* a, int backward) {
-    return backward ? 4 * a->total_q * a->heads * (int64_t)a->n_buckets : 0;
+    return backward ? 4 * a->total_q * a->heads * (int64_t)a->n_buckets : attn_fwd_workspace(a);
 }
 
 static int check_workspace(const dctr_attention* a, int backward, const void* ws, size_t bytes) {
@@ -259,16 +219,6 @@ static int check_workspace(const dctr_attention* a, int backward, const void* ws
 static int grid_of(int64_t blocks, unsigned* grid) {
     DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many rows for one launch");
     *grid = (unsigned)blocks;
-    return DCTR_OK;
-}
-
-template <typename T>
-static int run_fwd(const AttnView& a, void* out, int64_t out_ld, float* lse, hipStream_t st) {
-    unsigned grid;
-    DCTR_TRY(grid_of(((int64_t)a.n_seg * a.max_q * a.heads + WAVES - 1) / WAVES, &grid));
-    if (grid == 0) return DCTR_OK;
-    attn_fwd_kernel<T><<<grid, 64 * WAVES, 0, st>>>(a, (T*)out, out_ld, lse);
-    DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
 
@@ -322,7 +272,7 @@ int dctr_cross_attention_fwd(const dctr_attention* a, const void* d_q, int q_ld,
         DCTR_LAUNCH_CHECK();
     }
     if (a->total_q == 0) return DCTR_OK;
-    return f32 ? run_fwd<float>(v, d_out, out_ld, d_lse, st) : run_fwd<__hip_bfloat16>(v, d_out, out_ld, d_lse, st);
+    return attn_fwd(a, v, d_out, out_ld, d_lse, (float*)d_workspace, st);
 }
 
 int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld, const void* d_k, int k_ld, const void* d_v, int v_ld,
@@ -344,7 +294,7 @@ int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld,
     hipStream_t st = as_stream(stream);
     float* part = (float*)d_workspace;
     return elem == 4 ? run_bwd<float>(v, d_out, out_ld, d_lse, d_dout, dout_ld, d_dq, dq_ld, d_dk, dk_ld, d_dv, dv_ld, d_drel_bias, part, st)
-                     : run_bwd<__hip_bfloat16>(v, d_out, out_ld, d_lse, d_dout, dout_ld, d_dq, dq_ld, d_dk, dk_ld, d_dv, dv_ld, d_drel_bias,
+                     : run_bwd<__bf16>(v, d_out, out_ld, d_lse, d_dout, dout_ld, d_dq, dq_ld, d_dk, dk_ld, d_dv, dv_ld, d_drel_bias,
                                                part, st);
 }
 

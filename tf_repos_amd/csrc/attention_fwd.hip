@@ -1,0 +1,393 @@
+// Forward of the ragged cross attention (attention.h: formulas; seq_mma.h: the matrix blocks).  One pass over the keys with a running maximum
+// and sum: S^T = K Q^T puts a query's scores into one lane pair, so the softmax statistics are a number a lane and P feeds O^T += V^T P from
+// the registers it lies in.  Two forms:
+//   rows   4 waves of 32 queries of one head share 64-key tiles (double-buffered; the next tile's loads run under the products)
+//   split  32 rows = (query, head of the key head's group) pairs; every wave takes its own 32-key tiles, waves and, for long histories, blocks
+//          split the keys and join their (maximum, sum, weighted sum): few queries still use the whole chip, and shared key heads are read once
+#include <cmath>
+
+#include "attention.h"
+
+namespace dctr {
+
+// Running softmax of a wave's 32 columns: m (base 2) and this half's share of the sum, the weighted sum as O^T blocks.
+template <typename T, int DP>
+struct Softmax {
+    float m = -INFINITY, l = 0.f;
+    f32x16 acc[DP / 32] = {};
+
+    // Takes one 32 x NB*32 step's scores: t = fma(s, c, b), hidden entries -inf already where c = 1, b = 0.  Returns the weights in s.
+    // The running maximum moves only when a score passes it by 2^8: weights up to 256 lose nothing in either type, and most steps
+    // then skip the rescaling of the accumulators.
+    template <int NB>
+    __device__ __forceinline__ void step(f32x16 (&s)[NB], float c, float b) {
+        float top = s[0][0];
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[k][r]);
+        top = both_max(fmaf(top, c, b));
+        if (__any(top > m + 8.f)) {
+            const float mn = fmaxf(m, top), shrink = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            l *= shrink;
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k) acc[k] *= shrink;
+            m = mn;
+        }
+        const float off = b - (m == -INFINITY ? 0.f : m);
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[k][r] = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, off));
+                part[r & 3] += s[k][r];
+            }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    template <int NB>
+    __device__ __forceinline__ void weigh(const T* tile, const f32x16 (&p)[NB]) {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const auto w = Mma<T>::pack(p[k]);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(tile, 32 * k, 32 * d, w, acc[d]);
+        }
+    }
+};
+
+constexpr int ROWS_THREADS = 256, ROWS_KEYS = 64;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(ROWS_THREADS) void attn_rows_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int row_blocks) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int TILE = ROWS_KEYS * DP;
+    T *kt = reinterpret_cast<T*>(lds), *vt = kt + 2 * TILE;
+    float* lut = reinterpret_cast<float*>(vt + 2 * TILE);
+    int32_t* edges = reinterpret_cast<int32_t*>(kt);                    // (until the first tile is stored)
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int rb = blockIdx.x % row_blocks, h = blockIdx.x / row_blocks % a.heads, b = blockIdx.x / row_blocks / a.heads;
+    const Segment s = load_segment(a, b);
+    const int row0 = rb * 128;
+    if (row0 >= s.nq) return;
+    const int wrow = row0 + wave * 32, row = wrow + (lane & 31);
+    const int chunks = a.dim / Tile<T, DP>::PER;
+    const float scale = fabsf(a.scale) * LOG2E;
+
+    const int reach = a.rel.n > 1 ? a.rel.edge[a.rel.n - 2] - a.rel.edge[0] + 2 * REL_PAD : 0;
+    if (reach > 0) {
+        for (int u = tid; u + 1 < a.rel.n; u += ROWS_THREADS) edges[u] = a.rel.edge[u];
+        __syncthreads();
+        for (int u = tid; u < reach; u += ROWS_THREADS) lut[u] = LOG2E * a.bias[bucket_of(edges, a.rel.n, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
+        __syncthreads();
+    }
+
+    RowFrags<T, DP> q;
+    q.load((const T*)a.q + (s.q0 + row) * a.q_ld + (int64_t)h * a.dim, chunks, row < s.nq);
+    if (a.scale < 0.f) q.negate();                                      // the running maximum is taken before the scale
+
+    const T* K = (const T*)a.k + s.k0 * a.k_ld + (int64_t)(h / a.group) * a.dim;
+    const T* V = (const T*)a.v + s.k0 * a.v_ld + (int64_t)(h / a.group) * a.dim;
+    int keys = s.nk;                                                    // of this block
+    if (a.causal) keys = max(0, min(keys, s.start + min(row0 + 128, s.nq)));
+    const int tiles = (keys + ROWS_KEYS - 1) / ROWS_KEYS;
+    const bool busy = wrow < s.nq;
+    const int wend = a.causal ? s.start + min(wrow + 32, s.nq) : keys;  // keys from here on are hidden from the whole wave
+
+    Softmax<T, DP> o;
+    Staged<T, DP, ROWS_KEYS, ROWS_THREADS> ks, vs;
+    uint8_t kept = 1;
+    uint64_t bits = 0;
+    auto fetch = [&](int j0) {
+        ks.fetch(K, a.k_ld, j0, s.nk, chunks, tid);
+        vs.fetch(V, a.v_ld, j0, s.nk, chunks, tid);
+        kept = j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
+    };
+    auto store = [&](int buf) {
+        bits = __ballot(kept != 0);
+        ks.store(kt + buf * TILE, tid, bits);
+        vs.store(vt + buf * TILE, tid, bits);
+    };
+    if (tiles > 0) {
+        fetch(0);
+        store(0);
+    }
+    __syncthreads();
+    for (int t = 0; t < tiles; ++t) {
+        const int j0 = t * ROWS_KEYS;
+        const uint64_t now = bits;
+        if (t + 1 < tiles) fetch(j0 + ROWS_KEYS);
+        if (busy && j0 < wend) {
+            const T* kb = kt + (t & 1) * TILE;
+            f32x16 sc[2];
+            sc[0] = scores<T, DP>(kb, 0, q);
+            sc[1] = scores<T, DP>(kb, 32, q);
+            const int d0 = j0 - s.start - wrow;                         // distance of the tile's first key from the wave's first query
+            const bool near = near_tile(a.rel, d0 - 31, d0 + ROWS_KEYS - 1);
+            const float far = a.rel.n > 0 && !near ? LOG2E * a.bias[far_bucket(a.rel, d0 - 31) * a.heads + h] : 0.f;
+            const bool cut = a.causal && d0 + ROWS_KEYS - 1 > 0;
+            if (near || cut || now != ~0ull) {
+                uint64_t seen = now;
+                if (cut) {
+                    const int last = row + s.start - j0;                // last key of the tile that this query sees
+                    seen &= last < 0 ? 0ull : last >= 63 ? ~0ull : (2ull << last) - 1;
+                }
+                seen = lane_bits(seen);
+                const float* tab = lut + (near ? d0 - (lane & 31) + 4 * (lane >> 5) - a.rel.edge[0] + REL_PAD : 0);
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int at = 32 * k + reg_row(r);
+                        const float x = fmaf(sc[k][r], scale, near ? tab[at] : far);
+                        sc[k][r] = (seen >> at & 1) ? x : -INFINITY;
+                    }
+                o.template step<2>(sc, 1.f, 0.f);
+            } else {
+                o.template step<2>(sc, scale, far);
+            }
+            o.template weigh<2>(vt + (t & 1) * TILE, sc);
+        }
+        if (t + 1 < tiles) store((t + 1) & 1);
+        __syncthreads();
+    }
+    if (row >= s.nq) return;
+    const float l = both_sum(o.l), inv = l == 0.f ? 0.f : 1.f / l;             // (0: no key was seen)
+    if (lse != nullptr && lane < 32) lse[(s.q0 + row) * a.heads + h] = l == 0.f ? -INFINITY : LN2 * (o.m + log2f(l));
+    T* to = out + (s.q0 + row) * out_ld + (int64_t)h * a.dim + 4 * (lane >> 5);
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (32 * k + 8 * i < a.dim)
+                Mma<T>::store4(to + 32 * k + 8 * i, o.acc[k][4 * i] * inv, o.acc[k][4 * i + 1] * inv, o.acc[k][4 * i + 2] * inv, o.acc[k][4 * i + 3] * inv);
+}
+
+// ---- split form ----------------------------------------------------------------------------------------------------------------------
+constexpr int SPLIT_KEYS = 32;                                          // of a wave's tile
+// shared memory: 4 waves' K and V tiles, in whose place the waves' results meet (rows of DP + 4 floats: no two rows start at the same bank)
+template <typename T, int DP>
+struct SplitLds {
+    static constexpr size_t tiles = 4 * 2 * SPLIT_KEYS * DP * sizeof(T), join = 4 * 32 * (DP + 4) * sizeof(float);
+    static constexpr size_t first = tiles > join ? tiles : join, stats = 4 * 32 * 2 * sizeof(float);
+};
+
+// Joins n results (maximum, sum, weighted sum) of 32 rows: thread = (row, eighth of the columns).
+template <typename T, int DP, typename Get>
+__device__ __forceinline__ void join_rows(int n, int tid, Get get, float& m, float& l, float (&o)[DP / 8]) {
+    m = -INFINITY;
+    for (int w = 0; w < n; ++w) m = fmaxf(m, get(w, tid >> 3, -2));
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) o[d] = 0.f;
+    for (int w = 0; w < n; ++w) {
+        const float f = exp2f(get(w, tid >> 3, -2) - base);
+        l = fmaf(get(w, tid >> 3, -1), f, l);
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) o[d] = fmaf(get(w, tid >> 3, (tid & 7) * (DP / 8) + d), f, o[d]);
+    }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void finish_row(const AttnView& a, int64_t qrow, int h, int tid, float m, float l, const float (&o)[DP / 8], T* out,
+                                           int64_t out_ld, float* lse) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int d0 = (tid & 7) * (DP / 8);
+    if (lse != nullptr && (tid & 7) == 0) lse[qrow * a.heads + h] = l == 0.f ? -INFINITY : LN2 * (m + log2f(l));
+    T* to = out + qrow * out_ld + (int64_t)h * a.dim + d0;
+#pragma unroll
+    for (int d = 0; d < DP / 8; d += 4)
+        if (d0 + d < a.dim) Mma<T>::store4(to + d, o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
+}
+
+// part: [block item][split][32][DP + 2] (weighted sum, maximum, sum); not used when there is one split
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, float* part, AttnSplit cut) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    using L = SplitLds<T, DP>;
+    constexpr int TILE = SPLIT_KEYS * DP;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kv_heads = a.heads / a.group;
+    T* kt = reinterpret_cast<T*>(lds) + wave * 2 * TILE;
+    T* vt = kt + TILE;
+    float* join = reinterpret_cast<float*>(lds);
+    float* stats = reinterpret_cast<float*>(lds + L::first);
+    const int sp = blockIdx.x % cut.splits, item = blockIdx.x / cut.splits;
+    const int rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
+    const Segment s = load_segment(a, b);
+    const int rows = s.nq * a.group, r0 = rb * 32;
+    if (r0 >= rows) return;
+    const int r = r0 + (lane & 31), i = r / a.group, hg = r % a.group, h = g * a.group + hg;
+    const int chunks = a.dim / Tile<T, DP>::PER;
+    const float scale = fabsf(a.scale) * LOG2E;
+
+    // bias: bucket of a distance, then its value for the row's head (a block's rows have min(group, 32) different ones)
+    const int reach = a.rel.n > 1 ? a.rel.edge[a.rel.n - 2] - a.rel.edge[0] + 2 * REL_PAD : 0;
+    const int wide = min(a.group, 32), col = a.group <= 32 ? hg : r - r0;
+    float* table = stats + 4 * 32 * 2;                                  // [n_buckets][wide]
+    int32_t* edges = reinterpret_cast<int32_t*>(table + a.rel.n * wide);
+    int32_t* lut = edges + a.rel.n;
+    for (int u = tid; u < a.rel.n * wide; u += 256)
+        table[u] = LOG2E * a.bias[u / wide * a.heads + g * a.group + (a.group <= 32 ? u % wide : (r0 + u % wide) % a.group)];
+    if (reach > 0) {
+        for (int u = tid; u + 1 < a.rel.n; u += 256) edges[u] = a.rel.edge[u];
+        __syncthreads();
+        for (int u = tid; u < reach; u += 256) lut[u] = bucket_of(edges, a.rel.n, a.rel.edge[0] - REL_PAD + u) * wide;
+    }
+    if (a.rel.n > 0) __syncthreads();
+
+    RowFrags<T, DP> q;
+    q.load((const T*)a.q + (s.q0 + i) * a.q_ld + (int64_t)h * a.dim, chunks, r < rows);
+    if (a.scale < 0.f) q.negate();
+
+    const T* K = (const T*)a.k + s.k0 * a.k_ld + (int64_t)g * a.dim;
+    const T* V = (const T*)a.v + s.k0 * a.v_ld + (int64_t)g * a.dim;
+    const int i0 = r0 / a.group, i1 = min(r0 + 31, rows - 1) / a.group;
+    int keys = s.nk;
+    if (a.causal) keys = max(0, min(keys, s.start + i1 + 1));
+    const int tiles = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS, each = (tiles + cut.splits - 1) / cut.splits;
+    const int t1 = min(tiles, (sp + 1) * each);
+
+    Softmax<T, DP> o;
+    Staged<T, DP, SPLIT_KEYS, 64> ks, vs;
+    uint8_t kept = 0;
+    auto fetch = [&](int j0) {
+        ks.fetch(K, a.k_ld, j0, s.nk, chunks, lane);
+        vs.fetch(V, a.v_ld, j0, s.nk, chunks, lane);
+        kept = lane < SPLIT_KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
+    };
+    int t = sp * each + wave;
+    if (t < t1) fetch(t * SPLIT_KEYS);
+    for (; t < t1; t += 4) {
+        const int j0 = t * SPLIT_KEYS;
+        const uint64_t now = __ballot(kept != 0);
+        // the tile is this wave's own: its reads of the last step are behind these writes in program order
+        __builtin_amdgcn_wave_barrier();
+        ks.store(kt, lane, now);
+        vs.store(vt, lane, now);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (t + 4 < t1) fetch((t + 4) * SPLIT_KEYS);
+        f32x16 sc[1];
+        sc[0] = scores<T, DP>(kt, 0, q);
+        const int dmin = j0 - s.start - i1, dmax = j0 + SPLIT_KEYS - 1 - s.start - i0;
+        const bool near = near_tile(a.rel, dmin, dmax);
+        const float far = a.rel.n > 0 && !near ? table[far_bucket(a.rel, dmin) * wide + col] : 0.f;
+        const bool hide = a.causal && dmax > 0;
+        if (near || hide || now != 0xFFFFFFFFull) {
+            uint64_t seen = now;
+            if (hide) {
+                const int last = i + s.start - j0;
+                seen &= last < 0 ? 0ull : last >= 63 ? ~0ull : (2ull << last) - 1;
+            }
+            seen = lane_bits(seen);
+            const int32_t* at = lut + (near ? j0 - s.start - min(i, i1) + 4 * (lane >> 5) - a.rel.edge[0] + REL_PAD : 0);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = fmaf(sc[0][e], scale, near ? table[at[reg_row(e)] + col] : far);
+                sc[0][e] = (seen >> reg_row(e) & 1) ? x : -INFINITY;
+            }
+            o.template step<1>(sc, 1.f, 0.f);
+        } else {
+            o.template step<1>(sc, scale, far);
+        }
+        o.template weigh<1>(vt, sc);
+    }
+
+    __syncthreads();                                                    // every wave is done with the tiles
+    const float l = both_sum(o.l);
+    if (lane < 32) {
+        stats[(wave * 32 + lane) * 2] = o.m;
+        stats[(wave * 32 + lane) * 2 + 1] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<f32x4*>(join + (wave * 32 + (lane & 31)) * (DP + 4) + 32 * k + 8 * e + 4 * (lane >> 5)) =
+                f32x4{o.acc[k][4 * e], o.acc[k][4 * e + 1], o.acc[k][4 * e + 2], o.acc[k][4 * e + 3]};
+    __syncthreads();
+    float m, sum, w[DP / 8];
+    join_rows<T, DP>(4, tid, [&](int n, int row, int d) { return d == -2 ? stats[(n * 32 + row) * 2] : d == -1 ? stats[(n * 32 + row) * 2 + 1]
+                                                                                                    : join[(n * 32 + row) * (DP + 4) + d]; }, m, sum, w);
+    const int mine = r0 + (tid >> 3);
+    if (cut.splits == 1) {
+        if (mine < rows) finish_row<T, DP>(a, s.q0 + mine / a.group, g * a.group + mine % a.group, tid, m, sum, w, out, out_ld, lse);
+        return;
+    }
+    float* to = part + (((int64_t)item * cut.splits + sp) * 32 + (tid >> 3)) * (DP + 2);
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) to[(tid & 7) * (DP / 8) + d] = w[d];
+    if ((tid & 7) == 0) { to[DP] = m; to[DP + 1] = sum; }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnView a, T* out, int64_t out_ld, float* lse, const float* part, AttnSplit cut) {
+    const int tid = threadIdx.x, kv_heads = a.heads / a.group, item = blockIdx.x;
+    const int rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
+    const Segment s = load_segment(a, b);
+    const int mine = rb * 32 + (tid >> 3);
+    if (mine >= s.nq * a.group) return;
+    float m, sum, w[DP / 8];
+    join_rows<T, DP>(cut.splits, tid, [&](int n, int row, int d) { return part[(((int64_t)item * cut.splits + n) * 32 + row) * (DP + 2) + (d < 0 ? DP + 2 + d : d)]; },
+                     m, sum, w);
+    finish_row<T, DP>(a, s.q0 + mine / a.group, g * a.group + mine % a.group, tid, m, sum, w, out, out_ld, lse);
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------------
+static int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+
+AttnSplit attn_split(const dctr_attention* a) {
+    const int64_t rows = (int64_t)a->max_q * (a->heads / a->kv_heads);
+    if (rows > 128) return {0, 0};
+    const int64_t row_blocks = (rows + 31) / 32, items = row_blocks * a->kv_heads * a->n_seg;
+    if (items == 0) return {(int)row_blocks, 1};
+    const int64_t most = (a->max_k + 511) / 512, want = (2048 + items - 1) / items;
+    return {(int)row_blocks, (int)std::max<int64_t>(1, std::min(most, want))};
+}
+
+template <typename T, int DP>
+static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st) {
+    const AttnSplit cut = attn_split(a);
+    const int64_t table = a->n_buckets > 0 ? a->n_buckets * std::min<int64_t>(v.group, 32) + a->n_buckets + rel_reach(a) : 0;
+    if (cut.splits == 0) {
+        const int row_blocks = ceil_div(a->max_q, 128);
+        const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
+        DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
+        const size_t lds = 4 * ROWS_KEYS * DP * sizeof(T) + rel_reach(a) * sizeof(float);
+        attn_rows_kernel<T, DP><<<(unsigned)blocks, ROWS_THREADS, lds, st>>>(v, (T*)out, out_ld, lse, row_blocks);
+        DCTR_LAUNCH_CHECK();
+        return DCTR_OK;
+    }
+    const int64_t items = (int64_t)cut.row_blocks * a->kv_heads * a->n_seg;
+    DCTR_REQUIRE(items * cut.splits <= INT32_MAX, "attention: too many blocks for one launch");
+    if (items == 0) return DCTR_OK;
+    using L = SplitLds<T, DP>;
+    attn_split_kernel<T, DP><<<(unsigned)(items * cut.splits), 256, L::first + L::stats + table * sizeof(float), st>>>(v, (T*)out, out_ld, lse, ws, cut);
+    DCTR_LAUNCH_CHECK();
+    if (cut.splits > 1) {
+        attn_join_kernel<T, DP><<<(unsigned)items, 256, 0, st>>>(v, (T*)out, out_ld, lse, ws, cut);
+        DCTR_LAUNCH_CHECK();
+    }
+    return DCTR_OK;
+}
+
+template <typename T>
+static int by_width(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st) {
+    switch (padded(a->head_dim)) {
+        case 32: return launch_fwd<T, 32>(a, v, out, out_ld, lse, ws, st);
+        case 64: return launch_fwd<T, 64>(a, v, out, out_ld, lse, ws, st);
+        default: return launch_fwd<T, 128>(a, v, out, out_ld, lse, ws, st);
+    }
+}
+
+int64_t attn_fwd_workspace(const dctr_attention* a) {
+    const AttnSplit cut = attn_split(a);
+    return cut.splits > 1 ? (int64_t)cut.row_blocks * a->kv_heads * a->n_seg * cut.splits * 32 * (padded(a->head_dim) + 2) * (int64_t)sizeof(float) : 0;
+}
+
+int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st) {
+    return a->dtype == DCTR_TYPE_F32 ? by_width<float>(a, v, out, out_ld, lse, ws, st) : by_width<__bf16>(a, v, out, out_ld, lse, ws, st);
+}
+
+}  // namespace dctr

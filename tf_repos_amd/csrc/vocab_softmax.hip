@@ -5,7 +5,6 @@
 // The forward's sums leave the label out and add it at the end: with e the sum of the others, 1 - p_label = e / (e + exp(z_label - m)) has
 // no cancellation however sure the model is, nor has loss = log1p(e) where the label is the row's largest.
 #include <cmath>
-#include <hip/hip_bf16.h>
 
 #include "attention.h"
 
@@ -79,7 +78,7 @@ __global__ __launch_bounds__(64 * VS_WAVES) void vocab_fwd_kernel(VocabView a, f
     for (int c = 0; c < 4; ++c)
         if (c * 64 + lane < a.D)
             dx[n * dx_ld + c * 64 + lane] =
-                from_f32<T>(on ? c_n * (acc[c] - e * to_f32(((const T*)a.w + label * a.w_ld)[c * 64 + lane])) / all : 0.f);
+                (T)(on ? c_n * (acc[c] - e * to_f32(((const T*)a.w + label * a.w_ld)[c * 64 + lane])) / all : 0.f);
 }
 
 // one wave per vocabulary row
@@ -109,7 +108,7 @@ __global__ __launch_bounds__(64 * VS_WAVES) void vocab_dw_kernel(VocabView a, co
         }
     }
     for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < a.D) dw[v * dw_ld + c * 64 + lane] = from_f32<T>(acc[c]);
+        if (c * 64 + lane < a.D) dw[v * dw_ld + c * 64 + lane] = (T)(acc[c]);
     sum = vs_sum(sum);
     if (db != nullptr && lane == 0) db[v] = sum;
 }
@@ -176,7 +175,7 @@ int dctr_vocab_softmax_fwd(int dtype, const void* d_x, int x_ld, const void* d_w
     if (dtype == DCTR_TYPE_F32)
         vocab_fwd_kernel<float><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_loss, d_lse, (float*)d_dx, dx_ld, d_status);
     else
-        vocab_fwd_kernel<__hip_bfloat16><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_loss, d_lse, (__hip_bfloat16*)d_dx, dx_ld, d_status);
+        vocab_fwd_kernel<__bf16><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_loss, d_lse, (__bf16*)d_dx, dx_ld, d_status);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
@@ -193,7 +192,7 @@ int dctr_vocab_softmax_bwd_weights(int dtype, const void* d_x, int x_ld, const v
     if (dtype == DCTR_TYPE_F32)
         vocab_dw_kernel<float><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_lse, (float*)d_dw, dw_ld, d_db);
     else
-        vocab_dw_kernel<__hip_bfloat16><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_lse, (__hip_bfloat16*)d_dw, dw_ld, d_db);
+        vocab_dw_kernel<__bf16><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_lse, (__bf16*)d_dw, dw_ld, d_db);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
