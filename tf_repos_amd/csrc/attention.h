@@ -54,15 +54,6 @@ __device__ __forceinline__ bool segment_is_bad(const AttnView& a, int b) {
            (int64_t)k1 - k0 > a.max_k || st < -DCTR_MAX_POSITION || st > DCTR_MAX_POSITION;
 }
 
-__device__ __forceinline__ int bucket_of(const RelBuckets& r, int d) {
-    int lo = 0, hi = r.n - 1;                           // number of edges <= d
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (r.edge[mid] <= d) lo = mid + 1; else hi = mid;
-    }
-    return lo;
-}
-
 // The bias of one tile of scores.  Distances below the first boundary all share bucket 0, those from the last boundary on the last bucket: only
 // a tile that reaches between the two ("near") looks values up, any other adds one number.  Tables hold log2(e) x the bias (the kernels'
 // exponents are base 2) and reach REL_PAD distances past either boundary, so that a near tile's lookups need no clamp.
@@ -91,5 +82,17 @@ struct AttnSplit { int row_blocks, splits; };           // the forward's form fo
 AttnSplit attn_split(const dctr_attention* a);
 int64_t attn_fwd_workspace(const dctr_attention* a);      // bytes
 int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st);
+
+struct AttnGrads {
+    const void* out; int64_t out_ld;
+    const float* lse;
+    const void* dout; int64_t dout_ld;
+    void* dq; int64_t dq_ld;
+    void* dk; int64_t dk_ld;
+    void* dv; int64_t dv_ld;
+    float* dbias;                                       // may be null
+};
+int64_t attn_bwd_workspace(const dctr_attention* a);
+int attn_bwd(const dctr_attention* a, const AttnView& v, const AttnGrads& x, float* ws, hipStream_t st);
 
 }  // namespace dctr
