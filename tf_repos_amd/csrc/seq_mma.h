@@ -189,4 +189,50 @@ struct Staged {
 // bits of 64 consecutive tile rows as register r of 32-row block `blk` sees them: bit reg_row(r) + 32 blk of the shifted word
 __device__ __forceinline__ uint64_t lane_bits(uint64_t rows) { return rows >> (4 * ((threadIdx.x >> 5) & 1)); }
 
+// Running softmax of a wave's 32 columns: m (base 2) and this half's share of the sum, the weighted sum as O^T blocks.
+template <typename T, int DP>
+struct Softmax {
+    float m = -INFINITY, l = 0.f;
+    f32x16 acc[DP / 32] = {};
+
+    // Takes one 32 x NB*32 step's scores: t = fma(s, c, b), hidden entries -inf already where c = 1, b = 0.  Returns the weights in s.
+    // The running maximum moves only when a score passes it by 2^8: weights up to 256 lose nothing in either type, and most steps
+    // then skip the rescaling of the accumulators.
+    template <int NB>
+    __device__ __forceinline__ void step(f32x16 (&s)[NB], float c, float b) {
+        float top = s[0][0];
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[k][r]);
+        top = both_max(fmaf(top, c, b));
+        if (__any(top > m + 8.f)) {
+            const float mn = fmaxf(m, top), shrink = exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            l *= shrink;
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k) acc[k] *= shrink;
+            m = mn;
+        }
+        const float off = b - (m == -INFINITY ? 0.f : m);
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[k][r] = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, off));
+                part[r & 3] += s[k][r];
+            }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    template <int NB>
+    __device__ __forceinline__ void weigh(const T* tile, const f32x16 (&p)[NB]) {
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+            const auto w = Mma<T>::pack(p[k]);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(tile, 32 * k, 32 * d, w, acc[d]);
+        }
+    }
+};
+
 }  // namespace dctr

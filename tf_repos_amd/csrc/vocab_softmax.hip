@@ -1,12 +1,14 @@
-// Softmax cross entropy over a large vocabulary from the hidden rows and the vocabulary's table: the [N, V] logits exist 64 at a time.
+// Softmax cross entropy over a large vocabulary from the hidden rows and the vocabulary's table: the [N, V] logits exist a tile at a time, in
+// registers (seq_mma.h).
 //     z_nv = <x_n, w_v> + b_v        lse_n = log sum_v exp(z_nv)        loss_n = lse_n - z_n,label(n)
 //     g_nv = c_n (exp(z_nv - lse_n) - [v = label(n)]),  c_n = scale row_scale_n (0 for a row without a label)
 //     dx_n = sum_v g_nv w_v          dw_v = sum_n g_nv x_n              db_v = sum_n g_nv
 // The forward's sums leave the label out and add it at the end: with e the sum of the others, 1 - p_label = e / (e + exp(z_label - m)) has
 // no cancellation however sure the model is, nor has loss = log1p(e) where the label is the row's largest.
+#include <algorithm>
 #include <cmath>
 
-#include "attention.h"
+#include "seq_mma.h"
 
 namespace dctr {
 
@@ -20,100 +22,414 @@ struct VocabView {
     int32_t N, D;
 };
 
-constexpr int VS_WAVES = 4;
+constexpr int VS_THREADS = 256;
 
-template <typename T>
-__device__ __forceinline__ float logit(const VocabView& a, const T* x, int64_t v) {
-    const T* w = (const T*)a.w + v * a.w_ld;
-    float s = 0.f;
-    for (int d = 0; d < a.D; ++d) s = fmaf(to_f32(x[d]), to_f32(w[d]), s);
-    return a.b != nullptr ? s + a.b[v] : s;
-}
-
-__device__ __forceinline__ float vs_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
-}
-__device__ __forceinline__ float vs_sum(float x) {
+__device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
     return x;
 }
 
-// one wave per row
-template <typename T>
-__global__ __launch_bounds__(64 * VS_WAVES) void vocab_fwd_kernel(VocabView a, float* loss, float* lse, T* dx, int64_t dx_ld, int32_t* status) {
-    const int n = blockIdx.x * VS_WAVES + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+// ---- forward: the same pass as an attention whose keys and values are both the table --------------------------------------------------
+// What a split of the vocabulary leaves for every row, the label's column left out: maximum (base 2), sum, weighted sum of table rows.
+struct VocabParts {
+    float *m, *e, *acc;             // [splits][N], [splits][N], [splits][N][DP]
+    int splits;
+    int64_t each;                   // vocabulary rows of a split, a multiple of the tile
+};
+
+template <typename T, int DP>
+struct VocabTile { static constexpr int ROWS = sizeof(T) * DP <= 512 ? 64 : 32, NB = ROWS / 32, SIZE = ROWS * DP; };
+
+// One step of a wave's 32 rows against NB * 32 table rows from v0 on: scores, bias, hidden columns (behind the table, the row's label).
+// `bt`: log2(e) b of the tile's rows, in shared memory, or null.
+template <typename T, int DP, int NB, bool DX>
+__device__ __forceinline__ void vocab_step(const T* tile, const float* bt, const RowFrags<T, DP>& x, int64_t v0, int64_t v1, int64_t label,
+                                           Softmax<T, DP>& o) {
+    const int half = (threadIdx.x >> 5) & 1;
+    f32x16 s[NB];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) s[k] = scores<T, DP>(tile, 32 * k, x);
+    const int64_t own = label - v0;
+    const bool hide = v0 + 32 * NB > v1 || __any(own >= 0 && own < 32 * NB);
+    if (bt != nullptr || hide) {
+        uint64_t seen = v1 - v0 >= 64 ? ~0ull : (1ull << (v1 - v0)) - 1;
+        if (own >= 0 && own < 64) seen &= ~(1ull << own);
+        seen = lane_bits(seen);
+#pragma unroll
+        for (int k = 0; k < NB; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 add = bt != nullptr ? *reinterpret_cast<const f32x4*>(bt + 32 * k + 8 * i + 4 * half) : f32x4{};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[k][4 * i + j] = fmaf(s[k][4 * i + j], LOG2E, add[j]);
+            }
+        if (hide) {
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[k][r] = (seen >> (32 * k + reg_row(r)) & 1) ? s[k][r] : -INFINITY;
+        }
+        o.template step<NB>(s, 1.f, 0.f);
+    } else {
+        o.template step<NB>(s, LOG2E, 0.f);
+    }
+    if (DX) o.template weigh<NB>(tile, s);
+}
+
+template <typename T, int DP, bool DX>
+__device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, int64_t n, bool on, const Softmax<T, DP>& o) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const float e = both_sum(o.l);
+    if (!on) return;
+    const int64_t at = (int64_t)sp * N + n;
+    if (half == 0) { p.m[at] = o.m; p.e[at] = e; }
+    if (DX)
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(p.acc + at * DP + 32 * k + 8 * i + 4 * half) =
+                    f32x4{o.acc[k][4 * i], o.acc[k][4 * i + 1], o.acc[k][4 * i + 2], o.acc[k][4 * i + 3]};
+}
+
+// 4 waves of 32 rows share the table's tiles, double-buffered
+template <typename T, int DP, bool DX>
+__global__ __launch_bounds__(VS_THREADS) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    using Ti = VocabTile<T, DP>;
+    T* tiles = reinterpret_cast<T*>(lds);
+    float* bias = reinterpret_cast<float*>(tiles + 2 * Ti::SIZE);                       // [2][ROWS]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int rb = blockIdx.x % row_blocks, sp = blockIdx.x / row_blocks;
+    const int64_t n = (int64_t)rb * 128 + wave * 32 + (lane & 31), v0 = sp * p.each, v1 = min(a.V, v0 + p.each);
+    const int chunks = a.D / Tile<T, DP>::PER;
+    const bool on = n < a.N, busy = rb * 128 + wave * 32 < a.N;
+    RowFrags<T, DP> x;
+    x.load((const T*)a.x + n * a.x_ld, chunks, on);
+    const int64_t label = on ? a.labels[n] : -1;
+    Softmax<T, DP> o;
+    Staged<T, DP, Ti::ROWS, VS_THREADS> ws;
+    float bv = 0.f;
+    auto fetch = [&](int64_t v) {
+        ws.fetch((const T*)a.w, a.w_ld, v, v1, chunks, tid);
+        if (a.b != nullptr && tid < Ti::ROWS) bv = v + tid < v1 ? LOG2E * a.b[v + tid] : 0.f;
+    };
+    auto store = [&](int buf) {
+        ws.store(tiles + buf * Ti::SIZE, tid);
+        if (a.b != nullptr && tid < Ti::ROWS) bias[buf * Ti::ROWS + tid] = bv;
+    };
+    if (v0 < v1) {
+        fetch(v0);
+        store(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int64_t v = v0; v < v1; v += Ti::ROWS, buf ^= 1) {
+        const bool more = v + Ti::ROWS < v1;
+        if (more) fetch(v + Ti::ROWS);
+        if (busy) vocab_step<T, DP, Ti::NB, DX>(tiles + buf * Ti::SIZE, a.b != nullptr ? bias + buf * Ti::ROWS : nullptr, x, v, v1, label, o);
+        if (more) store(buf ^ 1);
+        __syncthreads();
+    }
+    write_parts<T, DP, DX>(p, sp, a.N, n, on, o);
+}
+
+// up to 32 rows: every wave is a split of its own with tiles of its own
+template <typename T, int DP, bool DX>
+__global__ __launch_bounds__(VS_THREADS) void vocab_few_kernel(VocabView a, VocabParts p) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sp = blockIdx.x * 4 + wave;
+    T* tile = reinterpret_cast<T*>(lds) + wave * 32 * DP;
+    float* bias = reinterpret_cast<float*>(reinterpret_cast<T*>(lds) + 4 * 32 * DP) + wave * 32;
+    if (sp >= p.splits) return;
+    const int64_t n = lane & 31, v0 = sp * p.each, v1 = min(a.V, v0 + p.each);
+    const int chunks = a.D / Tile<T, DP>::PER;
+    const bool on = n < a.N;
+    RowFrags<T, DP> x;
+    x.load((const T*)a.x + n * a.x_ld, chunks, on);
+    const int64_t label = on ? a.labels[n] : -1;
+    Softmax<T, DP> o;
+    Staged<T, DP, 32, 64> ws;
+    float bv = 0.f;
+    auto fetch = [&](int64_t v) {
+        ws.fetch((const T*)a.w, a.w_ld, v, v1, chunks, lane);
+        if (a.b != nullptr && lane < 32) bv = v + lane < v1 ? LOG2E * a.b[v + lane] : 0.f;
+    };
+    if (v0 < v1) fetch(v0);
+    for (int64_t v = v0; v < v1; v += 32) {
+        __builtin_amdgcn_wave_barrier();
+        ws.store(tile, lane);
+        if (a.b != nullptr && lane < 32) bias[lane] = bv;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (v + 32 < v1) fetch(v + 32);
+        vocab_step<T, DP, 1, DX>(tile, a.b != nullptr ? bias : nullptr, x, v, v1, label, o);
+    }
+    write_parts<T, DP, DX>(p, sp, a.N, n, on, o);
+}
+
+// Joins the splits and adds the label's column: one wave a row.
+template <typename T, int DP, bool DX>
+__global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, VocabParts p, float* loss, float* lse, T* dx, int64_t dx_ld, int32_t* status) {
+    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
     if (n >= a.N) return;
-    const T* x = (const T*)a.x + n * a.x_ld;
     const int label = a.labels[n];
     const bool on = label >= 0 && label < a.V;
     if (label >= a.V && lane == 0 && status != nullptr) { status[0] = 1; status[1] = label; }
-    float m = on ? logit<T>(a, x, label) : -INFINITY, e = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const float mine = m;
-    for (int64_t v0 = 0; v0 < a.V; v0 += 64) {
-        const int64_t v = v0 + lane;
-        const float z = v < a.V && v != label ? logit<T>(a, x, v) : -INFINITY;
-        const float top = fmaxf(m, vs_max(z)), base = top == -INFINITY ? 0.f : top;
-        const float p = expf(z - base), shrink = expf(m - base);
-        e = e * shrink + vs_sum(p);
-        m = top;
-        if (dx == nullptr) continue;
-        for (int c = 0; c < 4; ++c) acc[c] *= shrink;
-        for (int t = 0; t < 64 && v0 + t < a.V; ++t) {
-            const float q = __shfl(p, t);
-            const T* w = (const T*)a.w + (v0 + t) * a.w_ld;
-            for (int c = 0; c < 4; ++c)
-                if (c * 64 + lane < a.D) acc[c] = fmaf(q, to_f32(w[c * 64 + lane]), acc[c]);
-        }
+    const T* x = (const T*)a.x + n * a.x_ld;
+    const T* w = (const T*)a.w + (on ? label : 0) * a.w_ld;
+    float mine = -INFINITY;                                             // the label's logit, base 2
+    if (on) {
+        float z = 0.f;
+        for (int d = lane; d < a.D; d += 64) z = fmaf(to_f32(x[d]), to_f32(w[d]), z);
+        z = wave_sum(z);
+        mine = LOG2E * (a.b != nullptr ? z + a.b[label] : z);
     }
-    const float base = m == -INFINITY ? 0.f : m, all = e + (on ? expf(mine - base) : 0.f);
+    float m = mine;
+    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.m[(int64_t)s * a.N + n]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    const float base = m == -INFINITY ? 0.f : m;
+    float e = 0.f;
+    for (int s = lane; s < p.splits; s += 64) e = fmaf(p.e[(int64_t)s * a.N + n], exp2f(p.m[(int64_t)s * a.N + n] - base), e);
+    e = wave_sum(e);
+    const float all = e + (on ? exp2f(mine - base) : 0.f);
     if (lane == 0) {
-        if (lse != nullptr) lse[n] = base + logf(all);
-        loss[n] = !on ? 0.f : mine == m ? log1pf(e) : (base - mine) + logf(all);
+        if (lse != nullptr) lse[n] = LN2 * base + logf(all);
+        loss[n] = !on ? 0.f : mine == m ? log1pf(e) : LN2 * (base - mine) + logf(all);
     }
-    if (dx == nullptr) return;
-    const float c_n = on ? a.scale * (a.row_scale != nullptr ? a.row_scale[n] : 1.f) : 0.f;
-    for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < a.D)
-            dx[n * dx_ld + c * 64 + lane] =
-                (T)(on ? c_n * (acc[c] - e * to_f32(((const T*)a.w + label * a.w_ld)[c * 64 + lane])) / all : 0.f);
+    if (!DX) return;
+    const float c = on ? a.scale * (a.row_scale != nullptr ? a.row_scale[n] : 1.f) : 0.f;
+    constexpr int PER = DP > 64 ? DP / 64 : 1;
+    if (lane * PER >= a.D) return;
+    float acc[PER] = {};
+    if (on)
+        for (int s = 0; s < p.splits; ++s) {
+            const float f = exp2f(p.m[(int64_t)s * a.N + n] - base);
+#pragma unroll
+            for (int d = 0; d < PER; ++d) acc[d] = fmaf(p.acc[((int64_t)s * a.N + n) * DP + lane * PER + d], f, acc[d]);
+        }
+#pragma unroll
+    for (int d = 0; d < PER; ++d)
+        if (lane * PER + d < a.D) dx[n * dx_ld + lane * PER + d] = (T)(on ? c * (acc[d] - e * to_f32(w[lane * PER + d])) / all : 0.f);
 }
 
-// one wave per vocabulary row
-template <typename T>
-__global__ __launch_bounds__(64 * VS_WAVES) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db) {
-    const int64_t v = (int64_t)blockIdx.x * VS_WAVES + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
+// ---- dw, db: 32 table rows a wave, over the rows of x ---------------------------------------------------------------------------------
+// With more than one split (a short vocabulary): part [splits][V][DP], part_b [splits][V], joined by vocab_dw_join_kernel.
+template <typename T, int DP>
+__global__ __launch_bounds__(VS_THREADS) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
+                                                              int splits, int each, int table_blocks) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    using Ti = VocabTile<T, DP>;
+    T* tiles = reinterpret_cast<T*>(lds);
+    float* stats = reinterpret_cast<float*>(tiles + 2 * Ti::SIZE);                      // [2][-log2(e) lse, row scale, label][ROWS]
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int tb = blockIdx.x % table_blocks, sp = blockIdx.x / table_blocks;
+    const int64_t w0 = (int64_t)tb * 128 + wave * 32, v = w0 + (lane & 31);
+    const int chunks = a.D / Tile<T, DP>::PER, n0 = sp * each, n1 = min(a.N, n0 + each);
+    const bool on = v < a.V;
+    RowFrags<T, DP> w;
+    w.load((const T*)a.w + v * a.w_ld, chunks, on);
+    const float bv = on && a.b != nullptr ? LOG2E * a.b[v] : 0.f;
+    f32x16 acc[DP / 32] = {};
+    float sum = 0.f;
+    Staged<T, DP, Ti::ROWS, VS_THREADS> xs;
+    float lv = 0.f, cv = 0.f;
+    int label = -1;
+    auto fetch = [&](int n) {
+        xs.fetch((const T*)a.x, a.x_ld, n, n1, chunks, tid);
+        const int r = n + lane;                                                         // (every wave: the rows' bits)
+        label = lane < Ti::ROWS && r < n1 ? a.labels[r] : -1;
+        if (label >= a.V) label = -1;
+        lv = label >= 0 ? -LOG2E * lse[r] : -INFINITY;                                  // no label: p = 2^-inf = 0
+        if (a.row_scale != nullptr) cv = label >= 0 ? a.row_scale[r] : 0.f;
+    };
+    auto store = [&](int buf) {
+        xs.store(tiles + buf * Ti::SIZE, tid, __ballot(label >= 0));
+        if (wave == 0 && lane < Ti::ROWS) {
+            float* st = stats + buf * 3 * Ti::ROWS + lane;
+            st[0] = lv;
+            st[Ti::ROWS] = cv;
+            reinterpret_cast<int32_t*>(st)[2 * Ti::ROWS] = label;
+        }
+    };
+    if (n0 < n1) {
+        fetch(n0);
+        store(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int n = n0; n < n1; n += Ti::ROWS, buf ^= 1) {
+        const bool more = n + Ti::ROWS < n1;
+        if (more) fetch(n + Ti::ROWS);
+        const T* xt = tiles + buf * Ti::SIZE;
+        const float* st = stats + buf * 3 * Ti::ROWS;
+        const int32_t* lt = reinterpret_cast<const int32_t*>(st) + 2 * Ti::ROWS;
+        const int64_t there = lane < Ti::ROWS ? (int64_t)lt[lane] - w0 : -1;
+        const bool hot = __any(there >= 0 && there < 32);                               // a row's label is one of the wave's table rows
+#pragma unroll
+        for (int k = 0; k < Ti::NB; ++k) {
+            f32x16 p = scores<T, DP>(xt, 32 * k, w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 ml = *reinterpret_cast<const f32x4*>(st + 32 * k + 8 * i + 4 * half);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(p[4 * i + j], LOG2E, ml[j] + bv));
+            }
+            if (hot) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] -= lt[32 * k + reg_row(r) + 4 * half] == v ? 1.f : 0.f;
+            }
+            if (a.row_scale != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 c = *reinterpret_cast<const f32x4*>(st + Ti::ROWS + 32 * k + 8 * i + 4 * half);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[4 * i + j] *= c[j];
+                }
+            }
+            if (db != nullptr) {
+                float part4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < 16; ++r) part4[r & 3] += p[r];
+                sum += (part4[0] + part4[1]) + (part4[2] + part4[3]);
+            }
+            const auto g = Mma<T>::pack(p);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(xt, 32 * k, 32 * d, g, acc[d]);
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
+    }
+    sum = both_sum(sum);
+    if (!on) return;
+    if (splits > 1) {
+        const int64_t at = (int64_t)sp * a.V + v;
+        if (db != nullptr && half == 0) part_b[at] = sum;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(part + at * DP + 32 * d + 8 * i + 4 * half) =
+                    f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+        return;
+    }
+    if (db != nullptr && half == 0) db[v] = a.scale * sum;
+    T* to = dw + v * dw_ld + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (32 * d + 8 * i < a.D)
+                Mma<T>::store4(to + 32 * d + 8 * i, a.scale * acc[d][4 * i], a.scale * acc[d][4 * i + 1], a.scale * acc[d][4 * i + 2],
+                               a.scale * acc[d][4 * i + 3]);
+}
+
+// thread = 4 columns of a table row
+template <typename T, int DP>
+__global__ __launch_bounds__(VS_THREADS) void vocab_dw_join_kernel(VocabView a, T* dw, int64_t dw_ld, float* db, const float* part, const float* part_b,
+                                                                   int splits) {
+    const int64_t at = (int64_t)blockIdx.x * VS_THREADS + threadIdx.x, v = at / (DP / 4);
+    const int d = (int)(at % (DP / 4)) * 4;
     if (v >= a.V) return;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-    for (int n0 = 0; n0 < a.N; n0 += 64) {
-        const int n = n0 + lane;
-        const int label = n < a.N ? a.labels[n] : -1;
-        const bool on = label >= 0 && label < a.V;
-        float g = 0.f;
-        if (on) {
-            const float t = logit<T>(a, (const T*)a.x + n * a.x_ld, v) - lse[n];
-            g = a.scale * (a.row_scale != nullptr ? a.row_scale[n] : 1.f) * (v == label ? expm1f(t) : expf(t));
-        }
-        sum += g;
-        const uint64_t rows = __ballot(on);
-        for (int t = 0; t < 64; ++t) {
-            const float q = __shfl(g, t);
-            if (!(rows >> t & 1)) continue;
-            const T* x = (const T*)a.x + (n0 + t) * a.x_ld;
-            for (int c = 0; c < 4; ++c)
-                if (c * 64 + lane < a.D) acc[c] = fmaf(q, to_f32(x[c * 64 + lane]), acc[c]);
-        }
+    if (db != nullptr && d == 0) {
+        float x = 0.f;
+        for (int s = 0; s < splits; ++s) x += part_b[(int64_t)s * a.V + v];
+        db[v] = a.scale * x;
     }
-    for (int c = 0; c < 4; ++c)
-        if (c * 64 + lane < a.D) dw[v * dw_ld + c * 64 + lane] = (T)(acc[c]);
-    sum = vs_sum(sum);
-    if (db != nullptr && lane == 0) db[v] = sum;
+    if (d >= a.D) return;
+    f32x4 x = {};
+    for (int s = 0; s < splits; ++s) x += *reinterpret_cast<const f32x4*>(part + ((int64_t)s * a.V + v) * DP + d);
+    x *= a.scale;
+    Mma<T>::store4(dw + v * dw_ld + d, x[0], x[1], x[2], x[3]);
 }
 
-// ---- host side ---------------------------------------------------------------------------------------------------------------------
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+static int padded(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+
+struct VocabPlan { bool few; int row_blocks, splits; int64_t each; };
+// Splits of the vocabulary: two blocks a compute unit, no split below 256 rows of the table.
+static VocabPlan plan_fwd(int N, int64_t V) {
+    VocabPlan p;
+    p.few = N <= 32;
+    p.row_blocks = p.few ? 1 : ceil_div(N, 128);
+    const int64_t want = p.few ? 2048 : (512 + p.row_blocks - 1) / p.row_blocks, most = p.few ? (V + 63) / 64 : (V + 255) / 256;
+    p.each = round_up((V + std::min(want, most) - 1) / std::min(want, most), p.few ? 32 : 64);
+    p.splits = (int)((V + p.each - 1) / p.each);
+    return p;
+}
+struct VocabWPlan { int table_blocks, splits, each; };
+// Splits of the rows: a vocabulary of fewer than 512 blocks of 128 rows leaves compute units idle.
+static VocabWPlan plan_dw(int N, int64_t V) {
+    VocabWPlan p;
+    p.table_blocks = ceil_div(V, 128);
+    const int64_t want = std::max<int64_t>(1, 512 / p.table_blocks), most = std::max(1, ceil_div(N, 256));
+    const int64_t cut = std::min(want, most);
+    p.each = (int)std::max<int64_t>(64, round_up((N + cut - 1) / cut, 64));
+    p.splits = std::max(1, ceil_div(N, p.each));
+    return p;
+}
+
+static int64_t workspace_bytes(int N, int64_t V, int D, int train) {
+    const VocabPlan f = plan_fwd(N, V);
+    const int64_t rows = (int64_t)f.splits * N, stats = round_up(2 * rows, 4);
+    int64_t floats = stats + (train ? rows * padded(D) : 0);
+    if (train) {
+        const VocabWPlan w = plan_dw(N, V);
+        if (w.splits > 1) floats = std::max(floats, (int64_t)w.splits * V * (padded(D) + 1));
+    }
+    return floats * (int64_t)sizeof(float);
+}
+
+template <typename T, int DP, bool DX>
+static int launch_fwd(const VocabView& a, float* loss, float* lse, void* dx, int64_t dx_ld, int32_t* status, float* ws, hipStream_t st) {
+    const VocabPlan f = plan_fwd(a.N, a.V);
+    const int64_t rows = (int64_t)f.splits * a.N;
+    const VocabParts p{ws, ws + rows, ws + round_up(2 * rows, 4), f.splits, f.each};
+    DCTR_REQUIRE((int64_t)f.row_blocks * f.splits <= INT32_MAX, "vocab softmax: too many blocks for one launch");
+    if (f.few)
+        vocab_few_kernel<T, DP, DX><<<ceil_div(f.splits, 4), VS_THREADS, 4 * (32 * DP * sizeof(T) + 32 * sizeof(float)), st>>>(a, p);
+    else
+        vocab_rows_kernel<T, DP, DX><<<(unsigned)(f.row_blocks * f.splits), VS_THREADS,
+                                       2 * (VocabTile<T, DP>::SIZE * sizeof(T) + VocabTile<T, DP>::ROWS * sizeof(float)), st>>>(a, p, f.row_blocks);
+    DCTR_LAUNCH_CHECK();
+    vocab_join_kernel<T, DP, DX><<<ceil_div(a.N, 4), VS_THREADS, 0, st>>>(a, p, loss, lse, (T*)dx, dx_ld, status);
+    DCTR_LAUNCH_CHECK();
+    return DCTR_OK;
+}
+
+template <typename T, int DP>
+static int launch_dw(const VocabView& a, const float* lse, void* dw, int64_t dw_ld, float* db, float* ws, hipStream_t st) {
+    const VocabWPlan w = plan_dw(a.N, a.V);
+    float *part = ws, *part_b = ws + (int64_t)w.splits * a.V * DP;
+    DCTR_REQUIRE((int64_t)w.table_blocks * w.splits <= INT32_MAX, "vocab softmax: too many blocks for one launch");
+    const size_t lds = 2 * (VocabTile<T, DP>::SIZE * sizeof(T) + 3 * VocabTile<T, DP>::ROWS * sizeof(float));
+    vocab_dw_kernel<T, DP><<<(unsigned)(w.table_blocks * w.splits), VS_THREADS, lds, st>>>(a, lse, (T*)dw, dw_ld, db, part, part_b, w.splits, w.each,
+                                                                                           w.table_blocks);
+    DCTR_LAUNCH_CHECK();
+    if (w.splits > 1) {
+        vocab_dw_join_kernel<T, DP><<<ceil_div(a.V * (DP / 4), VS_THREADS), VS_THREADS, 0, st>>>(a, (T*)dw, dw_ld, db, part, part_b, w.splits);
+        DCTR_LAUNCH_CHECK();
+    }
+    return DCTR_OK;
+}
+
+template <typename T, int DP>
+static int fwd(const VocabView& a, float* loss, float* lse, void* dx, int64_t dx_ld, int32_t* status, float* ws, hipStream_t st) {
+    return dx != nullptr ? launch_fwd<T, DP, true>(a, loss, lse, dx, dx_ld, status, ws, st)
+                         : launch_fwd<T, DP, false>(a, loss, lse, dx, dx_ld, status, ws, st);
+}
+
+#define VOCAB_BY_WIDTH(T, D, FN, ...)                     \
+    switch (padded(D)) {                                  \
+        case 32: return FN<T, 32>(__VA_ARGS__);           \
+        case 64: return FN<T, 64>(__VA_ARGS__);           \
+        case 128: return FN<T, 128>(__VA_ARGS__);         \
+        default: return FN<T, 256>(__VA_ARGS__);          \
+    }
+
 static int check_sizes(int dtype, int N, int64_t V, int D) {
     DCTR_REQUIRE(dtype == DCTR_TYPE_F32 || dtype == DCTR_TYPE_BF16, "vocab softmax: unknown element type %d", dtype);
     DCTR_REQUIRE(N >= 0, "vocab softmax: %d rows", N);
@@ -128,8 +444,6 @@ static int check_rows(const char* what, const void* p, int ld, int D, int elem) 
     DCTR_REQUIRE(ld >= D, "vocab softmax: row stride %d of %s is below %d", ld, what, D);
     return DCTR_OK;
 }
-
-static int64_t workspace_bytes(int, int64_t, int, int) { return 0; }
 
 static int make_view(int dtype, const void* x, int x_ld, const void* w, int w_ld, const float* b, const int32_t* labels, int N, int64_t V, int D,
                      const float* row_scale, float scale, int train, const void* ws, size_t ws_bytes, VocabView* view) {
@@ -171,13 +485,9 @@ int dctr_vocab_softmax_fwd(int dtype, const void* d_x, int x_ld, const void* d_w
     DCTR_REQUIRE(d_loss != nullptr, "vocab softmax: loss is null");
     if (d_dx != nullptr) DCTR_TRY(check_rows("dx", d_dx, dx_ld, D, dtype == DCTR_TYPE_F32 ? 4 : 2));
     hipStream_t st = as_stream(stream);
-    const int grid = ceil_div(N, VS_WAVES);
-    if (dtype == DCTR_TYPE_F32)
-        vocab_fwd_kernel<float><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_loss, d_lse, (float*)d_dx, dx_ld, d_status);
-    else
-        vocab_fwd_kernel<__bf16><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_loss, d_lse, (__bf16*)d_dx, dx_ld, d_status);
-    DCTR_LAUNCH_CHECK();
-    return DCTR_OK;
+    float* ws = (float*)d_workspace;
+    if (dtype == DCTR_TYPE_F32) VOCAB_BY_WIDTH(float, D, fwd, a, d_loss, d_lse, d_dx, dx_ld, d_status, ws, st)
+    VOCAB_BY_WIDTH(__bf16, D, fwd, a, d_loss, d_lse, d_dx, dx_ld, d_status, ws, st)
 }
 
 int dctr_vocab_softmax_bwd_weights(int dtype, const void* d_x, int x_ld, const void* d_w, int w_ld, const float* d_b, const int32_t* d_labels, int N,
@@ -188,13 +498,9 @@ int dctr_vocab_softmax_bwd_weights(int dtype, const void* d_x, int x_ld, const v
     DCTR_REQUIRE(N == 0 || d_lse != nullptr, "vocab softmax: lse is null");
     DCTR_TRY(check_rows("dw", d_dw, dw_ld, D, dtype == DCTR_TYPE_F32 ? 4 : 2));
     hipStream_t st = as_stream(stream);
-    const int grid = ceil_div(V, VS_WAVES);
-    if (dtype == DCTR_TYPE_F32)
-        vocab_dw_kernel<float><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_lse, (float*)d_dw, dw_ld, d_db);
-    else
-        vocab_dw_kernel<__bf16><<<grid, 64 * VS_WAVES, 0, st>>>(a, d_lse, (__bf16*)d_dw, dw_ld, d_db);
-    DCTR_LAUNCH_CHECK();
-    return DCTR_OK;
+    float* ws = (float*)d_workspace;
+    if (dtype == DCTR_TYPE_F32) VOCAB_BY_WIDTH(float, D, launch_dw, a, d_lse, d_dw, dw_ld, d_db, ws, st)
+    VOCAB_BY_WIDTH(__bf16, D, launch_dw, a, d_lse, d_dw, dw_ld, d_db, ws, st)
 }
 
 }  // extern "C"
