@@ -53,6 +53,9 @@ __device__ __forceinline__ bool segment_is_bad(const AttnView& a, int b) {
     return q0 < 0 || q1 < q0 || q1 > a.total_q || (int64_t)q1 - q0 > a.max_q || k0 < 0 || k1 < k0 || k1 > a.total_k ||
            (int64_t)k1 - k0 > a.max_k || st < -DCTR_MAX_POSITION || st > DCTR_MAX_POSITION;
 }
+__device__ __forceinline__ void flag_segment(const AttnView& a, int b, int32_t* status) {
+    if (status != nullptr && segment_is_bad(a, b)) { status[0] = 1; status[1] = b; }
+}
 
 // The bias of one tile of scores.  Distances below the first boundary all share bucket 0, those from the last boundary on the last bucket: only
 // a tile that reaches between the two ("near") looks values up, any other adds one number.  Tables hold log2(e) x the bias (the kernels'
@@ -63,15 +66,13 @@ __device__ __forceinline__ bool near_tile(const RelBuckets& r, int dmin, int dma
 // bucket of every distance of a tile that is not near
 __device__ __forceinline__ int far_bucket(const RelBuckets& r, int dmin) { return r.n > 1 && dmin >= r.edge[r.n - 2] ? r.n - 1 : 0; }
 
-// number of the r.n - 1 edges (staged in shared memory: kernel arguments are not indexed by lanes) that are <= d
-__device__ __forceinline__ int bucket_of(const int32_t* edges, int n, int d) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (edges[mid] <= d) lo = mid + 1; else hi = mid;
-    }
-    return lo;
+// bucket of distance d; the edges come by scalar loads, one compare each for the whole wave
+__device__ __forceinline__ int bucket_of(const RelBuckets& r, int d) {
+    int n = 0;
+    for (int u = 0; u + 1 < r.n; ++u) n += r.edge[u] <= d;
+    return n;
 }
+__device__ __forceinline__ int rel_reach(const RelBuckets& r) { return r.n > 1 ? r.edge[r.n - 2] - r.edge[0] + 2 * REL_PAD : 0; }
 
 inline int rel_reach(const dctr_attention* a) {         // entries of a table over distances
     return a->n_buckets > 1 ? a->boundaries[a->n_buckets - 2] - a->boundaries[0] + 2 * REL_PAD : 0;
@@ -81,7 +82,7 @@ inline int rel_reach(const dctr_attention* a) {         // entries of a table ov
 struct AttnSplit { int row_blocks, splits; };           // the forward's form for few query rows a key head (splits = 0: the other form)
 AttnSplit attn_split(const dctr_attention* a);
 int64_t attn_fwd_workspace(const dctr_attention* a);      // bytes
-int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st);
+int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st);
 
 struct AttnGrads {
     const void* out; int64_t out_ld;

@@ -7,7 +7,7 @@ namespace dctr {
 
 __global__ void attn_check_kernel(AttnView a, int32_t* status) {
     const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b < a.n_seg && segment_is_bad(a, b)) { status[0] = 1; status[1] = b; }
+    if (b < a.n_seg) flag_segment(a, b, status);
 }
 
 __global__ void fill_zero_kernel(float* x, int n) {
@@ -98,12 +98,12 @@ int dctr_cross_attention_fwd(const dctr_attention* a, const void* d_q, int q_ld,
     DCTR_TRY(check_workspace(a, 0, d_workspace, workspace_bytes));
     hipStream_t st = as_stream(stream);
     if (a->n_seg == 0) return DCTR_OK;
-    if (d_status != nullptr) {
+    const bool none = a->total_q == 0 || a->max_q == 0;                  // (otherwise the forward's blocks look at their segments)
+    if (none && d_status != nullptr) {
         attn_check_kernel<<<ceil_div(a->n_seg, 256), 256, 0, st>>>(v, d_status);
         DCTR_LAUNCH_CHECK();
     }
-    if (a->total_q == 0) return DCTR_OK;
-    return attn_fwd(a, v, d_out, out_ld, d_lse, (float*)d_workspace, st);
+    return none ? DCTR_OK : attn_fwd(a, v, d_out, out_ld, d_lse, d_status, (float*)d_workspace, st);
 }
 
 int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld, const void* d_k, int k_ld, const void* d_v, int v_ld,

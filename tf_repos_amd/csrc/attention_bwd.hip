@@ -26,11 +26,15 @@ __device__ __forceinline__ void lds_add(float* cell, float x) { __hip_atomic_fet
 
 // part: [head][segment * row_blocks + row block][n_buckets] shares of the bias gradient, or null; delta [total_q, heads]
 template <typename T, int DP, int QW>
-__global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
+__global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
                                                                  T* dq, int64_t dq_ld, float* delta, float* part, int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Q = QuerySide<T, DP, QW>;
     constexpr int NB = Q::NB, TILE = Q::TILE;
+    // For bf16 <do, out> is off by the rounding of `out`, an error that all of a row's ds share.  The walk sums p dp over every key, which is the
+    // same number unrounded, and P K besides: dq is put right with (rounded - unrounded) P K at the end, the key side and the bias gradient take
+    // the unrounded one.  (Measured: the relative error of dq and dk 0.0030 -> 0.0023 at 777 x 1531 x 128.)
+    constexpr bool ROUNDED = sizeof(T) == 2;
     T *kt = reinterpret_cast<T*>(lds), *vt = kt + Q::BUFS * TILE;
     float* lut = reinterpret_cast<float*>(lds + Q::first);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
@@ -46,16 +50,8 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
     const int wrow = row0 + 32 * (wave % QW), row = wrow + (lane & 31), first_key = 32 * NB * (wave / QW);
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = a.scale * LOG2E;
-    const int reach = a.rel.n > 1 ? a.rel.edge[a.rel.n - 2] - a.rel.edge[0] + 2 * REL_PAD : 0;
+    const int reach = rel_reach(a.rel);
     float* cells = lut + reach;                                         // [4 waves][2 halves][reach], then 2 x 4 far sums
-    int32_t* edges = reinterpret_cast<int32_t*>(cells + 8 * reach + 8);
-    if (reach > 0) {
-        for (int u = tid; u + 1 < a.rel.n; u += BWD_THREADS) edges[u] = a.rel.edge[u];
-        __syncthreads();
-        for (int u = tid; u < reach; u += BWD_THREADS) lut[u] = LOG2E * a.bias[bucket_of(edges, a.rel.n, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
-        for (int u = tid; u < 8 * reach; u += BWD_THREADS) cells[u] = 0.f;
-        __syncthreads();
-    }
     float* mine = cells + (2 * wave + half) * reach;
 
     RowFrags<T, DP> q, go;
@@ -73,7 +69,7 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
         if (row < s.nq) {
             const float L = lse[(s.q0 + row) * a.heads + h];
             if (L != -INFINITY) minus_lse = -LOG2E * L;
-            if (wave < QW && half == 0) delta[(s.q0 + row) * a.heads + h] = dl;
+            if (!ROUNDED && wave < QW && half == 0) delta[(s.q0 + row) * a.heads + h] = dl;
         }
     }
 
@@ -85,7 +81,7 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
     const bool busy = wrow < s.nq;
     const int wend = a.causal ? s.start + min(wrow + 32, s.nq) : keys;
 
-    f32x16 acc[DP / 32] = {};
+    f32x16 acc[DP / 32] = {}, pk[ROUNDED ? DP / 32 : 1] = {};
     float far_ds[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, pdp = 0.f;     // [below the first boundary, from the last one on]
     Staged<T, DP, Q::KEYS, BWD_THREADS> ks, vs;
     uint64_t bits[2] = {0, 0};                                          // kept keys of the tile
@@ -160,6 +156,11 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
         if (t >= last) return;
         __syncthreads();
         fetch(t * Q::KEYS);
+        if (!second) {                                                  // under the first tile's loads
+            for (int u = tid; u < reach; u += BWD_THREADS) lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
+            if (part != nullptr)
+                for (int u = tid; u < 8 * reach; u += BWD_THREADS) cells[u] = 0.f;
+        }
         store(0);
         __syncthreads();
         for (int n = 0; t < last; ++t, ++n) {
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
                 int cell, side;
                 const bool near = pair(kb, vb, j0, now, p, dp, cell, side);
                 if (!second) {
-                    if (part != nullptr && (sizeof(T) == 2 || !near)) {
+                    if (ROUNDED || (part != nullptr && !near)) {
                         float x = 0.f, y = 0.f;
 #pragma unroll
                         for (int k = 0; k < NB; ++k)
@@ -183,9 +184,15 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
                     }
 #pragma unroll
                     for (int k = 0; k < NB; ++k) {
+                        if (ROUNDED) {
+                            const auto w = Mma<T>::pack(p[k]);
+#pragma unroll
+                            for (int d = 0; d < DP / 32; ++d)
+                                pk[ROUNDED ? d : 0] = Mma<T>::template weigh<DP>(kb, first_key + 32 * k, 32 * d, w, pk[ROUNDED ? d : 0]);
+                        }
 #pragma unroll
                         for (int r = 0; r < 16; ++r) p[k][r] *= dp[k][r] - dl;
-                        if (sizeof(T) == 4 && part != nullptr && near)
+                        if (!ROUNDED && part != nullptr && near)
 #pragma unroll
                             for (int r = 0; r < 16; ++r) lds_add(mine + cell + 32 * k + reg_row(r), p[k][r]);
                         const auto w = Mma<T>::pack(p[k]);
@@ -206,20 +213,22 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
     };
     walk(false);
 
-    if (part != nullptr) {
-        // The bias gradient is f32 whatever the type: for bf16, <do, out> as `out` was rounded would be off by 2^-9.  The first walk has summed
-        // p dp over every key, which is the same number unrounded; the far buckets' sums take it afterwards, the near tiles are walked again.
-        if (sizeof(T) == 2) {
-            dl = both_sum(pdp);
-            if (QW == 1) {                                              // the waves hold different keys of the same rows
-                float* meet = reinterpret_cast<float*>(lds);
-                __syncthreads();
-                if (half == 0) meet[wave * 32 + lane] = dl;
-                __syncthreads();
-                dl = meet[lane & 31] + meet[32 + (lane & 31)] + meet[64 + (lane & 31)] + meet[96 + (lane & 31)];
-            }
-            if (a.rel.n > 1) walk(true);
+    if (ROUNDED) {
+        float exact = both_sum(pdp);
+        if (QW == 1) {                                                  // the waves hold different keys of the same rows
+            float* meet = reinterpret_cast<float*>(lds);
+            __syncthreads();
+            if (half == 0) meet[wave * 32 + lane] = exact;
+            __syncthreads();
+            exact = (meet[lane & 31] + meet[32 + (lane & 31)]) + (meet[64 + (lane & 31)] + meet[96 + (lane & 31)]);
         }
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] += (dl - exact) * pk[ROUNDED ? d : 0];
+        dl = exact;
+        if (wave < QW && half == 0 && row < s.nq) delta[(s.q0 + row) * a.heads + h] = dl;
+    }
+    if (part != nullptr) {
+        if (ROUNDED && a.rel.n > 1) walk(true);                         // the near tiles again, for their distances' sums
         float* fars = cells + 8 * reach;
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
@@ -229,19 +238,25 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
             if (lane == 0) fars[4 * side + wave] = x;
         }
         __syncthreads();
-        for (int u = tid; u < a.rel.n; u += BWD_THREADS) {
+        // every distance's eight cells, then a wave a bucket
+        if (tiles > 0)
+            for (int u = tid; u < reach; u += BWD_THREADS) {
+                float x = cells[u];
+#pragma unroll
+                for (int w = 1; w < 8; ++w) x += cells[w * reach + u];
+                cells[u] = x;
+            }
+        __syncthreads();
+        for (int u = wave; u < a.rel.n; u += 4) {
             float x = 0.f;
-            if (reach > 0) {
-                const int lo = u == 0 ? 0 : edges[u - 1] - edges[0] + REL_PAD, hi = u + 1 == a.rel.n ? reach : edges[u] - edges[0] + REL_PAD;
-                for (int w = 0; w < 8; ++w) {
-                    float y = 0.f;
-                    for (int d = lo; d < hi; ++d) y += cells[w * reach + d];
-                    x += y;
-                }
+            if (reach > 0 && tiles > 0) {
+                const int lo = u == 0 ? 0 : a.rel.edge[u - 1] - a.rel.edge[0] + REL_PAD, hi = u + 1 == a.rel.n ? reach : a.rel.edge[u] - a.rel.edge[0] + REL_PAD;
+                for (int d = lo + lane; d < hi; d += 64) x += cells[d];
+                x = wave_sum(x);
             }
             if (u == 0) x += (fars[0] + fars[1]) + (fars[2] + fars[3]);
             if (u > 0 && u + 1 == a.rel.n) x += (fars[4] + fars[5]) + (fars[6] + fars[7]);
-            share[u] = x;
+            if (lane == 0) share[u] = x;
         }
     }
 
@@ -280,18 +295,21 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_q_kernel(AttnView a, con
                                acc[k][4 * i + 3] * a.scale);
 }
 
-// one block per head: thread = (slice of the shares, bucket), slices added in order
-__global__ __launch_bounds__(1024) void attn_bias_sum_kernel(const float* part, int64_t shares, int n, int heads, float* dbias) {
-    __shared__ float red[1024];
-    const int slices = 1024 / n, u = threadIdx.x % n, sl = threadIdx.x / n, h = blockIdx.x;
-    float x = 0.f;
-    if (sl < slices)
-        for (int64_t i = sl; i < shares; i += slices) x += part[((int64_t)h * shares + i) * n + u];
-    red[threadIdx.x] = x;
+// One block a head, behind the key side's blocks: thread = (slice of the shares, bucket), slices added in order.
+struct BiasShares { const float* part; int64_t shares; float* dbias; };
+__device__ __forceinline__ void sum_shares(const BiasShares& x, int n, int heads, int h, float* red) {
+    const int slices = BWD_THREADS / n, u = threadIdx.x % n, sl = threadIdx.x / n;
+    float y = 0.f;
+    if (sl < slices) {
+        const float* p = x.part + (int64_t)h * x.shares * n + u;
+#pragma unroll 8
+        for (int64_t i = sl; i < x.shares; i += slices) y += p[i * n];
+    }
+    red[threadIdx.x] = y;
     __syncthreads();
     if (sl == 0) {
-        for (int w = 1; w < slices; ++w) x += red[w * n + u];
-        dbias[u * heads + h] = x;
+        for (int w = 1; w < slices; ++w) y += red[w * n + u];
+        x.dbias[u * heads + h] = y;
     }
 }
 
@@ -303,8 +321,8 @@ struct KeySide {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(BWD_THREADS) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout, int64_t dout_ld, T* dk,
-                                                                  int64_t dk_ld, T* dv, int64_t dv_ld, int key_blocks) {
+__global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout, int64_t dout_ld, T* dk,
+                                                                  int64_t dk_ld, T* dv, int64_t dv_ld, int key_blocks, BiasShares shares, int blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Kd = KeySide<T, DP>;
     constexpr int QT = Kd::QT, TILE = Kd::TILE;
@@ -312,6 +330,10 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_kv_kernel(AttnView a, co
     float* stats = reinterpret_cast<float*>(lds + Kd::tiles);           // [buffer][-log2(e) lse, delta][QT]
     float* lut = reinterpret_cast<float*>(lds + Kd::tiles + Kd::stats);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, kv_heads = a.heads / a.group;
+    if ((int)blockIdx.x >= blocks) {
+        sum_shares(shares, a.rel.n, a.heads, blockIdx.x - blocks, stats);
+        return;
+    }
     const int kb = blockIdx.x % key_blocks, g = blockIdx.x / key_blocks % kv_heads, b = blockIdx.x / key_blocks / kv_heads;
     const Segment s = load_segment(a, b);
     const int key0 = kb * 128;
@@ -319,14 +341,9 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_kv_kernel(AttnView a, co
     const int wkey = key0 + wave * 32, key = wkey + (lane & 31);
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = a.scale * LOG2E;
-    const int reach = a.rel.n > 1 ? a.rel.edge[a.rel.n - 2] - a.rel.edge[0] + 2 * REL_PAD : 0;
+    const int reach = rel_reach(a.rel);
     int32_t* buckets = reinterpret_cast<int32_t*>(lut + reach);         // of every distance
-    int32_t* edges = buckets + reach;
-    if (reach > 0) {
-        for (int u = tid; u + 1 < a.rel.n; u += BWD_THREADS) edges[u] = a.rel.edge[u];
-        __syncthreads();
-        for (int u = tid; u < reach; u += BWD_THREADS) buckets[u] = bucket_of(edges, a.rel.n, a.rel.edge[0] - REL_PAD + u);
-    }
+    for (int u = tid; u < reach; u += BWD_THREADS) buckets[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u);
     const bool on = key < s.nk && (a.keep == nullptr || a.keep[s.k0 + key] != 0);
     RowFrags<T, DP> k, v;
     k.load((const T*)a.k + (s.k0 + key) * a.k_ld + (int64_t)g * a.dim, chunks, on);
@@ -362,8 +379,8 @@ __global__ __launch_bounds__(BWD_THREADS) void attn_bwd_kv_kernel(AttnView a, co
     for (int h = g * a.group; h < (g + 1) * a.group; ++h) {
         if (tiles == 0) break;
         __syncthreads();
-        for (int u = tid; u < reach; u += BWD_THREADS) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
         fetch(h, first * QT);
+        for (int u = tid; u < reach; u += BWD_THREADS) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
         store(0);
         __syncthreads();
         for (int t = 0; t < tiles; ++t) {
@@ -452,7 +469,7 @@ static int launch_q(const dctr_attention* a, const AttnView& v, const void* out,
     const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
     DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
     if (blocks == 0) return DCTR_OK;
-    const size_t lds = QuerySide<T, DP, QW>::first + sizeof(float) * (9 * rel_reach(a) + 8 + a->n_buckets);
+    const size_t lds = QuerySide<T, DP, QW>::first + sizeof(float) * (9 * rel_reach(a) + 8);
     attn_bwd_q_kernel<T, DP, QW><<<(unsigned)blocks, BWD_THREADS, lds, st>>>(v, (const T*)out, out_ld, lse, (const T*)dout, dout_ld, (T*)dq, dq_ld, delta, part,
                                                                              row_blocks);
     DCTR_LAUNCH_CHECK();
@@ -467,17 +484,15 @@ static int launch_bwd(const dctr_attention* a, const AttnView& v, const AttnGrad
         DCTR_TRY((launch_q<T, DP, wide ? 4 : 1>(a, v, x.out, x.out_ld, x.lse, x.dout, x.dout_ld, x.dq, x.dq_ld, delta, part, st)));
     else
         DCTR_TRY((launch_q<T, DP, 4>(a, v, x.out, x.out_ld, x.lse, x.dout, x.dout_ld, x.dq, x.dq_ld, delta, part, st)));
-    if (part != nullptr) {
-        attn_bias_sum_kernel<<<a->heads, 1024, 0, st>>>(part, (int64_t)a->n_seg * row_blocks_of(a), a->n_buckets, a->heads, x.dbias);
-        DCTR_LAUNCH_CHECK();
-    }
     const int key_blocks = ceil_div(a->max_k, 128);
     const int64_t blocks = (int64_t)key_blocks * a->kv_heads * a->n_seg;
-    DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
-    if (blocks == 0) return DCTR_OK;
-    const size_t lds = KeySide<T, DP>::tiles + KeySide<T, DP>::stats + sizeof(float) * (2 * rel_reach(a) + a->n_buckets);
-    attn_bwd_kv_kernel<T, DP><<<(unsigned)blocks, BWD_THREADS, lds, st>>>(v, x.lse, delta, (const T*)x.dout, x.dout_ld, (T*)x.dk, x.dk_ld, (T*)x.dv, x.dv_ld,
-                                                                          key_blocks);
+    DCTR_REQUIRE(blocks + a->heads <= INT32_MAX, "attention: too many blocks for one launch");
+    const int sums = part != nullptr ? a->heads : 0;
+    if (blocks + sums == 0) return DCTR_OK;
+    const size_t lds = KeySide<T, DP>::tiles + std::max<size_t>(KeySide<T, DP>::stats, BWD_THREADS * sizeof(float)) + sizeof(float) * 2 * rel_reach(a);
+    attn_bwd_kv_kernel<T, DP><<<(unsigned)(blocks + sums), BWD_THREADS, lds, st>>>(v, x.lse, delta, (const T*)x.dout, x.dout_ld, (T*)x.dk, x.dk_ld, (T*)x.dv,
+                                                                                   x.dv_ld, key_blocks,
+                                                                                   BiasShares{part, (int64_t)a->n_seg * row_blocks_of(a), x.dbias}, (int)blocks);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }

@@ -13,28 +13,21 @@ namespace dctr {
 constexpr int ROWS_THREADS = 256, ROWS_KEYS = 64;
 
 template <typename T, int DP>
-__global__ __launch_bounds__(ROWS_THREADS) void attn_rows_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int row_blocks) {
+__global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_rows_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status,
+                                                                                                            int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int TILE = ROWS_KEYS * DP;
     T *kt = reinterpret_cast<T*>(lds), *vt = kt + 2 * TILE;
     float* lut = reinterpret_cast<float*>(vt + 2 * TILE);
-    int32_t* edges = reinterpret_cast<int32_t*>(kt);                    // (until the first tile is stored)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int rb = blockIdx.x % row_blocks, h = blockIdx.x / row_blocks % a.heads, b = blockIdx.x / row_blocks / a.heads;
     const Segment s = load_segment(a, b);
+    if (rb == 0 && h == 0 && tid == 0) flag_segment(a, b, status);
     const int row0 = rb * 128;
     if (row0 >= s.nq) return;
     const int wrow = row0 + wave * 32, row = wrow + (lane & 31);
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = fabsf(a.scale) * LOG2E;
-
-    const int reach = a.rel.n > 1 ? a.rel.edge[a.rel.n - 2] - a.rel.edge[0] + 2 * REL_PAD : 0;
-    if (reach > 0) {
-        for (int u = tid; u + 1 < a.rel.n; u += ROWS_THREADS) edges[u] = a.rel.edge[u];
-        __syncthreads();
-        for (int u = tid; u < reach; u += ROWS_THREADS) lut[u] = LOG2E * a.bias[bucket_of(edges, a.rel.n, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
-        __syncthreads();
-    }
 
     RowFrags<T, DP> q;
     q.load((const T*)a.q + (s.q0 + row) * a.q_ld + (int64_t)h * a.dim, chunks, row < s.nq);
@@ -62,10 +55,10 @@ __global__ __launch_bounds__(ROWS_THREADS) void attn_rows_kernel(AttnView a, T* 
         ks.store(kt + buf * TILE, tid, bits);
         vs.store(vt + buf * TILE, tid, bits);
     };
-    if (tiles > 0) {
-        fetch(0);
-        store(0);
-    }
+    if (tiles > 0) fetch(0);
+    const int reach = rel_reach(a.rel);                                 // (under the first tile's loads)
+    for (int u = tid; u < reach; u += ROWS_THREADS) lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
+    if (tiles > 0) store(0);
     __syncthreads();
     for (int t = 0; t < tiles; ++t) {
         const int j0 = t * ROWS_KEYS;
@@ -80,6 +73,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void attn_rows_kernel(AttnView a, T* 
             const bool near = near_tile(a.rel, d0 - 31, d0 + ROWS_KEYS - 1);
             const float far = a.rel.n > 0 && !near ? LOG2E * a.bias[far_bucket(a.rel, d0 - 31) * a.heads + h] : 0.f;
             const bool cut = a.causal && d0 + ROWS_KEYS - 1 > 0;
+            float c = scale, add = far;
             if (near || cut || now != ~0ull) {
                 uint64_t seen = now;
                 if (cut) {
@@ -96,10 +90,10 @@ __global__ __launch_bounds__(ROWS_THREADS) void attn_rows_kernel(AttnView a, T* 
                         const float x = fmaf(sc[k][r], scale, near ? tab[at] : far);
                         sc[k][r] = (seen >> at & 1) ? x : -INFINITY;
                     }
-                o.template step<2>(sc, 1.f, 0.f);
-            } else {
-                o.template step<2>(sc, scale, far);
+                c = 1.f;
+                add = 0.f;
             }
+            o.template step<2>(sc, c, add);
             o.template weigh<2>(vt + (t & 1) * TILE, sc);
         }
         if (t + 1 < tiles) store((t + 1) & 1);
@@ -118,30 +112,13 @@ __global__ __launch_bounds__(ROWS_THREADS) void attn_rows_kernel(AttnView a, T* 
 }
 
 // ---- split form ----------------------------------------------------------------------------------------------------------------------
-constexpr int SPLIT_KEYS = 32;                                          // of a wave's tile
+constexpr int SPLIT_KEYS = 32, SPLIT_TILES = 16;                       // keys of a wave's tile, tiles below which a block is not split
 // shared memory: 4 waves' K and V tiles, in whose place the waves' results meet (rows of DP + 4 floats: no two rows start at the same bank)
 template <typename T, int DP>
 struct SplitLds {
     static constexpr size_t tiles = 4 * 2 * SPLIT_KEYS * DP * sizeof(T), join = 4 * 32 * (DP + 4) * sizeof(float);
     static constexpr size_t first = tiles > join ? tiles : join, stats = 4 * 32 * 2 * sizeof(float);
 };
-
-// Joins n results (maximum, sum, weighted sum) of 32 rows: thread = (row, eighth of the columns).
-template <typename T, int DP, typename Get>
-__device__ __forceinline__ void join_rows(int n, int tid, Get get, float& m, float& l, float (&o)[DP / 8]) {
-    m = -INFINITY;
-    for (int w = 0; w < n; ++w) m = fmaxf(m, get(w, tid >> 3, -2));
-    const float base = m == -INFINITY ? 0.f : m;
-    l = 0.f;
-#pragma unroll
-    for (int d = 0; d < DP / 8; ++d) o[d] = 0.f;
-    for (int w = 0; w < n; ++w) {
-        const float f = exp2f(get(w, tid >> 3, -2) - base);
-        l = fmaf(get(w, tid >> 3, -1), f, l);
-#pragma unroll
-        for (int d = 0; d < DP / 8; ++d) o[d] = fmaf(get(w, tid >> 3, (tid & 7) * (DP / 8) + d), f, o[d]);
-    }
-}
 
 template <typename T, int DP>
 __device__ __forceinline__ void finish_row(const AttnView& a, int64_t qrow, int h, int tid, float m, float l, const float (&o)[DP / 8], T* out,
@@ -157,7 +134,8 @@ __device__ __forceinline__ void finish_row(const AttnView& a, int64_t qrow, int 
 
 // part: [block item][split][32][DP + 2] (weighted sum, maximum, sum); not used when there is one split
 template <typename T, int DP>
-__global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, float* part, AttnSplit cut) {
+__global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status, float* part,
+                                                                                              AttnSplit cut) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using L = SplitLds<T, DP>;
     constexpr int TILE = SPLIT_KEYS * DP;
@@ -169,26 +147,12 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int
     const int sp = blockIdx.x % cut.splits, item = blockIdx.x / cut.splits;
     const int rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
     const Segment s = load_segment(a, b);
+    if (rb == 0 && g == 0 && sp == 0 && tid == 0) flag_segment(a, b, status);
     const int rows = s.nq * a.group, r0 = rb * 32;
     if (r0 >= rows) return;
     const int r = r0 + (lane & 31), i = r / a.group, hg = r % a.group, h = g * a.group + hg;
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = fabsf(a.scale) * LOG2E;
-
-    // bias: bucket of a distance, then its value for the row's head (a block's rows have min(group, 32) different ones)
-    const int reach = a.rel.n > 1 ? a.rel.edge[a.rel.n - 2] - a.rel.edge[0] + 2 * REL_PAD : 0;
-    const int wide = min(a.group, 32), col = a.group <= 32 ? hg : r - r0;
-    float* table = stats + 4 * 32 * 2;                                  // [n_buckets][wide]
-    int32_t* edges = reinterpret_cast<int32_t*>(table + a.rel.n * wide);
-    int32_t* lut = edges + a.rel.n;
-    for (int u = tid; u < a.rel.n * wide; u += 256)
-        table[u] = LOG2E * a.bias[u / wide * a.heads + g * a.group + (a.group <= 32 ? u % wide : (r0 + u % wide) % a.group)];
-    if (reach > 0) {
-        for (int u = tid; u + 1 < a.rel.n; u += 256) edges[u] = a.rel.edge[u];
-        __syncthreads();
-        for (int u = tid; u < reach; u += 256) lut[u] = bucket_of(edges, a.rel.n, a.rel.edge[0] - REL_PAD + u) * wide;
-    }
-    if (a.rel.n > 0) __syncthreads();
 
     RowFrags<T, DP> q;
     q.load((const T*)a.q + (s.q0 + i) * a.q_ld + (int64_t)h * a.dim, chunks, r < rows);
@@ -199,7 +163,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int
     const int i0 = r0 / a.group, i1 = min(r0 + 31, rows - 1) / a.group;
     int keys = s.nk;
     if (a.causal) keys = max(0, min(keys, s.start + i1 + 1));
-    const int tiles = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS, each = (tiles + cut.splits - 1) / cut.splits;
+    const int tiles = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS, each = max(SPLIT_TILES, (tiles + cut.splits - 1) / cut.splits);
     const int t1 = min(tiles, (sp + 1) * each);
 
     Softmax<T, DP> o;
@@ -212,6 +176,17 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int
     };
     int t = sp * each + wave;
     if (t < t1) fetch(t * SPLIT_KEYS);
+
+    // Bias, under the first loads: bucket of a distance, then its value for the row's head (a block's rows have min(group, 32) different ones)
+    const int wide = min(a.group, 32), col = a.group <= 32 ? hg : r - r0;
+    float* table = stats + 4 * 32 * 2;                                  // [n_buckets][wide]
+    int32_t* lut = reinterpret_cast<int32_t*>(table + a.rel.n * wide);
+    for (int u = tid; u < a.rel.n * wide; u += 256)
+        table[u] = LOG2E * a.bias[u / wide * a.heads + g * a.group + (a.group <= 32 ? u % wide : (r0 + u % wide) % a.group)];
+    const int reach = rel_reach(a.rel);
+    if (near_tile(a.rel, sp * each * SPLIT_KEYS - s.start - i1, t1 * SPLIT_KEYS - 1 - s.start - i0))
+        for (int u = tid; u < reach; u += 256) lut[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * wide;
+    if (a.rel.n > 0) __syncthreads();
     for (; t < t1; t += 4) {
         const int j0 = t * SPLIT_KEYS;
         const uint64_t now = __ballot(kept != 0);
@@ -228,6 +203,7 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int
         const bool near = near_tile(a.rel, dmin, dmax);
         const float far = a.rel.n > 0 && !near ? table[far_bucket(a.rel, dmin) * wide + col] : 0.f;
         const bool hide = a.causal && dmax > 0;
+        float c = scale, add = far;
         if (near || hide || now != 0xFFFFFFFFull) {
             uint64_t seen = now;
             if (hide) {
@@ -241,29 +217,15 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int
                 const float x = fmaf(sc[0][e], scale, near ? table[at[reg_row(e)] + col] : far);
                 sc[0][e] = (seen >> reg_row(e) & 1) ? x : -INFINITY;
             }
-            o.template step<1>(sc, 1.f, 0.f);
-        } else {
-            o.template step<1>(sc, scale, far);
+            c = 1.f;
+            add = 0.f;
         }
+        o.template step<1>(sc, c, add);
         o.template weigh<1>(vt, sc);
     }
 
-    __syncthreads();                                                    // every wave is done with the tiles
-    const float l = both_sum(o.l);
-    if (lane < 32) {
-        stats[(wave * 32 + lane) * 2] = o.m;
-        stats[(wave * 32 + lane) * 2 + 1] = l;
-    }
-#pragma unroll
-    for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            *reinterpret_cast<f32x4*>(join + (wave * 32 + (lane & 31)) * (DP + 4) + 32 * k + 8 * e + 4 * (lane >> 5)) =
-                f32x4{o.acc[k][4 * e], o.acc[k][4 * e + 1], o.acc[k][4 * e + 2], o.acc[k][4 * e + 3]};
-    __syncthreads();
     float m, sum, w[DP / 8];
-    join_rows<T, DP>(4, tid, [&](int n, int row, int d) { return d == -2 ? stats[(n * 32 + row) * 2] : d == -1 ? stats[(n * 32 + row) * 2 + 1]
-                                                                                                    : join[(n * 32 + row) * (DP + 4) + d]; }, m, sum, w);
+    join_waves<T, DP>(o, join, stats, m, sum, w);
     const int mine = r0 + (tid >> 3);
     if (cut.splits == 1) {
         if (mine < rows) finish_row<T, DP>(a, s.q0 + mine / a.group, g * a.group + mine % a.group, tid, m, sum, w, out, out_ld, lse);
@@ -275,17 +237,42 @@ __global__ __launch_bounds__(256) void attn_split_kernel(AttnView a, T* out, int
     if ((tid & 7) == 0) { to[DP] = m; to[DP + 1] = sum; }
 }
 
+// one wave a row: the splits' statistics by lanes, their sums one split after the other
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnView a, T* out, int64_t out_ld, float* lse, const float* part, AttnSplit cut) {
-    const int tid = threadIdx.x, kv_heads = a.heads / a.group, item = blockIdx.x;
+    const int lane = threadIdx.x & 63, kv_heads = a.heads / a.group, item = blockIdx.x >> 3, r = (blockIdx.x & 7) * 4 + (threadIdx.x >> 6);
     const int rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
     const Segment s = load_segment(a, b);
-    const int mine = rb * 32 + (tid >> 3);
+    const int mine = rb * 32 + r;
     if (mine >= s.nq * a.group) return;
-    float m, sum, w[DP / 8];
-    join_rows<T, DP>(cut.splits, tid, [&](int n, int row, int d) { return part[(((int64_t)item * cut.splits + n) * 32 + row) * (DP + 2) + (d < 0 ? DP + 2 + d : d)]; },
-                     m, sum, w);
-    finish_row<T, DP>(a, s.q0 + mine / a.group, g * a.group + mine % a.group, tid, m, sum, w, out, out_ld, lse);
+    const int64_t step = 32 * (DP + 2);
+    const float* p = part + ((int64_t)item * cut.splits * 32 + r) * (DP + 2);
+    float m = -INFINITY;
+    for (int n = lane; n < cut.splits; n += 64) m = fmaxf(m, p[n * step + DP]);
+    m = wave_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    constexpr int PER = DP > 64 ? 2 : 1;
+    const int d0 = lane * PER < DP ? lane * PER : 0;
+    float l = 0.f, o[PER] = {};
+    for (int n0 = 0; n0 < cut.splits; n0 += 64) {
+        const int n = n0 + lane;
+        const float f = n < cut.splits ? exp2f(p[n * step + DP] - base) : 0.f;
+        if (n < cut.splits) l = fmaf(p[n * step + DP + 1], f, l);
+        const int many = min(64, cut.splits - n0);
+        for (int k = 0; k < many; ++k) {
+            const float w = __shfl(f, k);
+#pragma unroll
+            for (int d = 0; d < PER; ++d) o[d] = fmaf(p[(n0 + k) * step + d0 + d], w, o[d]);
+        }
+    }
+    l = wave_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t qrow = s.q0 + mine / a.group;
+    const int h = g * a.group + mine % a.group;
+    if (lse != nullptr && lane == 0) lse[qrow * a.heads + h] = l == 0.f ? -INFINITY : LN2 * (m + log2f(l));
+#pragma unroll
+    for (int d = 0; d < PER; ++d)
+        if (lane * PER + d < a.dim) out[qrow * out_ld + (int64_t)h * a.dim + lane * PER + d] = (T)(o[d] * inv);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
@@ -296,42 +283,42 @@ AttnSplit attn_split(const dctr_attention* a) {
     if (rows > 128) return {0, 0};
     const int64_t row_blocks = (rows + 31) / 32, items = row_blocks * a->kv_heads * a->n_seg;
     if (items == 0) return {(int)row_blocks, 1};
-    const int64_t most = (a->max_k + 511) / 512, want = (2048 + items - 1) / items;
+    const int64_t most = (a->max_k + SPLIT_KEYS * SPLIT_TILES - 1) / (SPLIT_KEYS * SPLIT_TILES), want = (4096 + items - 1) / items;
     return {(int)row_blocks, (int)std::max<int64_t>(1, std::min(most, want))};
 }
 
 template <typename T, int DP>
-static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st) {
+static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st) {
     const AttnSplit cut = attn_split(a);
-    const int64_t table = a->n_buckets > 0 ? a->n_buckets * std::min<int64_t>(v.group, 32) + a->n_buckets + rel_reach(a) : 0;
+    const int64_t table = a->n_buckets > 0 ? a->n_buckets * std::min<int64_t>(v.group, 32) + rel_reach(a) : 0;
     if (cut.splits == 0) {
         const int row_blocks = ceil_div(a->max_q, 128);
         const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
         DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
         const size_t lds = 4 * ROWS_KEYS * DP * sizeof(T) + rel_reach(a) * sizeof(float);
-        attn_rows_kernel<T, DP><<<(unsigned)blocks, ROWS_THREADS, lds, st>>>(v, (T*)out, out_ld, lse, row_blocks);
+        attn_rows_kernel<T, DP><<<(unsigned)blocks, ROWS_THREADS, lds, st>>>(v, (T*)out, out_ld, lse, status, row_blocks);
         DCTR_LAUNCH_CHECK();
         return DCTR_OK;
     }
     const int64_t items = (int64_t)cut.row_blocks * a->kv_heads * a->n_seg;
-    DCTR_REQUIRE(items * cut.splits <= INT32_MAX, "attention: too many blocks for one launch");
+    DCTR_REQUIRE(items * std::max(8, cut.splits) <= INT32_MAX, "attention: too many blocks for one launch");
     if (items == 0) return DCTR_OK;
     using L = SplitLds<T, DP>;
-    attn_split_kernel<T, DP><<<(unsigned)(items * cut.splits), 256, L::first + L::stats + table * sizeof(float), st>>>(v, (T*)out, out_ld, lse, ws, cut);
+    attn_split_kernel<T, DP><<<(unsigned)(items * cut.splits), 256, L::first + L::stats + table * sizeof(float), st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     DCTR_LAUNCH_CHECK();
     if (cut.splits > 1) {
-        attn_join_kernel<T, DP><<<(unsigned)items, 256, 0, st>>>(v, (T*)out, out_ld, lse, ws, cut);
+        attn_join_kernel<T, DP><<<(unsigned)(items * 8), 256, 0, st>>>(v, (T*)out, out_ld, lse, ws, cut);
         DCTR_LAUNCH_CHECK();
     }
     return DCTR_OK;
 }
 
 template <typename T>
-static int by_width(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st) {
+static int by_width(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st) {
     switch (padded(a->head_dim)) {
-        case 32: return launch_fwd<T, 32>(a, v, out, out_ld, lse, ws, st);
-        case 64: return launch_fwd<T, 64>(a, v, out, out_ld, lse, ws, st);
-        default: return launch_fwd<T, 128>(a, v, out, out_ld, lse, ws, st);
+        case 32: return launch_fwd<T, 32>(a, v, out, out_ld, lse, status, ws, st);
+        case 64: return launch_fwd<T, 64>(a, v, out, out_ld, lse, status, ws, st);
+        default: return launch_fwd<T, 128>(a, v, out, out_ld, lse, status, ws, st);
     }
 }
 
@@ -340,8 +327,8 @@ int64_t attn_fwd_workspace(const dctr_attention* a) {
     return cut.splits > 1 ? (int64_t)cut.row_blocks * a->kv_heads * a->n_seg * cut.splits * 32 * (padded(a->head_dim) + 2) * (int64_t)sizeof(float) : 0;
 }
 
-int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, float* ws, hipStream_t st) {
-    return a->dtype == DCTR_TYPE_F32 ? by_width<float>(a, v, out, out_ld, lse, ws, st) : by_width<__bf16>(a, v, out, out_ld, lse, ws, st);
+int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st) {
+    return a->dtype == DCTR_TYPE_F32 ? by_width<float>(a, v, out, out_ld, lse, status, ws, st) : by_width<__bf16>(a, v, out, out_ld, lse, status, ws, st);
 }
 
 }  // namespace dctr

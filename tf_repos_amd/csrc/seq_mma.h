@@ -44,6 +44,15 @@ __device__ __forceinline__ float both_sum(float x) { const Halves h = halves(x);
 // row of register r within its 32-row block
 __device__ __forceinline__ constexpr int reg_row(int r) { return 8 * (r >> 2) + (r & 3); }      // + 4 * (lane >> 5)
 
+// The lane, for the addresses of a tile's reads.  At the widest rows the compiler would keep every address of the loop in a register of its own
+// and spill the accumulators for them: there it is told nothing, and forms them again a tile (one exclusive or each).
+template <int DP>
+__device__ __forceinline__ int tile_lane() {
+    int l = threadIdx.x & 63;
+    if (DP > 128) asm volatile("" : "+v"(l));
+    return l;
+}
+
 template <typename T, int DP>
 struct Tile {
     static constexpr int CHUNKS = DP * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
@@ -74,7 +83,7 @@ template <> struct Mma<__bf16> {
     }
     template <int DP>
     static __device__ __forceinline__ f32x16 weigh(const __bf16* tile, int row0, int col0, const Weights& p, f32x16 acc) {
-        const int l = threadIdx.x & 63, row = row0 + 4 * (l >> 5) + ((l & 15) >> 2), col = col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+        const int l = tile_lane<DP>(), row = row0 + 4 * (l >> 5) + ((l & 15) >> 2), col = col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             bf16x8 a;
@@ -113,7 +122,7 @@ template <> struct Mma<float> {
     static __device__ __forceinline__ Weights pack(const f32x16& p) { return {p}; }
     template <int DP>
     static __device__ __forceinline__ f32x16 weigh(const float* tile, int row0, int col0, const Weights& p, f32x16 acc) {
-        const int l = threadIdx.x & 63, row = row0 + 4 * (l >> 5), col = col0 + (l & 31);
+        const int l = tile_lane<DP>(), row = row0 + 4 * (l >> 5), col = col0 + (l & 31);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             acc = __builtin_amdgcn_mfma_f32_32x32x2f32(tile[Tile<float, DP>::at(row + reg_row(r), col >> 2) + (col & 3)], p.w[r], acc, 0, 0, 0);
@@ -145,7 +154,7 @@ struct RowFrags {
 // S of tile rows [row0, row0 + 32) against held rows
 template <typename T, int DP>
 __device__ __forceinline__ f32x16 scores(const T* tile, int row0, const RowFrags<T, DP>& held) {
-    const int l = threadIdx.x & 63, row = row0 + (l & 31), g = l >> 5;
+    const int l = tile_lane<DP>(), row = row0 + (l & 31), g = l >> 5;
     f32x16 s = {};
 #pragma unroll
     for (int k = 0; k < RowFrags<T, DP>::STEPS; ++k)
@@ -210,7 +219,10 @@ struct Softmax {
             const float mn = fmaxf(m, top), shrink = exp2f(m - (mn == -INFINITY ? 0.f : mn));
             l *= shrink;
 #pragma unroll
-            for (int k = 0; k < DP / 32; ++k) acc[k] *= shrink;
+            for (int k = 0; k < DP / 32; ++k) {
+                acc[k] *= shrink;
+                if (DP > 64) __builtin_amdgcn_sched_barrier(0);         // one block at a time: accumulators live in the other register file there
+            }
             m = mn;
         }
         const float off = b - (m == -INFINITY ? 0.f : m);
@@ -234,5 +246,54 @@ struct Softmax {
         }
     }
 };
+
+// The results of a block's four waves on the same 32 rows meet in shared memory: `join` 4 x 32 rows of DP + 4 floats (no two rows start at the
+// same bank), `stats` 4 x 32 pairs (maximum, sum).  Afterwards thread t holds row t / 8's maximum, sum and columns [t % 8 * DP/8, + DP/8).
+template <typename T, int DP>
+__device__ __forceinline__ void join_waves(const Softmax<T, DP>& o, float* join, float* stats, float& m, float& l, float (&w)[DP / 8]) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = tid >> 3;
+    __syncthreads();                                                    // every wave is done with the tiles
+    const float sum = both_sum(o.l);
+    if (lane < 32) {
+        stats[(wave * 32 + lane) * 2] = o.m;
+        stats[(wave * 32 + lane) * 2 + 1] = sum;
+    }
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<f32x4*>(join + (wave * 32 + (lane & 31)) * (DP + 4) + 32 * k + 8 * e + 4 * (lane >> 5)) =
+                f32x4{o.acc[k][4 * e], o.acc[k][4 * e + 1], o.acc[k][4 * e + 2], o.acc[k][4 * e + 3]};
+    __syncthreads();
+    m = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) m = fmaxf(m, stats[(n * 32 + row) * 2]);
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d) w[d] = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const float f = exp2f(stats[(n * 32 + row) * 2] - base);
+        l = fmaf(stats[(n * 32 + row) * 2 + 1], f, l);
+#pragma unroll
+        for (int d = 0; d < DP / 8; d += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(join + (n * 32 + row) * (DP + 4) + (tid & 7) * (DP / 8) + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[d + e] = fmaf(x[e], f, w[d + e]);
+        }
+    }
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
 
 }  // namespace dctr

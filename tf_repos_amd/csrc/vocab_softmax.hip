@@ -24,12 +24,6 @@ struct VocabView {
 
 constexpr int VS_THREADS = 256;
 
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-    return x;
-}
-
 // ---- forward: the same pass as an attention whose keys and values are both the table --------------------------------------------------
 // What a split of the vocabulary leaves for every row, the label's column left out: maximum (base 2), sum, weighted sum of table rows.
 struct VocabParts {
@@ -39,7 +33,7 @@ struct VocabParts {
 };
 
 template <typename T, int DP>
-struct VocabTile { static constexpr int ROWS = sizeof(T) * DP <= 512 ? 64 : 32, NB = ROWS / 32, SIZE = ROWS * DP; };
+struct VocabTile { static constexpr int ROWS = sizeof(T) * DP <= 256 ? 64 : 32, NB = ROWS / 32, SIZE = ROWS * DP; };
 
 // One step of a wave's 32 rows against NB * 32 table rows from v0 on: scores, bias, hidden columns (behind the table, the row's label).
 // `bt`: log2(e) b of the tile's rows, in shared memory, or null.
@@ -51,6 +45,7 @@ __device__ __forceinline__ void vocab_step(const T* tile, const float* bt, const
 #pragma unroll
     for (int k = 0; k < NB; ++k) s[k] = scores<T, DP>(tile, 32 * k, x);
     const int64_t own = label - v0;
+    float c = LOG2E;
     const bool hide = v0 + 32 * NB > v1 || __any(own >= 0 && own < 32 * NB);
     if (bt != nullptr || hide) {
         uint64_t seen = v1 - v0 >= 64 ? ~0ull : (1ull << (v1 - v0)) - 1;
@@ -70,10 +65,9 @@ __device__ __forceinline__ void vocab_step(const T* tile, const float* bt, const
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[k][r] = (seen >> (32 * k + reg_row(r)) & 1) ? s[k][r] : -INFINITY;
         }
-        o.template step<NB>(s, 1.f, 0.f);
-    } else {
-        o.template step<NB>(s, LOG2E, 0.f);
+        c = 1.f;
     }
+    o.template step<NB>(s, c, 0.f);
     if (DX) o.template weigh<NB>(tile, s);
 }
 
@@ -95,7 +89,7 @@ __device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, 
 
 // 4 waves of 32 rows share the table's tiles, double-buffered
 template <typename T, int DP, bool DX>
-__global__ __launch_bounds__(VS_THREADS) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
+__global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= (DX ? 256 : 512) ? 2 : 1)) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Ti = VocabTile<T, DP>;
     T* tiles = reinterpret_cast<T*>(lds);
@@ -135,14 +129,19 @@ __global__ __launch_bounds__(VS_THREADS) void vocab_rows_kernel(VocabView a, Voc
     write_parts<T, DP, DX>(p, sp, a.N, n, on, o);
 }
 
-// up to 32 rows: every wave is a split of its own with tiles of its own
+// Up to 32 rows: every wave takes tiles of its own, the four join before they leave their part.
+template <typename T, int DP>
+struct FewLds {
+    static constexpr size_t tiles = 4 * 32 * DP * sizeof(T), join = 4 * 32 * (DP + 4) * sizeof(float), first = tiles > join ? tiles : join;
+    static constexpr size_t all = first + 4 * 32 * 2 * sizeof(float) + 4 * 32 * sizeof(float);      // + statistics + bias
+};
 template <typename T, int DP, bool DX>
-__global__ __launch_bounds__(VS_THREADS) void vocab_few_kernel(VocabView a, VocabParts p) {
+__global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void vocab_few_kernel(VocabView a, VocabParts p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sp = blockIdx.x * 4 + wave;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sp = blockIdx.x;
     T* tile = reinterpret_cast<T*>(lds) + wave * 32 * DP;
-    float* bias = reinterpret_cast<float*>(reinterpret_cast<T*>(lds) + 4 * 32 * DP) + wave * 32;
-    if (sp >= p.splits) return;
+    float* stats = reinterpret_cast<float*>(lds + FewLds<T, DP>::first);
+    float* bias = stats + 4 * 32 * 2 + wave * 32;
     const int64_t n = lane & 31, v0 = sp * p.each, v1 = min(a.V, v0 + p.each);
     const int chunks = a.D / Tile<T, DP>::PER;
     const bool on = n < a.N;
@@ -156,70 +155,98 @@ __global__ __launch_bounds__(VS_THREADS) void vocab_few_kernel(VocabView a, Voca
         ws.fetch((const T*)a.w, a.w_ld, v, v1, chunks, lane);
         if (a.b != nullptr && lane < 32) bv = v + lane < v1 ? LOG2E * a.b[v + lane] : 0.f;
     };
-    if (v0 < v1) fetch(v0);
-    for (int64_t v = v0; v < v1; v += 32) {
+    int64_t v = v0 + 32 * wave;
+    if (v < v1) fetch(v);
+    for (; v < v1; v += 128) {
         __builtin_amdgcn_wave_barrier();
         ws.store(tile, lane);
         if (a.b != nullptr && lane < 32) bias[lane] = bv;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (v + 32 < v1) fetch(v + 32);
+        if (v + 128 < v1) fetch(v + 128);
         vocab_step<T, DP, 1, DX>(tile, a.b != nullptr ? bias : nullptr, x, v, v1, label, o);
     }
-    write_parts<T, DP, DX>(p, sp, a.N, n, on, o);
+    if (DX) {
+        float m, e, w[DP / 8];
+        join_waves<T, DP>(o, reinterpret_cast<float*>(lds), stats, m, e, w);
+        const int row = threadIdx.x >> 3, part = threadIdx.x & 7;
+        if (row >= a.N) return;
+        const int64_t at = (int64_t)sp * a.N + row;
+        if (part == 0) { p.m[at] = m; p.e[at] = e; }
+#pragma unroll
+        for (int d = 0; d < DP / 8; d += 4) *reinterpret_cast<f32x4*>(p.acc + at * DP + part * (DP / 8) + d) = f32x4{w[d], w[d + 1], w[d + 2], w[d + 3]};
+        return;
+    }
+    const float e = both_sum(o.l);
+    if (lane < 32) {
+        stats[(wave * 32 + lane) * 2] = o.m;
+        stats[(wave * 32 + lane) * 2 + 1] = e;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x >= a.N) return;
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m = fmaxf(m, stats[(k * 32 + threadIdx.x) * 2]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum = fmaf(stats[(k * 32 + threadIdx.x) * 2 + 1], exp2f(stats[(k * 32 + threadIdx.x) * 2] - (m == -INFINITY ? 0.f : m)), sum);
+    p.m[(int64_t)sp * a.N + threadIdx.x] = m;
+    p.e[(int64_t)sp * a.N + threadIdx.x] = sum;
 }
 
-// Joins the splits and adds the label's column: one wave a row.
+// Joins the splits and adds the label's column: one block a row, thread = (4 columns, slice of the splits) for dx.
 template <typename T, int DP, bool DX>
 __global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, VocabParts p, float* loss, float* lse, T* dx, int64_t dx_ld, int32_t* status) {
-    const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (n >= a.N) return;
+    __shared__ float red[3][4];
+    __shared__ f32x4 cols[VS_THREADS];
+    const int64_t n = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int label = a.labels[n];
     const bool on = label >= 0 && label < a.V;
-    if (label >= a.V && lane == 0 && status != nullptr) { status[0] = 1; status[1] = label; }
+    if (label >= a.V && tid == 0 && status != nullptr) { status[0] = 1; status[1] = label; }
     const T* x = (const T*)a.x + n * a.x_ld;
     const T* w = (const T*)a.w + (on ? label : 0) * a.w_ld;
-    float mine = -INFINITY;                                             // the label's logit, base 2
-    if (on) {
-        float z = 0.f;
-        for (int d = lane; d < a.D; d += 64) z = fmaf(to_f32(x[d]), to_f32(w[d]), z);
-        z = wave_sum(z);
-        mine = LOG2E * (a.b != nullptr ? z + a.b[label] : z);
-    }
-    float m = mine;
-    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.m[(int64_t)s * a.N + n]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    float z = on && tid < a.D ? to_f32(x[tid]) * to_f32(w[tid]) : 0.f, m = -INFINITY;
+    for (int s = tid; s < p.splits; s += VS_THREADS) m = fmaxf(m, p.m[(int64_t)s * a.N + n]);
+    z = wave_sum(z);
+    m = wave_max(m);
+    if (lane == 0) { red[0][wave] = z; red[1][wave] = m; }
+    __syncthreads();
+    z = (red[0][0] + red[0][1]) + (red[0][2] + red[0][3]);
+    const float mine = on ? LOG2E * (a.b != nullptr ? z + a.b[label] : z) : -INFINITY;           // the label's logit, base 2
+    m = fmaxf(mine, fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3])));
     const float base = m == -INFINITY ? 0.f : m;
     float e = 0.f;
-    for (int s = lane; s < p.splits; s += 64) e = fmaf(p.e[(int64_t)s * a.N + n], exp2f(p.m[(int64_t)s * a.N + n] - base), e);
+    for (int s = tid; s < p.splits; s += VS_THREADS) e = fmaf(p.e[(int64_t)s * a.N + n], exp2f(p.m[(int64_t)s * a.N + n] - base), e);
     e = wave_sum(e);
+    if (lane == 0) red[2][wave] = e;
+    f32x4 acc = {};
+    constexpr int COLS = DP / 4, SLICES = VS_THREADS / COLS;
+    const int col = tid % COLS * 4, slice = tid / COLS;
+    if (DX && on)
+#pragma unroll 4
+        for (int s = slice; s < p.splits; s += SLICES)
+            acc += exp2f(p.m[(int64_t)s * a.N + n] - base) * *reinterpret_cast<const f32x4*>(p.acc + ((int64_t)s * a.N + n) * DP + col);
+    if (DX) cols[tid] = acc;
+    __syncthreads();
+    e = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
     const float all = e + (on ? exp2f(mine - base) : 0.f);
-    if (lane == 0) {
+    if (tid == 0) {
         if (lse != nullptr) lse[n] = LN2 * base + logf(all);
         loss[n] = !on ? 0.f : mine == m ? log1pf(e) : LN2 * (base - mine) + logf(all);
     }
-    if (!DX) return;
+    if (!DX || slice > 0 || col >= a.D) return;
+    for (int s = 1; s < SLICES; ++s) acc += cols[s * COLS + tid];
     const float c = on ? a.scale * (a.row_scale != nullptr ? a.row_scale[n] : 1.f) : 0.f;
-    constexpr int PER = DP > 64 ? DP / 64 : 1;
-    if (lane * PER >= a.D) return;
-    float acc[PER] = {};
-    if (on)
-        for (int s = 0; s < p.splits; ++s) {
-            const float f = exp2f(p.m[(int64_t)s * a.N + n] - base);
+    float to[4];
 #pragma unroll
-            for (int d = 0; d < PER; ++d) acc[d] = fmaf(p.acc[((int64_t)s * a.N + n) * DP + lane * PER + d], f, acc[d]);
-        }
-#pragma unroll
-    for (int d = 0; d < PER; ++d)
-        if (lane * PER + d < a.D) dx[n * dx_ld + lane * PER + d] = (T)(on ? c * (acc[d] - e * to_f32(w[lane * PER + d])) / all : 0.f);
+    for (int d = 0; d < 4; ++d) to[d] = on ? c * (acc[d] - e * to_f32(w[col + d])) / all : 0.f;
+    Mma<T>::store4(dx + n * dx_ld + col, to[0], to[1], to[2], to[3]);
 }
 
 // ---- dw, db: 32 table rows a wave, over the rows of x ---------------------------------------------------------------------------------
 // With more than one split (a short vocabulary): part [splits][V][DP], part_b [splits][V], joined by vocab_dw_join_kernel.
 template <typename T, int DP>
-__global__ __launch_bounds__(VS_THREADS) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
+__global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
                                                               int splits, int each, int table_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Ti = VocabTile<T, DP>;
@@ -355,8 +382,8 @@ static VocabPlan plan_fwd(int N, int64_t V) {
     VocabPlan p;
     p.few = N <= 32;
     p.row_blocks = p.few ? 1 : ceil_div(N, 128);
-    const int64_t want = p.few ? 2048 : (512 + p.row_blocks - 1) / p.row_blocks, most = p.few ? (V + 63) / 64 : (V + 255) / 256;
-    p.each = round_up((V + std::min(want, most) - 1) / std::min(want, most), p.few ? 32 : 64);
+    const int64_t want = (512 + p.row_blocks - 1) / p.row_blocks, cut = std::min(want, (V + 255) / 256);
+    p.each = round_up((V + cut - 1) / cut, 64);
     p.splits = (int)((V + p.each - 1) / p.each);
     return p;
 }
@@ -390,12 +417,12 @@ static int launch_fwd(const VocabView& a, float* loss, float* lse, void* dx, int
     const VocabParts p{ws, ws + rows, ws + round_up(2 * rows, 4), f.splits, f.each};
     DCTR_REQUIRE((int64_t)f.row_blocks * f.splits <= INT32_MAX, "vocab softmax: too many blocks for one launch");
     if (f.few)
-        vocab_few_kernel<T, DP, DX><<<ceil_div(f.splits, 4), VS_THREADS, 4 * (32 * DP * sizeof(T) + 32 * sizeof(float)), st>>>(a, p);
+        vocab_few_kernel<T, DP, DX><<<f.splits, VS_THREADS, FewLds<T, DP>::all, st>>>(a, p);
     else
         vocab_rows_kernel<T, DP, DX><<<(unsigned)(f.row_blocks * f.splits), VS_THREADS,
                                        2 * (VocabTile<T, DP>::SIZE * sizeof(T) + VocabTile<T, DP>::ROWS * sizeof(float)), st>>>(a, p, f.row_blocks);
     DCTR_LAUNCH_CHECK();
-    vocab_join_kernel<T, DP, DX><<<ceil_div(a.N, 4), VS_THREADS, 0, st>>>(a, p, loss, lse, (T*)dx, dx_ld, status);
+    vocab_join_kernel<T, DP, DX><<<a.N, VS_THREADS, 0, st>>>(a, p, loss, lse, (T*)dx, dx_ld, status);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
