@@ -201,3 +201,19 @@ def test_gradients_against_differences(dev):
         slope = (ends[0] - ends[1]) / (2 * step)
         mine = (d[grad][:rows, :width].double() * way[:rows, :width].double()).sum().item()
         assert abs(slope - mine) <= 2e-3 * max(1.0, abs(mine)), (name, slope, mine)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,causal", [(4, 4, 16, False), (4, 2, 40, True), (8, 4, 64, True), (4, 4, 128, False)])
+def test_short_segments_in_number(dtype, heads, kv_heads, dim, causal, dev):
+    """More than 1024 (segment, head) pairs of short lists: a wave has each to itself."""
+    q, k = ragged(21, 330, 45), ragged(22, 330, 90)
+    start = [max(0, m - n) for n, m in zip(q, k)]
+    run(AttentionCase(dtype, q, k, heads, kv_heads, dim, causal=causal, boundaries=[-40, -8, -3, -1, 0, 2, 20], q_start=start, keep=lambda j: j % 9 != 4, seed=31), dev)
+    run(AttentionCase(dtype, q, k, heads, kv_heads, dim, causal=causal, seed=32), dev)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_long_histories_of_uneven_length_among_many(dtype, dev):
+    k = [9000 if i == 5 else 3 * i for i in range(40)]
+    run(AttentionCase(dtype, [1] * 40, k, 8, 2, 32, boundaries=[-64, -8, 0, 8], q_start=[max(0, n - 1) for n in k], seed=33), dev, ("out", "lse"))

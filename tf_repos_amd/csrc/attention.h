@@ -78,8 +78,15 @@ inline int rel_reach(const dctr_attention* a) {         // entries of a table ov
     return a->n_buckets > 1 ? a->boundaries[a->n_buckets - 2] - a->boundaries[0] + 2 * REL_PAD : 0;
 }
 
+// Items (32 rows of a segment and head) that are many and short go to a wave each, without barriers or joins; fewer or longer ones share a
+// block's waves.  (f32 heads wider than 64 would spill; a wave's own bias tables have to fit beside the tiles.)
+inline bool attn_solo(const dctr_attention* a, int64_t items) {
+    return items >= 1024 && a->max_k <= 512 && !(a->dtype == DCTR_TYPE_F32 && a->head_dim > 64) &&
+           a->n_buckets * std::min(a->heads / a->kv_heads, 32) <= 1024 && rel_reach(a) <= 512;
+}
+
 // ---- launchers (attention_fwd.hip, attention_bwd.hip): DP = 32, 64 or 128 by head_dim
-struct AttnSplit { int row_blocks, splits; };           // the forward's form for few query rows a key head (splits = 0: the other form)
+struct AttnSplit { int row_blocks, splits; bool solo; };           // the forward's form for few query rows a key head (splits = 0: the other form)
 AttnSplit attn_split(const dctr_attention* a);
 int64_t attn_fwd_workspace(const dctr_attention* a);      // bytes
 int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st);

@@ -11,12 +11,15 @@ namespace dctr {
 
 constexpr int BWD_THREADS = 256;
 
-// keys of a query-side tile: QW waves share the rows' work, 4 / QW the tile's keys
-template <typename T, int DP, int QW>
+// Query-side forms: ROWS a block's waves take 32 rows each and share 64-key tiles; SPLIT the waves take 32-key tiles of their own of the same 32
+// rows and add up at the end; SOLO a wave has 32 rows to itself.
+enum { ROWS = 0, SPLIT = 1, SOLO = 2 };
+
+template <typename T, int DP, int FORM>
 struct QuerySide {
-    static constexpr int KW = 4 / QW, NB = QW == 4 && sizeof(T) * DP <= 256 ? 2 : 1, KEYS = 32 * NB * KW, BUFS = QW == 4 ? 2 : 1;
-    static constexpr int TILE = KEYS * DP, ROWS = 32 * QW;
-    static constexpr size_t tiles = 2 * BUFS * TILE * sizeof(T), join = QW == 1 ? 4 * 32 * (DP + 4) * sizeof(float) : 0;
+    static constexpr int NB = FORM == ROWS && sizeof(T) * DP <= 256 ? 2 : 1, KEYS = 32 * NB, BUFS = FORM == ROWS ? 2 : 1, THREADS = FORM == ROWS ? 256 : 64;
+    static constexpr int TILE = KEYS * DP, ITEM_ROWS = FORM == ROWS ? 128 : 32;
+    static constexpr size_t tiles = (FORM == ROWS ? 1 : 4) * 2 * BUFS * TILE * sizeof(T), join = FORM == SPLIT ? 4 * 32 * (DP + 4) * sizeof(float) : 0;
     static constexpr size_t first = tiles > join ? tiles : join;
 };
 
@@ -25,34 +28,50 @@ struct QuerySide {
 __device__ __forceinline__ void lds_add(float* cell, float x) { __hip_atomic_fetch_add(cell, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 
 // part: [head][segment * row_blocks + row block][n_buckets] shares of the bias gradient, or null; delta [total_q, heads]
-template <typename T, int DP, int QW>
+template <typename T, int DP, int FORM>
 __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
                                                                  T* dq, int64_t dq_ld, float* delta, float* part, int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    using Q = QuerySide<T, DP, QW>;
+    using Q = QuerySide<T, DP, FORM>;
     constexpr int NB = Q::NB, TILE = Q::TILE;
     // For bf16 <do, out> is off by the rounding of `out`, an error that all of a row's ds share.  The walk sums p dp over every key, which is the
     // same number unrounded, and P K besides: dq is put right with (rounded - unrounded) P K at the end, the key side and the bias gradient take
     // the unrounded one.  (Measured: the relative error of dq and dk 0.0030 -> 0.0023 at 777 x 1531 x 128.)
     constexpr bool ROUNDED = sizeof(T) == 2;
-    T *kt = reinterpret_cast<T*>(lds), *vt = kt + Q::BUFS * TILE;
-    float* lut = reinterpret_cast<float*>(lds + Q::first);
+    constexpr bool OWN = FORM != ROWS;                                  // tiles of a wave's own
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-    const int rb = blockIdx.x % row_blocks, h = blockIdx.x / row_blocks % a.heads, b = blockIdx.x / row_blocks / a.heads;
+    T* kt = reinterpret_cast<T*>(lds) + (OWN ? wave * 2 * TILE : 0);
+    T* vt = kt + Q::BUFS * TILE;
+    const int64_t items = (int64_t)row_blocks * a.heads * a.n_seg, at_item = FORM == SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    const int item = (int)min(at_item, items - 1);
+    const int rb = item % row_blocks, h = item / row_blocks % a.heads, b = item / row_blocks / a.heads;
     const Segment s = load_segment(a, b);
-    const int row0 = rb * Q::ROWS;
+    const int row0 = rb * Q::ITEM_ROWS;
     float* share = part != nullptr ? part + ((int64_t)h * a.n_seg * row_blocks + (int64_t)b * row_blocks + rb) * a.rel.n : nullptr;
+    if (at_item >= items) return;                                       // (the forms that share have no such block)
     if (row0 >= s.nq) {
         if (share != nullptr)
-            for (int u = tid; u < a.rel.n; u += BWD_THREADS) share[u] = 0.f;
+            for (int u = FORM == SOLO ? lane : tid; u < a.rel.n; u += FORM == SOLO ? 64 : BWD_THREADS) share[u] = 0.f;
         return;
     }
-    const int wrow = row0 + 32 * (wave % QW), row = wrow + (lane & 31), first_key = 32 * NB * (wave / QW);
+    // one wave: what it wrote is what it reads, in program order; a block: a barrier
+    auto meet = [&] {
+        if (OWN) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            __syncthreads();
+        }
+    };
+    const int wrow = row0 + (OWN ? 0 : 32 * wave), row = wrow + (lane & 31);
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = a.scale * LOG2E;
     const int reach = rel_reach(a.rel);
-    float* cells = lut + reach;                                         // [4 waves][2 halves][reach], then 2 x 4 far sums
-    float* mine = cells + (2 * wave + half) * reach;
+    // SOLO: every wave's own table and 2 x reach cells; else one table, [4 waves][2 halves][reach] cells; 2 x 4 far sums
+    float* lut = reinterpret_cast<float*>(lds + Q::first) + (FORM == SOLO ? wave * 3 * reach : 0);
+    float* cells = lut + reach;
+    float* mine = cells + (FORM == SOLO ? half : 2 * wave + half) * reach;
+    const int loader = OWN ? lane : tid;
 
     RowFrags<T, DP> q, go;
     q.load((const T*)a.q + (s.q0 + row) * a.q_ld + (int64_t)h * a.dim, chunks, row < s.nq);
@@ -69,41 +88,36 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
         if (row < s.nq) {
             const float L = lse[(s.q0 + row) * a.heads + h];
             if (L != -INFINITY) minus_lse = -LOG2E * L;
-            if (!ROUNDED && wave < QW && half == 0) delta[(s.q0 + row) * a.heads + h] = dl;
+            if (!ROUNDED && (FORM != SPLIT || wave == 0) && half == 0) delta[(s.q0 + row) * a.heads + h] = dl;
         }
     }
 
     const T* K = (const T*)a.k + s.k0 * a.k_ld + (int64_t)(h / a.group) * a.dim;
     const T* V = (const T*)a.v + s.k0 * a.v_ld + (int64_t)(h / a.group) * a.dim;
     int keys = s.nk;
-    if (a.causal) keys = max(0, min(keys, s.start + min(row0 + Q::ROWS, s.nq)));
+    if (a.causal) keys = max(0, min(keys, s.start + min(row0 + Q::ITEM_ROWS, s.nq)));
     const int tiles = (keys + Q::KEYS - 1) / Q::KEYS;
     const bool busy = wrow < s.nq;
     const int wend = a.causal ? s.start + min(wrow + 32, s.nq) : keys;
 
     f32x16 acc[DP / 32] = {}, pk[ROUNDED ? DP / 32 : 1] = {};
     float far_ds[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, pdp = 0.f;     // [below the first boundary, from the last one on]
-    Staged<T, DP, Q::KEYS, BWD_THREADS> ks, vs;
-    uint64_t bits[2] = {0, 0};                                          // kept keys of the tile
-    uint8_t kept[2] = {0, 0};
+    Staged<T, DP, Q::KEYS, Q::THREADS> ks, vs;
+    uint64_t bits = 0;                                                  // kept keys of the tile
+    uint8_t kept = 0;
     auto fetch = [&](int j0) {
-        ks.fetch(K, a.k_ld, j0, s.nk, chunks, tid);
-        vs.fetch(V, a.v_ld, j0, s.nk, chunks, tid);
-#pragma unroll
-        for (int w = 0; w < (Q::KEYS + 63) / 64; ++w) {
-            const int j = j0 + 64 * w + lane;
-            kept[w] = 64 * w + lane < Q::KEYS && j < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j] : 1) : 0;
-        }
+        ks.fetch(K, a.k_ld, j0, s.nk, chunks, loader);
+        vs.fetch(V, a.v_ld, j0, s.nk, chunks, loader);
+        kept = lane < Q::KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
     auto store = [&](int buf) {
-#pragma unroll
-        for (int w = 0; w < (Q::KEYS + 63) / 64; ++w) bits[w] = __ballot(kept[w] != 0);
-        ks.store_kept(kt + buf * TILE, tid, bits);
-        vs.store_kept(vt + buf * TILE, tid, bits);
+        bits = __ballot(kept != 0);
+        ks.store(kt + buf * TILE, loader, bits);
+        vs.store(vt + buf * TILE, loader, bits);
     };
-    // p and dp of this wave's part of the tile at j0; returns whether the tile is near, `side` its far side otherwise
+    // p and dp of the tile at j0; returns whether it is near, `side` its far side otherwise
     auto pair = [&](const T* kb, const T* vb, int j0, uint64_t now, f32x16 (&p)[NB], f32x16 (&dp)[NB], int& cell, int& side) {
-        const int d0 = j0 + first_key - s.start - wrow;                 // the part's first key from the wave's first query
+        const int d0 = j0 - s.start - wrow;                             // the tile's first key from the wave's first query
         const bool near = near_tile(a.rel, d0 - 31, d0 + 32 * NB - 1);
         const int fb = a.rel.n > 0 && !near ? far_bucket(a.rel, d0 - 31) : 0;
         const float far = (a.rel.n > 0 && !near ? LOG2E * a.bias[fb * a.heads + h] : 0.f);
@@ -112,15 +126,15 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
         const bool cut = a.causal && d0 + 32 * NB - 1 > 0;
         uint64_t seen = now;
         if (cut) {
-            const int last = row + s.start - j0 - first_key;
+            const int last = row + s.start - j0;
             seen &= last < 0 ? 0ull : last >= 63 ? ~0ull : (2ull << last) - 1;
         }
         const bool hide = __any((uint32_t)(seen >> (32 * (NB - 1))) != ~0u || (uint32_t)seen != ~0u);
         seen = lane_bits(seen);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            p[k] = scores<T, DP>(kb, first_key + 32 * k, q);
-            dp[k] = scores<T, DP>(vb, first_key + 32 * k, go);
+            p[k] = scores<T, DP>(kb, 32 * k, q);
+            dp[k] = scores<T, DP>(vb, 32 * k, go);
         }
         if (near || hide) {
 #pragma unroll
@@ -140,34 +154,33 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
         }
         return near;
     };
-    auto part_bits = [&](const uint64_t (&w)[2]) { return first_key < 64 ? w[0] >> first_key : w[1] >> (first_key - 64); };
     // one walk over the tiles; `second`: only the near ones, for their cells
     auto walk = [&](bool second) {
-        int t = 0;
-        if (second) {                                                   // tiles before this one are far for every row of the block
+        int t = 0, last = tiles;
+        if (second) {                                                   // tiles before and behind these are far for every row of the block
             const int64_t from = (int64_t)a.rel.edge[0] + s.start + row0 - (Q::KEYS - 1);
+            const int64_t to = (int64_t)a.rel.edge[a.rel.n - 2] + s.start + row0 + Q::ITEM_ROWS - 1;      // (`near` goes by whole waves too)
             t = from <= 0 ? 0 : (int)min((int64_t)tiles, from / Q::KEYS);
-        }
-        int last = tiles;
-        if (second) {
-            const int64_t to = (int64_t)a.rel.edge[a.rel.n - 2] + s.start + row0 + Q::ROWS - 1;      // (`near` goes by whole waves too)
             last = to <= 0 ? 0 : (int)min((int64_t)tiles, (to + Q::KEYS - 1) / Q::KEYS);
         }
-        if (t >= last) return;
-        __syncthreads();
-        fetch(t * Q::KEYS);
+        constexpr int STEP = FORM == SPLIT ? 4 : 1;
+        if (FORM == SPLIT) t += wave;
+        meet();
+        if (t < last) fetch(t * Q::KEYS);
         if (!second) {                                                  // under the first tile's loads
-            for (int u = tid; u < reach; u += BWD_THREADS) lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
+            for (int u = FORM == SOLO ? lane : tid; u < reach; u += FORM == SOLO ? 64 : BWD_THREADS)
+                lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
             if (part != nullptr)
-                for (int u = tid; u < 8 * reach; u += BWD_THREADS) cells[u] = 0.f;
+                for (int u = FORM == SOLO ? lane : tid; u < (FORM == SOLO ? 2 : 8) * reach; u += FORM == SOLO ? 64 : BWD_THREADS) cells[u] = 0.f;
+            if (FORM == SPLIT) __syncthreads();
         }
-        store(0);
-        __syncthreads();
-        for (int n = 0; t < last; ++t, ++n) {
+        if (t < last) store(0);
+        meet();
+        for (int n = 0; t < last; t += STEP, ++n) {
             const int j0 = t * Q::KEYS, buf = Q::BUFS == 2 ? n & 1 : 0;
-            const uint64_t now = part_bits(bits);
-            if (t + 1 < last) fetch(j0 + Q::KEYS);
-            if (busy && j0 + first_key < wend) {
+            const uint64_t now = bits;
+            if (t + STEP < last) fetch(j0 + STEP * Q::KEYS);
+            if (busy && j0 < wend) {
                 const T *kb = kt + buf * TILE, *vb = vt + buf * TILE;
                 f32x16 p[NB], dp[NB];
                 int cell, side;
@@ -188,7 +201,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
                             const auto w = Mma<T>::pack(p[k]);
 #pragma unroll
                             for (int d = 0; d < DP / 32; ++d)
-                                pk[ROUNDED ? d : 0] = Mma<T>::template weigh<DP>(kb, first_key + 32 * k, 32 * d, w, pk[ROUNDED ? d : 0]);
+                                pk[ROUNDED ? d : 0] = Mma<T>::template weigh<DP>(kb, 32 * k, 32 * d, w, pk[ROUNDED ? d : 0]);
                         }
 #pragma unroll
                         for (int r = 0; r < 16; ++r) p[k][r] *= dp[k][r] - dl;
@@ -197,7 +210,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
                             for (int r = 0; r < 16; ++r) lds_add(mine + cell + 32 * k + reg_row(r), p[k][r]);
                         const auto w = Mma<T>::pack(p[k]);
 #pragma unroll
-                        for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(kb, first_key + 32 * k, 32 * d, w, acc[d]);
+                        for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(kb, 32 * k, 32 * d, w, acc[d]);
                     }
                 } else if (near) {
 #pragma unroll
@@ -206,61 +219,66 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
                         for (int r = 0; r < 16; ++r) lds_add(mine + cell + 32 * k + reg_row(r), p[k][r] * (dp[k][r] - dl));
                 }
             }
-            if (Q::BUFS == 1) __syncthreads();
-            if (t + 1 < last) store(Q::BUFS == 2 ? (n + 1) & 1 : 0);
-            __syncthreads();
+            if (Q::BUFS == 1) meet();
+            if (t + STEP < last) store(Q::BUFS == 2 ? (n + 1) & 1 : 0);
+            meet();
         }
     };
     walk(false);
 
     if (ROUNDED) {
         float exact = both_sum(pdp);
-        if (QW == 1) {                                                  // the waves hold different keys of the same rows
-            float* meet = reinterpret_cast<float*>(lds);
+        if (FORM == SPLIT) {                                            // the waves hold different keys of the same rows
+            float* sums = reinterpret_cast<float*>(lds);
             __syncthreads();
-            if (half == 0) meet[wave * 32 + lane] = exact;
+            if (half == 0) sums[wave * 32 + lane] = exact;
             __syncthreads();
-            exact = (meet[lane & 31] + meet[32 + (lane & 31)]) + (meet[64 + (lane & 31)] + meet[96 + (lane & 31)]);
+            exact = (sums[lane & 31] + sums[32 + (lane & 31)]) + (sums[64 + (lane & 31)] + sums[96 + (lane & 31)]);
+            __syncthreads();
         }
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) acc[d] += (dl - exact) * pk[ROUNDED ? d : 0];
         dl = exact;
-        if (wave < QW && half == 0 && row < s.nq) delta[(s.q0 + row) * a.heads + h] = dl;
+        if ((FORM != SPLIT || wave == 0) && half == 0 && row < s.nq) delta[(s.q0 + row) * a.heads + h] = dl;
     }
     if (part != nullptr) {
         if (ROUNDED && a.rel.n > 1) walk(true);                         // the near tiles again, for their distances' sums
-        float* fars = cells + 8 * reach;
+        float far_sum[2];
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-            float x = fmaf(-dl, far_p[side], far_ds[side]);
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-            if (lane == 0) fars[4 * side + wave] = x;
+        for (int side = 0; side < 2; ++side) far_sum[side] = wave_sum(fmaf(-dl, far_p[side], far_ds[side]));
+        constexpr int WAYS = FORM == SOLO ? 2 : 8;
+        float* fars = cells + 8 * reach;                                // (not SOLO's)
+        if (FORM != SOLO && lane == 0) {
+            fars[wave] = far_sum[0];
+            fars[4 + wave] = far_sum[1];
         }
-        __syncthreads();
-        // every distance's eight cells, then a wave a bucket
-        if (tiles > 0)
-            for (int u = tid; u < reach; u += BWD_THREADS) {
-                float x = cells[u];
+        if (FORM == SOLO) meet(); else __syncthreads();
+        if (FORM != SOLO) {
+            far_sum[0] = (fars[0] + fars[1]) + (fars[2] + fars[3]);
+            far_sum[1] = (fars[4] + fars[5]) + (fars[6] + fars[7]);
+        }
+        // every distance's cells, then a wave a bucket
+        for (int u = FORM == SOLO ? lane : tid; u < reach; u += FORM == SOLO ? 64 : BWD_THREADS) {
+            float x = cells[u];
 #pragma unroll
-                for (int w = 1; w < 8; ++w) x += cells[w * reach + u];
-                cells[u] = x;
-            }
-        __syncthreads();
-        for (int u = wave; u < a.rel.n; u += 4) {
+            for (int w = 1; w < WAYS; ++w) x += cells[w * reach + u];
+            cells[u] = x;
+        }
+        if (FORM == SOLO) meet(); else __syncthreads();
+        for (int u = FORM == SOLO ? 0 : wave; u < a.rel.n; u += FORM == SOLO ? 1 : 4) {
             float x = 0.f;
-            if (reach > 0 && tiles > 0) {
+            if (reach > 0) {
                 const int lo = u == 0 ? 0 : a.rel.edge[u - 1] - a.rel.edge[0] + REL_PAD, hi = u + 1 == a.rel.n ? reach : a.rel.edge[u] - a.rel.edge[0] + REL_PAD;
                 for (int d = lo + lane; d < hi; d += 64) x += cells[d];
                 x = wave_sum(x);
             }
-            if (u == 0) x += (fars[0] + fars[1]) + (fars[2] + fars[3]);
-            if (u > 0 && u + 1 == a.rel.n) x += (fars[4] + fars[5]) + (fars[6] + fars[7]);
+            if (u == 0) x += far_sum[0];
+            if (u > 0 && u + 1 == a.rel.n) x += far_sum[1];
             if (lane == 0) share[u] = x;
         }
     }
 
-    if (QW == 1) {                                                      // the four waves' sums meet
+    if (FORM == SPLIT) {                                                // the four waves' sums meet
         float* join = reinterpret_cast<float*>(lds);
         __syncthreads();
 #pragma unroll
@@ -314,36 +332,49 @@ __device__ __forceinline__ void sum_shares(const BiasShares& x, int n, int heads
 }
 
 // ---- key side ------------------------------------------------------------------------------------------------------------------------
-template <typename T, int DP>
+// A block's waves take 32 keys each and share the tiles of queries; ALONE: a wave has 32 keys, and 32-query tiles, to itself.
+template <typename T, int DP, bool ALONE>
 struct KeySide {
-    static constexpr int QT = sizeof(T) * DP <= 256 ? 64 : 32, TILE = QT * DP;      // queries of a tile
-    static constexpr size_t tiles = 2 * 2 * TILE * sizeof(T), stats = 2 * 2 * QT * sizeof(float);
+    static constexpr int QT = !ALONE && sizeof(T) * DP <= 256 ? 64 : 32, TILE = QT * DP, BUFS = ALONE ? 1 : 2, THREADS = ALONE ? 64 : 256;      // queries of a tile
+    static constexpr size_t tiles = (ALONE ? 4 : 1) * 2 * BUFS * TILE * sizeof(T), stats = (ALONE ? 4 : 1) * BUFS * 2 * QT * sizeof(float);
 };
 
-template <typename T, int DP>
-__global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout, int64_t dout_ld, T* dk,
-                                                                  int64_t dk_ld, T* dv, int64_t dv_ld, int key_blocks, BiasShares shares, int blocks) {
+template <typename T, int DP, bool ALONE>
+__global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout,
+                                                                                                   int64_t dout_ld, T* dk, int64_t dk_ld, T* dv, int64_t dv_ld,
+                                                                                                   int key_blocks, BiasShares shares, int blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    using Kd = KeySide<T, DP>;
+    using Kd = KeySide<T, DP, ALONE>;
     constexpr int QT = Kd::QT, TILE = Kd::TILE;
-    T *qt = reinterpret_cast<T*>(lds), *gt = qt + 2 * TILE;
-    float* stats = reinterpret_cast<float*>(lds + Kd::tiles);           // [buffer][-log2(e) lse, delta][QT]
-    float* lut = reinterpret_cast<float*>(lds + Kd::tiles + Kd::stats);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, kv_heads = a.heads / a.group;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, kv_heads = a.heads / a.group, loader = ALONE ? lane : tid;
+    T* qt = reinterpret_cast<T*>(lds) + (ALONE ? wave * 2 * TILE : 0);
+    T* gt = qt + Kd::BUFS * TILE;
+    float* stats = reinterpret_cast<float*>(lds + Kd::tiles) + (ALONE ? wave * 2 * QT : 0);       // [buffer][-log2(e) lse, delta][QT]
     if ((int)blockIdx.x >= blocks) {
-        sum_shares(shares, a.rel.n, a.heads, blockIdx.x - blocks, stats);
+        sum_shares(shares, a.rel.n, a.heads, blockIdx.x - blocks, reinterpret_cast<float*>(lds));
         return;
     }
-    const int kb = blockIdx.x % key_blocks, g = blockIdx.x / key_blocks % kv_heads, b = blockIdx.x / key_blocks / kv_heads;
+    const int64_t items = (int64_t)key_blocks * kv_heads * a.n_seg, at_item = ALONE ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    if (at_item >= items) return;                                       // (ALONE has no barriers)
+    const int item = (int)at_item, kb = item % key_blocks, g = item / key_blocks % kv_heads, b = item / key_blocks / kv_heads;
     const Segment s = load_segment(a, b);
-    const int key0 = kb * 128;
+    const int key0 = kb * (ALONE ? 32 : 128);
     if (key0 >= s.nk) return;
-    const int wkey = key0 + wave * 32, key = wkey + (lane & 31);
+    const int wkey = key0 + (ALONE ? 0 : wave * 32), key = wkey + (lane & 31);
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = a.scale * LOG2E;
-    const int reach = rel_reach(a.rel);
+    const int reach = rel_reach(a.rel), first_u = ALONE ? lane : tid, step_u = Kd::THREADS;
+    float* lut = reinterpret_cast<float*>(lds + Kd::tiles + Kd::stats) + (ALONE ? wave * 2 * reach : 0);
     int32_t* buckets = reinterpret_cast<int32_t*>(lut + reach);         // of every distance
-    for (int u = tid; u < reach; u += BWD_THREADS) buckets[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u);
+    for (int u = first_u; u < reach; u += step_u) buckets[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u);
+    auto meet = [&] {
+        if (ALONE) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            __syncthreads();
+        }
+    };
     const bool on = key < s.nk && (a.keep == nullptr || a.keep[s.k0 + key] != 0);
     RowFrags<T, DP> k, v;
     k.load((const T*)a.k + (s.k0 + key) * a.k_ld + (int64_t)g * a.dim, chunks, on);
@@ -355,39 +386,40 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
     const int first = a.causal ? max(0, key0 - s.start) / QT : 0;
     const int tiles = max(0, (s.nq + QT - 1) / QT - first);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
-    Staged<T, DP, QT, BWD_THREADS> qs, gs;
+    Staged<T, DP, QT, Kd::THREADS> qs, gs;
     float lv = -INFINITY, dv_ = 0.f;
     auto fetch = [&](int h, int i0) {
-        qs.fetch((const T*)a.q + s.q0 * a.q_ld + (int64_t)h * a.dim, a.q_ld, i0, s.nq, chunks, tid);
-        gs.fetch(dout + s.q0 * dout_ld + (int64_t)h * a.dim, dout_ld, i0, s.nq, chunks, tid);
+        qs.fetch((const T*)a.q + s.q0 * a.q_ld + (int64_t)h * a.dim, a.q_ld, i0, s.nq, chunks, loader);
+        gs.fetch(dout + s.q0 * dout_ld + (int64_t)h * a.dim, dout_ld, i0, s.nq, chunks, loader);
         lv = -INFINITY;
         dv_ = 0.f;
-        if (tid < QT && i0 + tid < s.nq) {
-            const float L = lse[(s.q0 + i0 + tid) * a.heads + h];
+        if (loader < QT && i0 + loader < s.nq) {
+            const float L = lse[(s.q0 + i0 + loader) * a.heads + h];
             lv = L == -INFINITY ? -INFINITY : -LOG2E * L;               // p = 2^-inf = 0 for a row that saw nothing, and behind the last row
-            dv_ = delta[(s.q0 + i0 + tid) * a.heads + h];
+            dv_ = delta[(s.q0 + i0 + loader) * a.heads + h];
         }
     };
     auto store = [&](int buf) {
-        qs.store(qt + buf * TILE, tid);
-        gs.store(gt + buf * TILE, tid);
-        if (tid < QT) {
-            stats[buf * 2 * QT + tid] = lv;
-            stats[buf * 2 * QT + QT + tid] = dv_;
+        qs.store(qt + buf * TILE, loader);
+        gs.store(gt + buf * TILE, loader);
+        if (loader < QT) {
+            stats[buf * 2 * QT + loader] = lv;
+            stats[buf * 2 * QT + QT + loader] = dv_;
         }
     };
     for (int h = g * a.group; h < (g + 1) * a.group; ++h) {
         if (tiles == 0) break;
-        __syncthreads();
+        meet();
         fetch(h, first * QT);
-        for (int u = tid; u < reach; u += BWD_THREADS) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
+        for (int u = first_u; u < reach; u += step_u) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
         store(0);
-        __syncthreads();
+        meet();
         for (int t = 0; t < tiles; ++t) {
             const int i0 = (first + t) * QT;
-            if (t + 1 < tiles) fetch(h, i0 + QT);
-            const T *qb = qt + (t & 1) * TILE, *gb = gt + (t & 1) * TILE;
-            const float* st = stats + (t & 1) * 2 * QT;
+            if (!ALONE && t + 1 < tiles) fetch(h, i0 + QT);             // (ALONE: the other waves cover the loads, the registers go further)
+            const int buf = Kd::BUFS == 2 ? t & 1 : 0;
+            const T *qb = qt + buf * TILE, *gb = gt + buf * TILE;
+            const float* st = stats + buf * 2 * QT;
             if (busy)
 #pragma unroll
                 for (int n = 0; n < QT / 32; ++n) {
@@ -429,8 +461,12 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
                         ak[d] = Mma<T>::template weigh<DP>(qb, 32 * n, 32 * d, wd, ak[d]);
                     }
                 }
-            if (t + 1 < tiles) store((t + 1) & 1);
-            __syncthreads();
+            if (ALONE) meet();
+            if (t + 1 < tiles) {
+                if (ALONE) fetch(h, i0 + QT);
+                store(ALONE ? 0 : (t + 1) & 1);
+            }
+            meet();
         }
     }
     if (key >= s.nk) return;
@@ -452,26 +488,44 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
 static int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
-// Rows of a query-side block: short query lists leave three of four row waves idle, so there the waves share the keys instead (not for f32
-// heads wider than 64, whose 128-key tiles do not fit the shared memory).
-static bool few_rows(const dctr_attention* a) { return a->max_q <= 64 && !(a->dtype == DCTR_TYPE_F32 && a->head_dim > 64); }
-static int row_blocks_of(const dctr_attention* a) { return ceil_div(a->max_q, few_rows(a) ? 32 : 128); }
+// Short query lists leave three of four row waves idle: there the waves share the keys instead, or are items of their own (not for f32 heads
+// wider than 64, whose registers do not suffice).
+static int query_form(const dctr_attention* a) {
+    if (a->max_q > 64 || (a->dtype == DCTR_TYPE_F32 && a->head_dim > 64)) return ROWS;
+    return attn_solo(a, (int64_t)ceil_div(a->max_q, 32) * a->heads * a->n_seg) ? SOLO : SPLIT;
+}
+static bool keys_alone(const dctr_attention* a) { return a->max_q <= 128 && attn_solo(a, (int64_t)ceil_div(a->max_k, 32) * a->kv_heads * a->n_seg); }
+static int row_blocks_of(const dctr_attention* a) { return ceil_div(a->max_q, query_form(a) == ROWS ? 128 : 32); }
 
 // delta, then the bias gradient's shares
 int64_t attn_bwd_workspace(const dctr_attention* a) {
     return 4 * (round_up(a->total_q * a->heads, 4) + (int64_t)a->heads * a->n_seg * row_blocks_of(a) * a->n_buckets);
 }
 
-template <typename T, int DP, int QW>
-static int launch_q(const dctr_attention* a, const AttnView& v, const void* out, int64_t out_ld, const float* lse, const void* dout, int64_t dout_ld,
-                    void* dq, int64_t dq_ld, float* delta, float* part, hipStream_t st) {
+template <typename T, int DP, int FORM>
+static int launch_q(const dctr_attention* a, const AttnView& v, const AttnGrads& x, float* delta, float* part, hipStream_t st) {
     const int row_blocks = row_blocks_of(a);
-    const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
-    DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
+    const int64_t items = (int64_t)row_blocks * a->heads * a->n_seg, blocks = FORM == SOLO ? (items + 3) / 4 : items;
+    DCTR_REQUIRE(items <= INT32_MAX, "attention: too many blocks for one launch");
     if (blocks == 0) return DCTR_OK;
-    const size_t lds = QuerySide<T, DP, QW>::first + sizeof(float) * (9 * rel_reach(a) + 8);
-    attn_bwd_q_kernel<T, DP, QW><<<(unsigned)blocks, BWD_THREADS, lds, st>>>(v, (const T*)out, out_ld, lse, (const T*)dout, dout_ld, (T*)dq, dq_ld, delta, part,
-                                                                             row_blocks);
+    const size_t lds = QuerySide<T, DP, FORM>::first + sizeof(float) * ((FORM == SOLO ? 12 : 9) * rel_reach(a) + 8);
+    attn_bwd_q_kernel<T, DP, FORM><<<(unsigned)blocks, BWD_THREADS, lds, st>>>(v, (const T*)x.out, x.out_ld, x.lse, (const T*)x.dout, x.dout_ld, (T*)x.dq, x.dq_ld,
+                                                                               delta, part, row_blocks);
+    DCTR_LAUNCH_CHECK();
+    return DCTR_OK;
+}
+
+template <typename T, int DP, bool ALONE>
+static int launch_kv(const dctr_attention* a, const AttnView& v, const AttnGrads& x, const float* delta, const float* part, hipStream_t st) {
+    using Kd = KeySide<T, DP, ALONE>;
+    const int key_blocks = ceil_div(a->max_k, ALONE ? 32 : 128), sums = part != nullptr ? a->heads : 0;
+    const int64_t items = (int64_t)key_blocks * a->kv_heads * a->n_seg, blocks = ALONE ? (items + 3) / 4 : items;
+    DCTR_REQUIRE(items + a->heads <= INT32_MAX, "attention: too many blocks for one launch");
+    if (blocks + sums == 0) return DCTR_OK;
+    const size_t lds = std::max(Kd::tiles + Kd::stats + sizeof(float) * (ALONE ? 8 : 2) * rel_reach(a), BWD_THREADS * sizeof(float));
+    attn_bwd_kv_kernel<T, DP, ALONE><<<(unsigned)(blocks + sums), BWD_THREADS, lds, st>>>(
+        v, x.lse, delta, (const T*)x.dout, x.dout_ld, (T*)x.dk, x.dk_ld, (T*)x.dv, x.dv_ld, key_blocks,
+        BiasShares{part, (int64_t)a->n_seg * row_blocks_of(a), x.dbias}, (int)blocks);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
@@ -479,22 +533,16 @@ static int launch_q(const dctr_attention* a, const AttnView& v, const void* out,
 template <typename T, int DP>
 static int launch_bwd(const dctr_attention* a, const AttnView& v, const AttnGrads& x, float* ws, hipStream_t st) {
     float *delta = ws, *part = x.dbias != nullptr ? ws + round_up(a->total_q * a->heads, 4) : nullptr;
-    constexpr bool wide = sizeof(T) == 4 && DP > 64;
-    if (!wide && few_rows(a))
-        DCTR_TRY((launch_q<T, DP, wide ? 4 : 1>(a, v, x.out, x.out_ld, x.lse, x.dout, x.dout_ld, x.dq, x.dq_ld, delta, part, st)));
+    constexpr bool wide = sizeof(T) == 4 && DP > 64;                    // (ROWS only)
+    const int form = query_form(a);
+    if (form == ROWS || wide)
+        DCTR_TRY((launch_q<T, DP, ROWS>(a, v, x, delta, part, st)));
+    else if (form == SPLIT)
+        DCTR_TRY((launch_q<T, DP, wide ? ROWS : SPLIT>(a, v, x, delta, part, st)));
     else
-        DCTR_TRY((launch_q<T, DP, 4>(a, v, x.out, x.out_ld, x.lse, x.dout, x.dout_ld, x.dq, x.dq_ld, delta, part, st)));
-    const int key_blocks = ceil_div(a->max_k, 128);
-    const int64_t blocks = (int64_t)key_blocks * a->kv_heads * a->n_seg;
-    DCTR_REQUIRE(blocks + a->heads <= INT32_MAX, "attention: too many blocks for one launch");
-    const int sums = part != nullptr ? a->heads : 0;
-    if (blocks + sums == 0) return DCTR_OK;
-    const size_t lds = KeySide<T, DP>::tiles + std::max<size_t>(KeySide<T, DP>::stats, BWD_THREADS * sizeof(float)) + sizeof(float) * 2 * rel_reach(a);
-    attn_bwd_kv_kernel<T, DP><<<(unsigned)(blocks + sums), BWD_THREADS, lds, st>>>(v, x.lse, delta, (const T*)x.dout, x.dout_ld, (T*)x.dk, x.dk_ld, (T*)x.dv,
-                                                                                   x.dv_ld, key_blocks,
-                                                                                   BiasShares{part, (int64_t)a->n_seg * row_blocks_of(a), x.dbias}, (int)blocks);
-    DCTR_LAUNCH_CHECK();
-    return DCTR_OK;
+        DCTR_TRY((launch_q<T, DP, wide ? ROWS : SOLO>(a, v, x, delta, part, st)));
+    if (!wide && keys_alone(a)) return launch_kv<T, DP, !wide>(a, v, x, delta, part, st);
+    return launch_kv<T, DP, false>(a, v, x, delta, part, st);
 }
 
 template <typename T>

@@ -10,6 +10,21 @@
 
 namespace dctr {
 
+// A wave's finished row: the lane pair's halves hold alternating groups of four columns.
+template <typename T, int DP>
+__device__ __forceinline__ void write_rows(const AttnView& a, const Softmax<T, DP>& o, int64_t qrow, int h, T* out, int64_t out_ld, float* lse) {
+    const int half = (threadIdx.x >> 5) & 1;
+    const float l = both_sum(o.l), inv = l == 0.f ? 0.f : 1.f / l;             // (0: no key was seen)
+    if (lse != nullptr && half == 0) lse[qrow * a.heads + h] = l == 0.f ? -INFINITY : LN2 * (o.m + log2f(l));
+    T* to = out + qrow * out_ld + (int64_t)h * a.dim + 4 * half;
+#pragma unroll
+    for (int k = 0; k < DP / 32; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (32 * k + 8 * i < a.dim)
+                Mma<T>::store4(to + 32 * k + 8 * i, o.acc[k][4 * i] * inv, o.acc[k][4 * i + 1] * inv, o.acc[k][4 * i + 2] * inv, o.acc[k][4 * i + 3] * inv);
+}
+
 constexpr int ROWS_THREADS = 256, ROWS_KEYS = 64;
 
 template <typename T, int DP>
@@ -99,19 +114,12 @@ __global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void
         if (t + 1 < tiles) store((t + 1) & 1);
         __syncthreads();
     }
-    if (row >= s.nq) return;
-    const float l = both_sum(o.l), inv = l == 0.f ? 0.f : 1.f / l;             // (0: no key was seen)
-    if (lse != nullptr && lane < 32) lse[(s.q0 + row) * a.heads + h] = l == 0.f ? -INFINITY : LN2 * (o.m + log2f(l));
-    T* to = out + (s.q0 + row) * out_ld + (int64_t)h * a.dim + 4 * (lane >> 5);
-#pragma unroll
-    for (int k = 0; k < DP / 32; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (32 * k + 8 * i < a.dim)
-                Mma<T>::store4(to + 32 * k + 8 * i, o.acc[k][4 * i] * inv, o.acc[k][4 * i + 1] * inv, o.acc[k][4 * i + 2] * inv, o.acc[k][4 * i + 3] * inv);
+    if (row < s.nq) write_rows<T, DP>(a, o, s.q0 + row, h, out, out_ld, lse);
 }
 
-// ---- split form ----------------------------------------------------------------------------------------------------------------------
+// ---- split form, solo form -----------------------------------------------------------------------------------------------------------
+// An item is 32 (query, head of the group) rows of a segment and key head.  Split: the block's waves, and the blocks of an item, share its keys.
+// Solo: a wave has an item to itself, nothing to join and nobody to wait for -- for short lists in number.
 constexpr int SPLIT_KEYS = 32, SPLIT_TILES = 16;                       // keys of a wave's tile, tiles below which a block is not split
 // shared memory: 4 waves' K and V tiles, in whose place the waves' results meet (rows of DP + 4 floats: no two rows start at the same bank)
 template <typename T, int DP>
@@ -132,40 +140,47 @@ __device__ __forceinline__ void finish_row(const AttnView& a, int64_t qrow, int 
         if (d0 + d < a.dim) Mma<T>::store4(to + d, o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
 }
 
-// part: [block item][split][32][DP + 2] (weighted sum, maximum, sum); not used when there is one split
-template <typename T, int DP>
+// Tiles of an item's keys, and how many of them a block takes.
+__device__ __forceinline__ int split_tiles(const AttnView& a, const Segment& s, int rb, int splits, int* each) {
+    int keys = s.nk;
+    if (a.causal) keys = max(0, min(keys, s.start + min(rb * 32 + 31, s.nq * a.group - 1) / a.group + 1));
+    const int tiles = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS;
+    *each = max(SPLIT_TILES, (tiles + splits - 1) / splits);
+    return tiles;
+}
+
+// part: [item][split][32][DP + 2] (weighted sum, maximum, sum); not used when there is one split, nor of splits behind the item's last tile
+template <typename T, int DP, bool SOLO>
 __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status, float* part,
                                                                                               AttnSplit cut) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using L = SplitLds<T, DP>;
-    constexpr int TILE = SPLIT_KEYS * DP;
+    constexpr int TILE = SPLIT_KEYS * DP, STEP = SOLO ? 1 : 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kv_heads = a.heads / a.group;
     T* kt = reinterpret_cast<T*>(lds) + wave * 2 * TILE;
     T* vt = kt + TILE;
-    float* join = reinterpret_cast<float*>(lds);
     float* stats = reinterpret_cast<float*>(lds + L::first);
-    const int sp = blockIdx.x % cut.splits, item = blockIdx.x / cut.splits;
+    const int64_t items = (int64_t)cut.row_blocks * kv_heads * a.n_seg, at_item = SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x / cut.splits;
+    const int sp = SOLO ? 0 : blockIdx.x % cut.splits, item = (int)min(at_item, items - 1);
     const int rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
     const Segment s = load_segment(a, b);
-    if (rb == 0 && g == 0 && sp == 0 && tid == 0) flag_segment(a, b, status);
+    if (rb == 0 && g == 0 && sp == 0 && (SOLO ? lane : tid) == 0) flag_segment(a, b, status);
     const int rows = s.nq * a.group, r0 = rb * 32;
-    if (r0 >= rows) return;
+    int each;
+    const int tiles = split_tiles(a, s, rb, cut.splits, &each), t1 = SOLO ? tiles : min(tiles, (sp + 1) * each);
+    const bool none = r0 >= rows || at_item >= items;
+    if (!SOLO && (none || (sp > 0 && sp * each >= tiles))) return;
     const int r = r0 + (lane & 31), i = r / a.group, hg = r % a.group, h = g * a.group + hg;
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = fabsf(a.scale) * LOG2E;
 
     RowFrags<T, DP> q;
-    q.load((const T*)a.q + (s.q0 + i) * a.q_ld + (int64_t)h * a.dim, chunks, r < rows);
+    q.load((const T*)a.q + (s.q0 + i) * a.q_ld + (int64_t)h * a.dim, chunks, !none && r < rows);
     if (a.scale < 0.f) q.negate();
 
     const T* K = (const T*)a.k + s.k0 * a.k_ld + (int64_t)g * a.dim;
     const T* V = (const T*)a.v + s.k0 * a.v_ld + (int64_t)g * a.dim;
     const int i0 = r0 / a.group, i1 = min(r0 + 31, rows - 1) / a.group;
-    int keys = s.nk;
-    if (a.causal) keys = max(0, min(keys, s.start + i1 + 1));
-    const int tiles = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS, each = max(SPLIT_TILES, (tiles + cut.splits - 1) / cut.splits);
-    const int t1 = min(tiles, (sp + 1) * each);
-
     Softmax<T, DP> o;
     Staged<T, DP, SPLIT_KEYS, 64> ks, vs;
     uint8_t kept = 0;
@@ -174,20 +189,20 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_spl
         vs.fetch(V, a.v_ld, j0, s.nk, chunks, lane);
         kept = lane < SPLIT_KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
-    int t = sp * each + wave;
+    int t = SOLO ? (none ? t1 : 0) : sp * each + wave;
     if (t < t1) fetch(t * SPLIT_KEYS);
 
-    // Bias, under the first loads: bucket of a distance, then its value for the row's head (a block's rows have min(group, 32) different ones)
-    const int wide = min(a.group, 32), col = a.group <= 32 ? hg : r - r0;
-    float* table = stats + 4 * 32 * 2;                                  // [n_buckets][wide]
-    int32_t* lut = reinterpret_cast<int32_t*>(table + a.rel.n * wide);
-    for (int u = tid; u < a.rel.n * wide; u += 256)
+    // Bias, under the first loads: bucket of a distance, then its value for the row's head (an item's rows have min(group, 32) different ones).
+    const int wide = min(a.group, 32), col = a.group <= 32 ? hg : r - r0, reach = rel_reach(a.rel);
+    int32_t* lut = reinterpret_cast<int32_t*>(stats + (SOLO ? 0 : 4 * 32 * 2));
+    float* table = reinterpret_cast<float*>(lut + reach) + (SOLO ? wave * a.rel.n * wide : 0);      // [n_buckets][wide]
+    for (int u = SOLO ? lane : tid; u < a.rel.n * wide; u += SOLO ? 64 : 256)
         table[u] = LOG2E * a.bias[u / wide * a.heads + g * a.group + (a.group <= 32 ? u % wide : (r0 + u % wide) % a.group)];
-    const int reach = rel_reach(a.rel);
-    if (near_tile(a.rel, sp * each * SPLIT_KEYS - s.start - i1, t1 * SPLIT_KEYS - 1 - s.start - i0))
+    if (SOLO ? reach > 0 : near_tile(a.rel, sp * each * SPLIT_KEYS - s.start - i1, t1 * SPLIT_KEYS - 1 - s.start - i0))
         for (int u = tid; u < reach; u += 256) lut[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * wide;
     if (a.rel.n > 0) __syncthreads();
-    for (; t < t1; t += 4) {
+    if (SOLO && none) return;
+    for (; t < t1; t += STEP) {
         const int j0 = t * SPLIT_KEYS;
         const uint64_t now = __ballot(kept != 0);
         // the tile is this wave's own: its reads of the last step are behind these writes in program order
@@ -196,7 +211,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_spl
         vs.store(vt, lane, now);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (t + 4 < t1) fetch((t + 4) * SPLIT_KEYS);
+        if (t + STEP < t1) fetch((t + STEP) * SPLIT_KEYS);
         f32x16 sc[1];
         sc[0] = scores<T, DP>(kt, 0, q);
         const int dmin = j0 - s.start - i1, dmax = j0 + SPLIT_KEYS - 1 - s.start - i0;
@@ -224,8 +239,12 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_spl
         o.template weigh<1>(vt, sc);
     }
 
+    if (SOLO) {
+        if (r < rows) write_rows<T, DP>(a, o, s.q0 + i, h, out, out_ld, lse);
+        return;
+    }
     float m, sum, w[DP / 8];
-    join_waves<T, DP>(o, join, stats, m, sum, w);
+    join_waves<T, DP>(o, reinterpret_cast<float*>(lds), stats, m, sum, w);
     const int mine = r0 + (tid >> 3);
     if (cut.splits == 1) {
         if (mine < rows) finish_row<T, DP>(a, s.q0 + mine / a.group, g * a.group + mine % a.group, tid, m, sum, w, out, out_ld, lse);
@@ -245,20 +264,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnView a, T* out, int6
     const Segment s = load_segment(a, b);
     const int mine = rb * 32 + r;
     if (mine >= s.nq * a.group) return;
+    int each;
+    const int tiles = split_tiles(a, s, rb, cut.splits, &each), splits = max(1, (tiles + each - 1) / each);      // that have left a part
     const int64_t step = 32 * (DP + 2);
     const float* p = part + ((int64_t)item * cut.splits * 32 + r) * (DP + 2);
     float m = -INFINITY;
-    for (int n = lane; n < cut.splits; n += 64) m = fmaxf(m, p[n * step + DP]);
+    for (int n = lane; n < splits; n += 64) m = fmaxf(m, p[n * step + DP]);
     m = wave_max(m);
     const float base = m == -INFINITY ? 0.f : m;
     constexpr int PER = DP > 64 ? 2 : 1;
     const int d0 = lane * PER < DP ? lane * PER : 0;
     float l = 0.f, o[PER] = {};
-    for (int n0 = 0; n0 < cut.splits; n0 += 64) {
+    for (int n0 = 0; n0 < splits; n0 += 64) {
         const int n = n0 + lane;
-        const float f = n < cut.splits ? exp2f(p[n * step + DP] - base) : 0.f;
-        if (n < cut.splits) l = fmaf(p[n * step + DP + 1], f, l);
-        const int many = min(64, cut.splits - n0);
+        const float f = n < splits ? exp2f(p[n * step + DP] - base) : 0.f;
+        if (n < splits) l = fmaf(p[n * step + DP + 1], f, l);
+        const int many = min(64, splits - n0);
         for (int k = 0; k < many; ++k) {
             const float w = __shfl(f, k);
 #pragma unroll
@@ -280,17 +301,18 @@ static int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
 AttnSplit attn_split(const dctr_attention* a) {
     const int64_t rows = (int64_t)a->max_q * (a->heads / a->kv_heads);
-    if (rows > 128) return {0, 0};
+    if (rows > 128) return {0, 0, false};
     const int64_t row_blocks = (rows + 31) / 32, items = row_blocks * a->kv_heads * a->n_seg;
-    if (items == 0) return {(int)row_blocks, 1};
+    if (items == 0) return {(int)row_blocks, 1, false};
+    if (attn_solo(a, items)) return {(int)row_blocks, 1, true};
     const int64_t most = (a->max_k + SPLIT_KEYS * SPLIT_TILES - 1) / (SPLIT_KEYS * SPLIT_TILES), want = (4096 + items - 1) / items;
-    return {(int)row_blocks, (int)std::max<int64_t>(1, std::min(most, want))};
+    return {(int)row_blocks, (int)std::max<int64_t>(1, std::min(most, want)), false};
 }
 
 template <typename T, int DP>
 static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st) {
     const AttnSplit cut = attn_split(a);
-    const int64_t table = a->n_buckets > 0 ? a->n_buckets * std::min<int64_t>(v.group, 32) + rel_reach(a) : 0;
+    const size_t table = sizeof(float) * a->n_buckets * std::min(v.group, 32), lut = sizeof(float) * rel_reach(a);
     if (cut.splits == 0) {
         const int row_blocks = ceil_div(a->max_q, 128);
         const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
@@ -304,7 +326,10 @@ static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int
     DCTR_REQUIRE(items * std::max(8, cut.splits) <= INT32_MAX, "attention: too many blocks for one launch");
     if (items == 0) return DCTR_OK;
     using L = SplitLds<T, DP>;
-    attn_split_kernel<T, DP><<<(unsigned)(items * cut.splits), 256, L::first + L::stats + table * sizeof(float), st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
+    if (cut.solo)
+        attn_split_kernel<T, DP, true><<<ceil_div(items, 4), 256, L::first + lut + 4 * table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
+    else
+        attn_split_kernel<T, DP, false><<<(unsigned)(items * cut.splits), 256, L::first + L::stats + lut + table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     DCTR_LAUNCH_CHECK();
     if (cut.splits > 1) {
         attn_join_kernel<T, DP><<<(unsigned)(items * 8), 256, 0, st>>>(v, (T*)out, out_ld, lse, ws, cut);

@@ -185,14 +185,6 @@ struct Staged {
             *reinterpret_cast<f32x4*>(tile + Tile<T, DP>::at(r, c)) = (rows >> r & 1) ? v[i] : f32x4{};
         }
     }
-    __device__ __forceinline__ void store_kept(T* tile, int tid, const uint64_t (&rows)[2]) const {      // up to 128 rows
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = tid + i * THREADS, r = at / CHUNKS, c = at % CHUNKS;
-            const uint64_t w = ROWS > 64 && r >= 64 ? rows[1] : rows[0];
-            *reinterpret_cast<f32x4*>(tile + Tile<T, DP>::at(r, c)) = (w >> (r & 63) & 1) ? v[i] : f32x4{};
-        }
-    }
 };
 
 // bits of 64 consecutive tile rows as register r of 32-row block `blk` sees them: bit reg_row(r) + 32 blk of the shifted word
