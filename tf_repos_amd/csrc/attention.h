@@ -18,7 +18,7 @@ namespace dctr {
 
 struct RelBuckets {                                     // passed by value: a captured graph keeps what it was captured with
     int32_t n;                                          // 0: no bias
-    int32_t edge[DCTR_MAX_REL_BUCKETS - 1];             // ascending; bucket(d) = #{u : edge[u] <= d}
+    int32_t edge[DCTR_MAX_REL_BUCKETS];                 // n - 1 ascending, then INT32_MAX; bucket(d) = #{u : edge[u] <= d}
 };
 
 struct AttnView {
@@ -35,16 +35,22 @@ struct AttnView {
 
 struct Segment { int64_t q0, k0; int nq, nk, start; };
 
+__device__ __forceinline__ int64_t cut_to(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
+
 // A segment's rows, kept inside the arrays whatever the offsets say (the forward reports the ones that had to be cut, see flag_segment).
 __device__ __forceinline__ Segment load_segment(const AttnView& a, int b) {
     Segment s;
-    auto cut = [](int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); };
-    s.q0 = cut(a.q_off[b], 0, a.total_q);
-    s.k0 = cut(a.k_off[b], 0, a.total_k);
-    s.nq = (int)cut(cut(a.q_off[b + 1], s.q0, a.total_q) - s.q0, 0, a.max_q);
-    s.nk = (int)cut(cut(a.k_off[b + 1], s.k0, a.total_k) - s.k0, 0, a.max_k);
-    s.start = a.q_start != nullptr ? (int)cut(a.q_start[b], -DCTR_MAX_POSITION, DCTR_MAX_POSITION) : 0;
+    s.q0 = cut_to(a.q_off[b], 0, a.total_q);
+    s.k0 = cut_to(a.k_off[b], 0, a.total_k);
+    s.nq = (int)cut_to(cut_to(a.q_off[b + 1], s.q0, a.total_q) - s.q0, 0, a.max_q);
+    s.nk = (int)cut_to(cut_to(a.k_off[b + 1], s.k0, a.total_k) - s.k0, 0, a.max_k);
+    s.start = a.q_start != nullptr ? (int)cut_to(a.q_start[b], -DCTR_MAX_POSITION, DCTR_MAX_POSITION) : 0;
     return s;
+}
+
+__device__ __forceinline__ int segment_keys(const AttnView& a, int b) {
+    const int64_t k0 = cut_to(a.k_off[b], 0, a.total_k);
+    return (int)cut_to(cut_to(a.k_off[b + 1], k0, a.total_k) - k0, 0, a.max_k);
 }
 
 __device__ __forceinline__ bool segment_is_bad(const AttnView& a, int b) {
@@ -69,7 +75,9 @@ __device__ __forceinline__ int far_bucket(const RelBuckets& r, int dmin) { retur
 // bucket of distance d; the edges come by scalar loads, one compare each for the whole wave
 __device__ __forceinline__ int bucket_of(const RelBuckets& r, int d) {
     int n = 0;
-    for (int u = 0; u + 1 < r.n; ++u) n += r.edge[u] <= d;
+    for (int u = 0; u + 1 < r.n; u += 8)
+#pragma unroll
+        for (int v = 0; v < 8; ++v) n += r.edge[u + v] <= d;
     return n;
 }
 __device__ __forceinline__ int rel_reach(const RelBuckets& r) { return r.n > 1 ? r.edge[r.n - 2] - r.edge[0] + 2 * REL_PAD : 0; }
@@ -86,7 +94,9 @@ inline bool attn_solo(const dctr_attention* a, int64_t items) {
 }
 
 // ---- launchers (attention_fwd.hip, attention_bwd.hip): DP = 32, 64 or 128 by head_dim
-struct AttnSplit { int row_blocks, splits; bool solo; };           // the forward's form for few query rows a key head (splits = 0: the other form)
+// The forward's form for few query rows a key head (splits = 0: the other form).  An item's keys are cut every `each` tiles, into `splits` at most;
+// chunks: no more pairs of segment and cut than these.
+struct AttnSplit { int row_blocks, splits, each, chunks; bool solo; };
 AttnSplit attn_split(const dctr_attention* a);
 int64_t attn_fwd_workspace(const dctr_attention* a);      // bytes
 int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st);

@@ -58,7 +58,7 @@ static int make_view(const dctr_attention* a, const void* q, int q_ld, const voi
     *view = AttnView{q, k, v, q_ld, k_ld, v_ld, q_off, k_off, q_start, keep, bias, a->total_q, a->total_k, a->n_seg, a->heads,
                      a->heads / a->kv_heads, a->head_dim, a->max_q, a->max_k, a->causal != 0, a->scale, {}};
     view->rel.n = a->n_buckets;
-    for (int u = 0; u + 1 < a->n_buckets; ++u) view->rel.edge[u] = a->boundaries[u];
+    for (int u = 0; u < DCTR_MAX_REL_BUCKETS; ++u) view->rel.edge[u] = u + 1 < a->n_buckets ? a->boundaries[u] : INT32_MAX;
     return DCTR_OK;
 }
 

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void
 // ---- split form, solo form -----------------------------------------------------------------------------------------------------------
 // An item is 32 (query, head of the group) rows of a segment and key head.  Split: the block's waves, and the blocks of an item, share its keys.
 // Solo: a wave has an item to itself, nothing to join and nobody to wait for -- for short lists in number.
-constexpr int SPLIT_KEYS = 32, SPLIT_TILES = 16;                       // keys of a wave's tile, tiles below which a block is not split
+constexpr int SPLIT_KEYS = 32, SPLIT_TILES = 16;                       // keys of a wave's tile, tiles below which an item is not split
 // shared memory: 4 waves' K and V tiles, in whose place the waves' results meet (rows of DP + 4 floats: no two rows start at the same bank)
 template <typename T, int DP>
 struct SplitLds {
@@ -140,18 +140,41 @@ __device__ __forceinline__ void finish_row(const AttnView& a, int64_t qrow, int 
         if (d0 + d < a.dim) Mma<T>::store4(to + d, o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
 }
 
-// Tiles of an item's keys, and how many of them a block takes.
-__device__ __forceinline__ int split_tiles(const AttnView& a, const Segment& s, int rb, int splits, int* each) {
+// Tiles of an item's keys
+__device__ __forceinline__ int item_tiles(const AttnView& a, const Segment& s, int rb) {
     int keys = s.nk;
     if (a.causal) keys = max(0, min(keys, s.start + min(rb * 32 + 31, s.nq * a.group - 1) / a.group + 1));
-    const int tiles = (keys + SPLIT_KEYS - 1) / SPLIT_KEYS;
-    *each = max(SPLIT_TILES, (tiles + splits - 1) / splits);
-    return tiles;
+    return (keys + SPLIT_KEYS - 1) / SPLIT_KEYS;
+}
+
+// Which segment and which of its cuts chunk c is: a wave counts the segments' cuts, 64 segments at a time.  (A grid of segments x cuts of the
+// longest one would mostly start blocks without work: 3072 for 340 of work in a batch of 48 histories of 1..16384 keys, 57 us against 24.)
+__device__ __forceinline__ bool find_chunk(const AttnView& a, const AttnSplit& cut, int c, int* b, int* sp) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int b0 = 0; b0 < a.n_seg; b0 += 64) {
+        const int mine = b0 + lane < a.n_seg ? max(1, (segment_keys(a, b0 + lane) + cut.each * SPLIT_KEYS - 1) / (cut.each * SPLIT_KEYS)) : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto, o);
+            if (lane >= o) upto += x;
+        }
+        const uint64_t past = __ballot(before + upto > c);
+        if (past != 0) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            *b = b0 + at;
+            *sp = c - before - __shfl(upto - mine, at);
+            return true;
+        }
+        before += __shfl(upto, 63);
+    }
+    return false;
 }
 
 // part: [item][split][32][DP + 2] (weighted sum, maximum, sum); not used when there is one split, nor of splits behind the item's last tile
 template <typename T, int DP, bool SOLO>
-__global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status, float* part,
+__global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 3 : 1)) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status, float* part,
                                                                                               AttnSplit cut) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using L = SplitLds<T, DP>;
@@ -160,16 +183,22 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_spl
     T* kt = reinterpret_cast<T*>(lds) + wave * 2 * TILE;
     T* vt = kt + TILE;
     float* stats = reinterpret_cast<float*>(lds + L::first);
-    const int64_t items = (int64_t)cut.row_blocks * kv_heads * a.n_seg, at_item = SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x / cut.splits;
-    const int sp = SOLO ? 0 : blockIdx.x % cut.splits, item = (int)min(at_item, items - 1);
-    const int rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
+    const int64_t items = (int64_t)cut.row_blocks * kv_heads * a.n_seg, at_item = SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    int rb, g, b, sp = 0, item;
+    if (SOLO || cut.splits == 1) {
+        item = (int)min(at_item, items - 1);
+        rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
+    } else {
+        rb = blockIdx.x % cut.row_blocks, g = blockIdx.x / cut.row_blocks % kv_heads;
+        if (!find_chunk(a, cut, blockIdx.x / cut.row_blocks / kv_heads, &b, &sp)) return;
+        item = (b * kv_heads + g) * cut.row_blocks + rb;
+    }
     const Segment s = load_segment(a, b);
     if (rb == 0 && g == 0 && sp == 0 && (SOLO ? lane : tid) == 0) flag_segment(a, b, status);
     const int rows = s.nq * a.group, r0 = rb * 32;
-    int each;
-    const int tiles = split_tiles(a, s, rb, cut.splits, &each), t1 = SOLO ? tiles : min(tiles, (sp + 1) * each);
-    const bool none = r0 >= rows || at_item >= items;
-    if (!SOLO && (none || (sp > 0 && sp * each >= tiles))) return;
+    const int tiles = item_tiles(a, s, rb), t0 = sp * cut.each, t1 = cut.splits == 1 ? tiles : min(tiles, t0 + cut.each);
+    const bool none = r0 >= rows || (SOLO && at_item >= items);
+    if (!SOLO && (none || (sp > 0 && t0 >= tiles))) return;
     const int r = r0 + (lane & 31), i = r / a.group, hg = r % a.group, h = g * a.group + hg;
     const int chunks = a.dim / Tile<T, DP>::PER;
     const float scale = fabsf(a.scale) * LOG2E;
@@ -189,7 +218,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_spl
         vs.fetch(V, a.v_ld, j0, s.nk, chunks, lane);
         kept = lane < SPLIT_KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
-    int t = SOLO ? (none ? t1 : 0) : sp * each + wave;
+    int t = SOLO ? (none ? t1 : 0) : t0 + wave;
     if (t < t1) fetch(t * SPLIT_KEYS);
 
     // Bias, under the first loads: bucket of a distance, then its value for the row's head (an item's rows have min(group, 32) different ones).
@@ -198,7 +227,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_spl
     float* table = reinterpret_cast<float*>(lut + reach) + (SOLO ? wave * a.rel.n * wide : 0);      // [n_buckets][wide]
     for (int u = SOLO ? lane : tid; u < a.rel.n * wide; u += SOLO ? 64 : 256)
         table[u] = LOG2E * a.bias[u / wide * a.heads + g * a.group + (a.group <= 32 ? u % wide : (r0 + u % wide) % a.group)];
-    if (SOLO ? reach > 0 : near_tile(a.rel, sp * each * SPLIT_KEYS - s.start - i1, t1 * SPLIT_KEYS - 1 - s.start - i0))
+    if (SOLO ? reach > 0 : near_tile(a.rel, t0 * SPLIT_KEYS - s.start - i1, t1 * SPLIT_KEYS - 1 - s.start - i0))
         for (int u = tid; u < reach; u += 256) lut[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * wide;
     if (a.rel.n > 0) __syncthreads();
     if (SOLO && none) return;
@@ -264,8 +293,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnView a, T* out, int6
     const Segment s = load_segment(a, b);
     const int mine = rb * 32 + r;
     if (mine >= s.nq * a.group) return;
-    int each;
-    const int tiles = split_tiles(a, s, rb, cut.splits, &each), splits = max(1, (tiles + each - 1) / each);      // that have left a part
+    const int splits = max(1, (item_tiles(a, s, rb) + cut.each - 1) / cut.each);                                 // that have left a part
     const int64_t step = 32 * (DP + 2);
     const float* p = part + ((int64_t)item * cut.splits * 32 + r) * (DP + 2);
     float m = -INFINITY;
@@ -280,10 +308,19 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnView a, T* out, int6
         const float f = n < splits ? exp2f(p[n * step + DP] - base) : 0.f;
         if (n < splits) l = fmaf(p[n * step + DP + 1], f, l);
         const int many = min(64, splits - n0);
-        for (int k = 0; k < many; ++k) {
-            const float w = __shfl(f, k);
+        for (int k = 0; k < many; k += 8) {                             // eight loads under way (the last ones again where there are fewer)
+            float w[8], x[8][PER];
 #pragma unroll
-            for (int d = 0; d < PER; ++d) o[d] = fmaf(p[(n0 + k) * step + d0 + d], w, o[d]);
+            for (int e = 0; e < 8; ++e) {
+                const int n1 = min(n0 + k + e, splits - 1);
+                w[e] = k + e < many ? __shfl(f, k + e) : 0.f;
+#pragma unroll
+                for (int d = 0; d < PER; ++d) x[e][d] = p[n1 * step + d0 + d];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int d = 0; d < PER; ++d) o[d] = fmaf(x[e][d], w[e], o[d]);
         }
     }
     l = wave_sum(l);
@@ -301,12 +338,20 @@ static int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
 AttnSplit attn_split(const dctr_attention* a) {
     const int64_t rows = (int64_t)a->max_q * (a->heads / a->kv_heads);
-    if (rows > 128) return {0, 0, false};
-    const int64_t row_blocks = (rows + 31) / 32, items = row_blocks * a->kv_heads * a->n_seg;
-    if (items == 0) return {(int)row_blocks, 1, false};
-    if (attn_solo(a, items)) return {(int)row_blocks, 1, true};
-    const int64_t most = (a->max_k + SPLIT_KEYS * SPLIT_TILES - 1) / (SPLIT_KEYS * SPLIT_TILES), want = (4096 + items - 1) / items;
-    return {(int)row_blocks, (int)std::max<int64_t>(1, std::min(most, want)), false};
+    AttnSplit c{0, 0, 0, 0, false};
+    if (rows > 128) return c;
+    c.row_blocks = (int)((rows + 31) / 32);
+    c.splits = 1;
+    const int64_t items = (int64_t)c.row_blocks * a->kv_heads * a->n_seg, tiles = (a->max_k + SPLIT_KEYS - 1) / SPLIT_KEYS;
+    c.solo = attn_solo(a, items);
+    if (c.solo || items == 0 || items > 4096) return c;
+    // cuts of 512 keys (4 tiles a wave: about 1 us each, after 5 us for a block's start and its join), longer ones where the parts would pass 64 MB
+    const int64_t most = std::min<int64_t>((tiles + SPLIT_TILES - 1) / SPLIT_TILES, std::max<int64_t>(1, 8192 / items));
+    if (most <= 1) return c;
+    c.each = (int)((tiles + most - 1) / most);
+    c.splits = (int)((tiles + c.each - 1) / c.each);
+    c.chunks = (int)std::min<int64_t>((int64_t)c.splits * a->n_seg, a->total_k / ((int64_t)c.each * SPLIT_KEYS) + a->n_seg);
+    return c;
 }
 
 template <typename T, int DP>
@@ -323,13 +368,13 @@ static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int
         return DCTR_OK;
     }
     const int64_t items = (int64_t)cut.row_blocks * a->kv_heads * a->n_seg;
-    DCTR_REQUIRE(items * std::max(8, cut.splits) <= INT32_MAX, "attention: too many blocks for one launch");
+    DCTR_REQUIRE(items * 8 <= INT32_MAX, "attention: too many blocks for one launch");
     if (items == 0) return DCTR_OK;
     using L = SplitLds<T, DP>;
     if (cut.solo)
         attn_split_kernel<T, DP, true><<<ceil_div(items, 4), 256, L::first + lut + 4 * table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     else
-        attn_split_kernel<T, DP, false><<<(unsigned)(items * cut.splits), 256, L::first + L::stats + lut + table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
+        attn_split_kernel<T, DP, false><<<(unsigned)(cut.splits > 1 ? items / a->n_seg * cut.chunks : items), 256, L::first + L::stats + lut + table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     DCTR_LAUNCH_CHECK();
     if (cut.splits > 1) {
         attn_join_kernel<T, DP><<<(unsigned)(items * 8), 256, 0, st>>>(v, (T*)out, out_ld, lse, ws, cut);
