@@ -11,6 +11,7 @@
 //     dq_i = scale sum_j ds_ij k_j                dk_j = scale sum_ih ds_ij q_i
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "seq_mma.h"
 
@@ -62,6 +63,13 @@ __device__ __forceinline__ bool segment_is_bad(const AttnView& a, int b) {
 __device__ __forceinline__ void flag_segment(const AttnView& a, int b, int32_t* status) {
     if (status != nullptr && segment_is_bad(a, b)) { status[0] = 1; status[1] = b; }
 }
+
+// Operand kind: float arrays in planes (seq_mma.h) up to heads of 64; wider ones' planes pass the registers of the backward and the shared memory
+// of the forms whose waves have tiles of their own.
+template <typename T, int DP>
+using AttnKind = std::conditional_t<std::is_same_v<T, float> && DP <= 64, Split, T>;
+template <typename T, int DP>
+constexpr int attn_width = Mma<AttnKind<T, DP>>::BYTES * DP;           // bytes of a row in a tile
 
 // The bias of one tile of scores.  Distances below the first boundary all share bucket 0, those from the last boundary on the last bucket: only
 // a tile that reaches between the two ("near") looks values up, any other adds one number.  Tables hold log2(e) x the bias (the kernels'

@@ -17,9 +17,10 @@ enum { ROWS = 0, SPLIT = 1, SOLO = 2 };
 
 template <typename T, int DP, int FORM>
 struct QuerySide {
-    static constexpr int NB = FORM == ROWS && sizeof(T) * DP <= 256 ? 2 : 1, KEYS = 32 * NB, BUFS = FORM == ROWS ? 2 : 1, THREADS = FORM == ROWS ? 256 : 64;
-    static constexpr int TILE = KEYS * DP, ITEM_ROWS = FORM == ROWS ? 128 : 32;
-    static constexpr size_t tiles = (FORM == ROWS ? 1 : 4) * 2 * BUFS * TILE * sizeof(T), join = FORM == SPLIT ? 4 * 32 * (DP + 4) * sizeof(float) : 0;
+    using M = AttnKind<T, DP>;
+    static constexpr int NB = FORM == ROWS && attn_width<T, DP> <= 256 ? 2 : 1, KEYS = 32 * NB, BUFS = FORM == ROWS ? 2 : 1, THREADS = FORM == ROWS ? 256 : 64;
+    static constexpr int TILE = KEYS * Tile<M, DP>::STRIDE, ITEM_ROWS = FORM == ROWS ? 128 : 32;
+    static constexpr size_t tiles = (FORM == ROWS ? 1 : 4) * 2 * BUFS * KEYS * attn_width<T, DP>, join = FORM == SPLIT ? 4 * 32 * (DP + 4) * sizeof(float) : 0;
     static constexpr size_t first = tiles > join ? tiles : join;
 };
 
@@ -29,7 +30,7 @@ __device__ __forceinline__ void lds_add(float* cell, float x) { __hip_atomic_fet
 
 // part: [head][segment * row_blocks + row block][n_buckets] shares of the bias gradient, or null; delta [total_q, heads]
 template <typename T, int DP, int FORM>
-__global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
+__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
                                                                  T* dq, int64_t dq_ld, float* delta, float* part, int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Q = QuerySide<T, DP, FORM>;
@@ -37,11 +38,13 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
     // For bf16 <do, out> is off by the rounding of `out`, an error that all of a row's ds share.  The walk sums p dp over every key, which is the
     // same number unrounded, and P K besides: dq is put right with (rounded - unrounded) P K at the end, the key side and the bias gradient take
     // the unrounded one.  (Measured: the relative error of dq and dk 0.0030 -> 0.0023 at 777 x 1531 x 128.)
-    constexpr bool ROUNDED = sizeof(T) == 2;
+    using M = AttnKind<T, DP>;
+    using S = typename Mma<M>::Store;
+    constexpr bool ROUNDED = Mma<M>::ROUNDS;
     constexpr bool OWN = FORM != ROWS;                                  // tiles of a wave's own
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-    T* kt = reinterpret_cast<T*>(lds) + (OWN ? wave * 2 * TILE : 0);
-    T* vt = kt + Q::BUFS * TILE;
+    S* kt = reinterpret_cast<S*>(lds) + (OWN ? wave * 2 * TILE : 0);
+    S* vt = kt + Q::BUFS * TILE;
     const int64_t items = (int64_t)row_blocks * a.heads * a.n_seg, at_item = FORM == SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     const int item = (int)min(at_item, items - 1);
     const int rb = item % row_blocks, h = item / row_blocks % a.heads, b = item / row_blocks / a.heads;
@@ -64,7 +67,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
         }
     };
     const int wrow = row0 + (OWN ? 0 : 32 * wave), row = wrow + (lane & 31);
-    const int chunks = a.dim / Tile<T, DP>::PER;
+    const int chunks = a.dim / Tile<M, DP>::PER;
     const float scale = a.scale * LOG2E;
     const int reach = rel_reach(a.rel);
     // SOLO: every wave's own table and 2 x reach cells; else one table, [4 waves][2 halves][reach] cells; 2 x 4 far sums
@@ -73,17 +76,15 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
     float* mine = cells + (FORM == SOLO ? half : 2 * wave + half) * reach;
     const int loader = OWN ? lane : tid;
 
-    RowFrags<T, DP> q, go;
+    RowFrags<M, DP> q, go;
     q.load((const T*)a.q + (s.q0 + row) * a.q_ld + (int64_t)h * a.dim, chunks, row < s.nq);
     go.load(dout + (s.q0 + row) * dout_ld + (int64_t)h * a.dim, chunks, row < s.nq);
     float dl = 0.f, minus_lse = -INFINITY;                              // (a row that saw nothing: p = 2^-inf = 0)
     {
-        RowFrags<T, DP> o;
+        RowFrags<M, DP> o;
         o.load(out + (s.q0 + row) * out_ld + (int64_t)h * a.dim, chunks, row < s.nq);
 #pragma unroll
-        for (int c = 0; c < RowFrags<T, DP>::STEPS; ++c)
-#pragma unroll
-            for (int e = 0; e < Tile<T, DP>::PER; ++e) dl = fmaf(to_f32(go.c[c][e]), to_f32(o.c[c][e]), dl);
+        for (int c = 0; c < RowFrags<M, DP>::STEPS; ++c) dl = Mma<M>::product(go.c[c], o.c[c], dl);
         dl = both_sum(dl);
         if (row < s.nq) {
             const float L = lse[(s.q0 + row) * a.heads + h];
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
 
     f32x16 acc[DP / 32] = {}, pk[ROUNDED ? DP / 32 : 1] = {};
     float far_ds[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, pdp = 0.f;     // [below the first boundary, from the last one on]
-    Staged<T, DP, Q::KEYS, Q::THREADS> ks, vs;
+    Staged<M, DP, Q::KEYS, Q::THREADS> ks, vs;
     uint64_t bits = 0;                                                  // kept keys of the tile
     uint8_t kept = 0;
     auto fetch = [&](int j0) {
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
         vs.store(vt + buf * TILE, loader, bits);
     };
     // p and dp of the tile at j0; returns whether it is near, `side` its far side otherwise
-    auto pair = [&](const T* kb, const T* vb, int j0, uint64_t now, f32x16 (&p)[NB], f32x16 (&dp)[NB], int& cell, int& side) {
+    auto pair = [&](const S* kb, const S* vb, int j0, uint64_t now, f32x16 (&p)[NB], f32x16 (&dp)[NB], int& cell, int& side) {
         const int d0 = j0 - s.start - wrow;                             // the tile's first key from the wave's first query
         const bool near = near_tile(a.rel, d0 - 31, d0 + 32 * NB - 1);
         const int fb = a.rel.n > 0 && !near ? far_bucket(a.rel, d0 - 31) : 0;
@@ -133,8 +134,8 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
         seen = lane_bits(seen);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            p[k] = scores<T, DP>(kb, 32 * k, q);
-            dp[k] = scores<T, DP>(vb, 32 * k, go);
+            p[k] = scores<M, DP>(kb, 32 * k, q);
+            dp[k] = scores<M, DP>(vb, 32 * k, go);
         }
         if (near || hide) {
 #pragma unroll
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
             const uint64_t now = bits;
             if (t + STEP < last) fetch(j0 + STEP * Q::KEYS);
             if (busy && j0 < wend) {
-                const T *kb = kt + buf * TILE, *vb = vt + buf * TILE;
+                const S *kb = kt + buf * TILE, *vb = vt + buf * TILE;
                 f32x16 p[NB], dp[NB];
                 int cell, side;
                 const bool near = pair(kb, vb, j0, now, p, dp, cell, side);
@@ -198,19 +199,19 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
 #pragma unroll
                     for (int k = 0; k < NB; ++k) {
                         if (ROUNDED) {
-                            const auto w = Mma<T>::pack(p[k]);
+                            const auto w = Mma<M>::pack(p[k]);
 #pragma unroll
                             for (int d = 0; d < DP / 32; ++d)
-                                pk[ROUNDED ? d : 0] = Mma<T>::template weigh<DP>(kb, 32 * k, 32 * d, w, pk[ROUNDED ? d : 0]);
+                                pk[ROUNDED ? d : 0] = Mma<M>::template weigh<DP>(kb, 32 * k, 32 * d, w, pk[ROUNDED ? d : 0]);
                         }
 #pragma unroll
                         for (int r = 0; r < 16; ++r) p[k][r] *= dp[k][r] - dl;
                         if (!ROUNDED && part != nullptr && near)
 #pragma unroll
                             for (int r = 0; r < 16; ++r) lds_add(mine + cell + 32 * k + reg_row(r), p[k][r]);
-                        const auto w = Mma<T>::pack(p[k]);
+                        const auto w = Mma<M>::pack(p[k]);
 #pragma unroll
-                        for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(kb, 32 * k, 32 * d, w, acc[d]);
+                        for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(kb, 32 * k, 32 * d, w, acc[d]);
                     }
                 } else if (near) {
 #pragma unroll
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
 #pragma unroll
             for (int w = 1; w < 4; ++w) x += *reinterpret_cast<f32x4*>(join + (w * 32 + r) * (DP + 4) + d0 + d);
             x *= a.scale;
-            Mma<T>::store4(to + d, x[0], x[1], x[2], x[3]);
+            Mma<M>::store4(to + d, x[0], x[1], x[2], x[3]);
         }
         return;
     }
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (32 * k + 8 * i < a.dim)
-                Mma<T>::store4(to + 32 * k + 8 * i, acc[k][4 * i] * a.scale, acc[k][4 * i + 1] * a.scale, acc[k][4 * i + 2] * a.scale,
+                Mma<M>::store4(to + 32 * k + 8 * i, acc[k][4 * i] * a.scale, acc[k][4 * i + 1] * a.scale, acc[k][4 * i + 2] * a.scale,
                                acc[k][4 * i + 3] * a.scale);
 }
 
@@ -335,20 +336,23 @@ __device__ __forceinline__ void sum_shares(const BiasShares& x, int n, int heads
 // A block's waves take 32 keys each and share the tiles of queries; ALONE: a wave has 32 keys, and 32-query tiles, to itself.
 template <typename T, int DP, bool ALONE>
 struct KeySide {
-    static constexpr int QT = !ALONE && sizeof(T) * DP <= 256 ? 64 : 32, TILE = QT * DP, BUFS = ALONE ? 1 : 2, THREADS = ALONE ? 64 : 256;      // queries of a tile
-    static constexpr size_t tiles = (ALONE ? 4 : 1) * 2 * BUFS * TILE * sizeof(T), stats = (ALONE ? 4 : 1) * BUFS * 2 * QT * sizeof(float);
+    using M = AttnKind<T, DP>;
+    static constexpr int QT = !ALONE && attn_width<T, DP> <= 256 ? 64 : 32, TILE = QT * Tile<M, DP>::STRIDE, BUFS = ALONE ? 1 : 2, THREADS = ALONE ? 64 : 256;      // queries of a tile
+    static constexpr size_t tiles = (ALONE ? 4 : 1) * 2 * BUFS * QT * attn_width<T, DP>, stats = (ALONE ? 4 : 1) * BUFS * 2 * QT * sizeof(float);
 };
 
 template <typename T, int DP, bool ALONE>
-__global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout,
+__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout,
                                                                                                    int64_t dout_ld, T* dk, int64_t dk_ld, T* dv, int64_t dv_ld,
                                                                                                    int key_blocks, BiasShares shares, int blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Kd = KeySide<T, DP, ALONE>;
+    using M = AttnKind<T, DP>;
+    using S = typename Mma<M>::Store;
     constexpr int QT = Kd::QT, TILE = Kd::TILE;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, kv_heads = a.heads / a.group, loader = ALONE ? lane : tid;
-    T* qt = reinterpret_cast<T*>(lds) + (ALONE ? wave * 2 * TILE : 0);
-    T* gt = qt + Kd::BUFS * TILE;
+    S* qt = reinterpret_cast<S*>(lds) + (ALONE ? wave * 2 * TILE : 0);
+    S* gt = qt + Kd::BUFS * TILE;
     float* stats = reinterpret_cast<float*>(lds + Kd::tiles) + (ALONE ? wave * 2 * QT : 0);       // [buffer][-log2(e) lse, delta][QT]
     if ((int)blockIdx.x >= blocks) {
         sum_shares(shares, a.rel.n, a.heads, blockIdx.x - blocks, reinterpret_cast<float*>(lds));
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
     const int key0 = kb * (ALONE ? 32 : 128);
     if (key0 >= s.nk) return;
     const int wkey = key0 + (ALONE ? 0 : wave * 32), key = wkey + (lane & 31);
-    const int chunks = a.dim / Tile<T, DP>::PER;
+    const int chunks = a.dim / Tile<M, DP>::PER;
     const float scale = a.scale * LOG2E;
     const int reach = rel_reach(a.rel), first_u = ALONE ? lane : tid, step_u = Kd::THREADS;
     float* lut = reinterpret_cast<float*>(lds + Kd::tiles + Kd::stats) + (ALONE ? wave * 2 * reach : 0);
@@ -376,7 +380,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
         }
     };
     const bool on = key < s.nk && (a.keep == nullptr || a.keep[s.k0 + key] != 0);
-    RowFrags<T, DP> k, v;
+    RowFrags<M, DP> k, v;
     k.load((const T*)a.k + (s.k0 + key) * a.k_ld + (int64_t)g * a.dim, chunks, on);
     v.load((const T*)a.v + (s.k0 + key) * a.v_ld + (int64_t)g * a.dim, chunks, on);
     const bool all_on = __all(on);
@@ -386,7 +390,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
     const int first = a.causal ? max(0, key0 - s.start) / QT : 0;
     const int tiles = max(0, (s.nq + QT - 1) / QT - first);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
-    Staged<T, DP, QT, Kd::THREADS> qs, gs;
+    Staged<M, DP, QT, Kd::THREADS> qs, gs;
     float lv = -INFINITY, dv_ = 0.f;
     auto fetch = [&](int h, int i0) {
         qs.fetch((const T*)a.q + s.q0 * a.q_ld + (int64_t)h * a.dim, a.q_ld, i0, s.nq, chunks, loader);
@@ -418,7 +422,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
             const int i0 = (first + t) * QT;
             if (!ALONE && t + 1 < tiles) fetch(h, i0 + QT);             // (ALONE: the other waves cover the loads, the registers go further)
             const int buf = Kd::BUFS == 2 ? t & 1 : 0;
-            const T *qb = qt + buf * TILE, *gb = gt + buf * TILE;
+            const S *qb = qt + buf * TILE, *gb = gt + buf * TILE;
             const float* st = stats + buf * 2 * QT;
             if (busy)
 #pragma unroll
@@ -430,7 +434,7 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
                     const bool near = near_tile(a.rel, d0 - 31, d0 + 31);
                     const float far = a.rel.n > 0 && !near ? LOG2E * a.bias[far_bucket(a.rel, d0 - 31) * a.heads + h] : 0.f;
                     const bool cut = a.causal && d0 + 31 > 0;
-                    f32x16 p = scores<T, DP>(qb, 32 * n, k), dp = scores<T, DP>(gb, 32 * n, v);
+                    f32x16 p = scores<M, DP>(qb, 32 * n, k), dp = scores<M, DP>(gb, 32 * n, v);
                     f32x4 ml[4], dl[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -451,14 +455,14 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
 #pragma unroll
                         for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], scale, far + ml[r >> 2][r & 3]));
                     }
-                    const auto wp = Mma<T>::pack(p);
+                    const auto wp = Mma<M>::pack(p);
 #pragma unroll
                     for (int r = 0; r < 16; ++r) p[r] *= dp[r] - dl[r >> 2][r & 3];
-                    const auto wd = Mma<T>::pack(p);
+                    const auto wd = Mma<M>::pack(p);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) {
-                        av[d] = Mma<T>::template weigh<DP>(gb, 32 * n, 32 * d, wp, av[d]);
-                        ak[d] = Mma<T>::template weigh<DP>(qb, 32 * n, 32 * d, wd, ak[d]);
+                        av[d] = Mma<M>::template weigh<DP>(gb, 32 * n, 32 * d, wp, av[d]);
+                        ak[d] = Mma<M>::template weigh<DP>(qb, 32 * n, 32 * d, wd, ak[d]);
                     }
                 }
             if (ALONE) meet();
@@ -481,8 +485,8 @@ __global__ __launch_bounds__(BWD_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void 
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (32 * d + 8 * i < a.dim) {
-                Mma<T>::store4(tk + 32 * d + 8 * i, ak[d][4 * i] * a.scale, ak[d][4 * i + 1] * a.scale, ak[d][4 * i + 2] * a.scale, ak[d][4 * i + 3] * a.scale);
-                Mma<T>::store4(tv + 32 * d + 8 * i, av[d][4 * i], av[d][4 * i + 1], av[d][4 * i + 2], av[d][4 * i + 3]);
+                Mma<M>::store4(tk + 32 * d + 8 * i, ak[d][4 * i] * a.scale, ak[d][4 * i + 1] * a.scale, ak[d][4 * i + 2] * a.scale, ak[d][4 * i + 3] * a.scale);
+                Mma<M>::store4(tv + 32 * d + 8 * i, av[d][4 * i], av[d][4 * i + 1], av[d][4 * i + 2], av[d][4 * i + 3]);
             }
 }
 

@@ -11,8 +11,8 @@
 namespace dctr {
 
 // A wave's finished row: the lane pair's halves hold alternating groups of four columns.
-template <typename T, int DP>
-__device__ __forceinline__ void write_rows(const AttnView& a, const Softmax<T, DP>& o, int64_t qrow, int h, T* out, int64_t out_ld, float* lse) {
+template <typename T, typename M, int DP>
+__device__ __forceinline__ void write_rows(const AttnView& a, const Softmax<M, DP>& o, int64_t qrow, int h, T* out, int64_t out_ld, float* lse) {
     const int half = (threadIdx.x >> 5) & 1;
     const float l = both_sum(o.l), inv = l == 0.f ? 0.f : 1.f / l;             // (0: no key was seen)
     if (lse != nullptr && half == 0) lse[qrow * a.heads + h] = l == 0.f ? -INFINITY : LN2 * (o.m + log2f(l));
@@ -22,17 +22,21 @@ __device__ __forceinline__ void write_rows(const AttnView& a, const Softmax<T, D
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (32 * k + 8 * i < a.dim)
-                Mma<T>::store4(to + 32 * k + 8 * i, o.acc[k][4 * i] * inv, o.acc[k][4 * i + 1] * inv, o.acc[k][4 * i + 2] * inv, o.acc[k][4 * i + 3] * inv);
+                Mma<M>::store4(to + 32 * k + 8 * i, o.acc[k][4 * i] * inv, o.acc[k][4 * i + 1] * inv, o.acc[k][4 * i + 2] * inv, o.acc[k][4 * i + 3] * inv);
 }
 
-constexpr int ROWS_THREADS = 256, ROWS_KEYS = 64;
+constexpr int ROWS_THREADS = 256;
+template <typename T, int DP>
+constexpr int rows_keys = attn_width<T, DP> <= 384 ? 64 : 32;           // keys of a tile
 
 template <typename T, int DP>
-__global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void attn_rows_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status,
+__global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) void attn_rows_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status,
                                                                                                             int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int TILE = ROWS_KEYS * DP;
-    T *kt = reinterpret_cast<T*>(lds), *vt = kt + 2 * TILE;
+    using M = AttnKind<T, DP>;
+    using S = typename Mma<M>::Store;
+    constexpr int ROWS_KEYS = rows_keys<T, DP>, NB = ROWS_KEYS / 32, TILE = ROWS_KEYS * Tile<M, DP>::STRIDE;
+    S *kt = reinterpret_cast<S*>(lds), *vt = kt + 2 * TILE;
     float* lut = reinterpret_cast<float*>(vt + 2 * TILE);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int rb = blockIdx.x % row_blocks, h = blockIdx.x / row_blocks % a.heads, b = blockIdx.x / row_blocks / a.heads;
@@ -41,10 +45,10 @@ __global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void
     const int row0 = rb * 128;
     if (row0 >= s.nq) return;
     const int wrow = row0 + wave * 32, row = wrow + (lane & 31);
-    const int chunks = a.dim / Tile<T, DP>::PER;
+    const int chunks = a.dim / Tile<M, DP>::PER;
     const float scale = fabsf(a.scale) * LOG2E;
 
-    RowFrags<T, DP> q;
+    RowFrags<M, DP> q;
     q.load((const T*)a.q + (s.q0 + row) * a.q_ld + (int64_t)h * a.dim, chunks, row < s.nq);
     if (a.scale < 0.f) q.negate();                                      // the running maximum is taken before the scale
 
@@ -56,14 +60,14 @@ __global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void
     const bool busy = wrow < s.nq;
     const int wend = a.causal ? s.start + min(wrow + 32, s.nq) : keys;  // keys from here on are hidden from the whole wave
 
-    Softmax<T, DP> o;
-    Staged<T, DP, ROWS_KEYS, ROWS_THREADS> ks, vs;
+    Softmax<M, DP> o;
+    Staged<M, DP, ROWS_KEYS, ROWS_THREADS> ks, vs;
     uint8_t kept = 1;
     uint64_t bits = 0;
     auto fetch = [&](int j0) {
         ks.fetch(K, a.k_ld, j0, s.nk, chunks, tid);
         vs.fetch(V, a.v_ld, j0, s.nk, chunks, tid);
-        kept = j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
+        kept = lane < ROWS_KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
     auto store = [&](int buf) {
         bits = __ballot(kept != 0);
@@ -80,16 +84,16 @@ __global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void
         const uint64_t now = bits;
         if (t + 1 < tiles) fetch(j0 + ROWS_KEYS);
         if (busy && j0 < wend) {
-            const T* kb = kt + (t & 1) * TILE;
-            f32x16 sc[2];
-            sc[0] = scores<T, DP>(kb, 0, q);
-            sc[1] = scores<T, DP>(kb, 32, q);
+            const S* kb = kt + (t & 1) * TILE;
+            f32x16 sc[NB];
+#pragma unroll
+            for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(kb, 32 * k, q);
             const int d0 = j0 - s.start - wrow;                         // distance of the tile's first key from the wave's first query
             const bool near = near_tile(a.rel, d0 - 31, d0 + ROWS_KEYS - 1);
             const float far = a.rel.n > 0 && !near ? LOG2E * a.bias[far_bucket(a.rel, d0 - 31) * a.heads + h] : 0.f;
             const bool cut = a.causal && d0 + ROWS_KEYS - 1 > 0;
             float c = scale, add = far;
-            if (near || cut || now != ~0ull) {
+            if (near || cut || now != ~0ull >> (64 - ROWS_KEYS)) {
                 uint64_t seen = now;
                 if (cut) {
                     const int last = row + s.start - j0;                // last key of the tile that this query sees
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void
                 seen = lane_bits(seen);
                 const float* tab = lut + (near ? d0 - (lane & 31) + 4 * (lane >> 5) - a.rel.edge[0] + REL_PAD : 0);
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < NB; ++k)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int at = 32 * k + reg_row(r);
@@ -108,13 +112,13 @@ __global__ __launch_bounds__(ROWS_THREADS, (sizeof(T) * DP <= 128 ? 2 : 1)) void
                 c = 1.f;
                 add = 0.f;
             }
-            o.template step<2>(sc, c, add);
-            o.template weigh<2>(vt + (t & 1) * TILE, sc);
+            o.template step<NB>(sc, c, add);
+            o.template weigh<NB>(vt + (t & 1) * TILE, sc);
         }
         if (t + 1 < tiles) store((t + 1) & 1);
         __syncthreads();
     }
-    if (row < s.nq) write_rows<T, DP>(a, o, s.q0 + row, h, out, out_ld, lse);
+    if (row < s.nq) write_rows<T, M, DP>(a, o, s.q0 + row, h, out, out_ld, lse);
 }
 
 // ---- split form, solo form -----------------------------------------------------------------------------------------------------------
@@ -124,7 +128,7 @@ constexpr int SPLIT_KEYS = 32, SPLIT_TILES = 16;                       // keys o
 // shared memory: 4 waves' K and V tiles, in whose place the waves' results meet (rows of DP + 4 floats: no two rows start at the same bank)
 template <typename T, int DP>
 struct SplitLds {
-    static constexpr size_t tiles = 4 * 2 * SPLIT_KEYS * DP * sizeof(T), join = 4 * 32 * (DP + 4) * sizeof(float);
+    static constexpr size_t tiles = 4 * 2 * SPLIT_KEYS * attn_width<T, DP>, join = 4 * 32 * (DP + 4) * sizeof(float);
     static constexpr size_t first = tiles > join ? tiles : join, stats = 4 * 32 * 2 * sizeof(float);
 };
 
@@ -174,14 +178,16 @@ __device__ __forceinline__ bool find_chunk(const AttnView& a, const AttnSplit& c
 
 // part: [item][split][32][DP + 2] (weighted sum, maximum, sum); not used when there is one split, nor of splits behind the item's last tile
 template <typename T, int DP, bool SOLO>
-__global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 3 : 1)) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status, float* part,
+__global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, DP> <= 192 ? 2 : 1)) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status, float* part,
                                                                                               AttnSplit cut) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using L = SplitLds<T, DP>;
-    constexpr int TILE = SPLIT_KEYS * DP, STEP = SOLO ? 1 : 4;
+    using M = AttnKind<T, DP>;
+    using S = typename Mma<M>::Store;
+    constexpr int TILE = SPLIT_KEYS * Tile<M, DP>::STRIDE, STEP = SOLO ? 1 : 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, kv_heads = a.heads / a.group;
-    T* kt = reinterpret_cast<T*>(lds) + wave * 2 * TILE;
-    T* vt = kt + TILE;
+    S* kt = reinterpret_cast<S*>(lds) + wave * 2 * TILE;
+    S* vt = kt + TILE;
     float* stats = reinterpret_cast<float*>(lds + L::first);
     const int64_t items = (int64_t)cut.row_blocks * kv_heads * a.n_seg, at_item = SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     int rb, g, b, sp = 0, item;
@@ -200,18 +206,18 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 3 : 1)) void attn_spl
     const bool none = r0 >= rows || (SOLO && at_item >= items);
     if (!SOLO && (none || (sp > 0 && t0 >= tiles))) return;
     const int r = r0 + (lane & 31), i = r / a.group, hg = r % a.group, h = g * a.group + hg;
-    const int chunks = a.dim / Tile<T, DP>::PER;
+    const int chunks = a.dim / Tile<M, DP>::PER;
     const float scale = fabsf(a.scale) * LOG2E;
 
-    RowFrags<T, DP> q;
+    RowFrags<M, DP> q;
     q.load((const T*)a.q + (s.q0 + i) * a.q_ld + (int64_t)h * a.dim, chunks, !none && r < rows);
     if (a.scale < 0.f) q.negate();
 
     const T* K = (const T*)a.k + s.k0 * a.k_ld + (int64_t)g * a.dim;
     const T* V = (const T*)a.v + s.k0 * a.v_ld + (int64_t)g * a.dim;
     const int i0 = r0 / a.group, i1 = min(r0 + 31, rows - 1) / a.group;
-    Softmax<T, DP> o;
-    Staged<T, DP, SPLIT_KEYS, 64> ks, vs;
+    Softmax<M, DP> o;
+    Staged<M, DP, SPLIT_KEYS, 64> ks, vs;
     uint8_t kept = 0;
     auto fetch = [&](int j0) {
         ks.fetch(K, a.k_ld, j0, s.nk, chunks, lane);
@@ -242,7 +248,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 3 : 1)) void attn_spl
         __builtin_amdgcn_wave_barrier();
         if (t + STEP < t1) fetch((t + STEP) * SPLIT_KEYS);
         f32x16 sc[1];
-        sc[0] = scores<T, DP>(kt, 0, q);
+        sc[0] = scores<M, DP>(kt, 0, q);
         const int dmin = j0 - s.start - i1, dmax = j0 + SPLIT_KEYS - 1 - s.start - i0;
         const bool near = near_tile(a.rel, dmin, dmax);
         const float far = a.rel.n > 0 && !near ? table[far_bucket(a.rel, dmin) * wide + col] : 0.f;
@@ -269,11 +275,11 @@ __global__ __launch_bounds__(256, (sizeof(T) * DP <= 128 ? 3 : 1)) void attn_spl
     }
 
     if (SOLO) {
-        if (r < rows) write_rows<T, DP>(a, o, s.q0 + i, h, out, out_ld, lse);
+        if (r < rows) write_rows<T, M, DP>(a, o, s.q0 + i, h, out, out_ld, lse);
         return;
     }
     float m, sum, w[DP / 8];
-    join_waves<T, DP>(o, reinterpret_cast<float*>(lds), stats, m, sum, w);
+    join_waves<M, DP>(o, reinterpret_cast<float*>(lds), stats, m, sum, w);
     const int mine = r0 + (tid >> 3);
     if (cut.splits == 1) {
         if (mine < rows) finish_row<T, DP>(a, s.q0 + mine / a.group, g * a.group + mine % a.group, tid, m, sum, w, out, out_ld, lse);
@@ -362,7 +368,7 @@ static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int
         const int row_blocks = ceil_div(a->max_q, 128);
         const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
         DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
-        const size_t lds = 4 * ROWS_KEYS * DP * sizeof(T) + rel_reach(a) * sizeof(float);
+        const size_t lds = 4 * rows_keys<T, DP> * attn_width<T, DP> + rel_reach(a) * sizeof(float);
         attn_rows_kernel<T, DP><<<(unsigned)blocks, ROWS_THREADS, lds, st>>>(v, (T*)out, out_ld, lse, status, row_blocks);
         DCTR_LAUNCH_CHECK();
         return DCTR_OK;

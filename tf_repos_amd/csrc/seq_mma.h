@@ -1,4 +1,9 @@
-// Matrix-core building blocks of the sequence operators (attention*.hip, vocab_softmax.hip), for float and bfloat16 operands alike.
+// Matrix-core building blocks of the sequence operators (attention*.hip, vocab_softmax.hip).  Operand kinds M:
+//   __bf16   bfloat16 arrays
+//   Split    float arrays, every element as three bfloat16 planes x = h + m + l (3 x 8 significand bits: exact) and the six leading plane products
+//            in f32 on the bf16 pipe: what is dropped is below 2^-25 of an element product.  The f32 matrix instructions run at the vector
+//            units' rate, 1/16 of the bf16 pipe's, and hold the vector units up meanwhile
+//   float    float arrays on the f32 matrix instructions: where the planes' registers do not suffice
 //
 // Every product is one of two, on 32 x 32 output blocks, f32 accumulators (16 a lane):
 //   scores    S[m, n] = sum_d A[m, d] B[n, d]    A: 32 rows of a tile in shared memory, B: 32 rows held in registers (RowFrags)
@@ -41,6 +46,7 @@ __device__ __forceinline__ Halves halves(float x) {
 __device__ __forceinline__ float both_max(float x) { const Halves h = halves(x); return fmaxf(h.lo, h.hi); }
 __device__ __forceinline__ float both_sum(float x) { const Halves h = halves(x); return h.lo + h.hi; }
 
+
 // row of register r within its 32-row block
 __device__ __forceinline__ constexpr int reg_row(int r) { return 8 * (r >> 2) + (r & 3); }      // + 4 * (lane >> 5)
 
@@ -53,11 +59,15 @@ __device__ __forceinline__ int tile_lane() {
     return l;
 }
 
-template <typename T, int DP>
+struct Split {};
+template <typename M> struct Mma;
+
+template <typename M, int DP>
 struct Tile {
-    static constexpr int CHUNKS = DP * (int)sizeof(T) / 16, PER = 16 / (int)sizeof(T);
+    using S = typename Mma<M>::Store;
+    static constexpr int PER = 16 / (int)sizeof(S), CHUNKS = DP / PER, STRIDE = DP * Mma<M>::PLANES;      // a row: its planes one after the other
     static __device__ __forceinline__ int swz(int r) {
-        if (sizeof(T) == 2) {
+        if (sizeof(S) == 2) {
             if (CHUNKS == 4) return (r >> 2) & 3;
             if (CHUNKS == 8) return ((r >> 1) & 1) << 2 | ((r >> 2) & 3);
             return (r & 3) << 2 | ((r >> 2) & 3);
@@ -65,16 +75,34 @@ struct Tile {
         if (CHUNKS == 8) return (r >> 1) & 7;
         return ((r >> 2) & 1) << 3 | ((r >> 3) & 1) << 2 | (r & 3);
     }
-    static __device__ __forceinline__ int at(int r, int c) { return r * DP + (c ^ swz(r)) * PER; }
+    static __device__ __forceinline__ int at(int r, int c) { return r * STRIDE + (c ^ swz(r)) * PER; }
 };
 
-// One 16-byte chunk a lane: 16 (bf16) or 8 (f32) columns of 32 rows.
-template <typename T> struct Mma;
+// 32 (rows) x 16 columns of a bf16 plane, transposed: the lane's column, rows 4 (lane >> 5) + {0..3} and + 8
+template <typename M, int DP>
+__device__ __forceinline__ bf16x8 column_chunk(const __bf16* tile, int row, int col) {
+    bf16x8 a;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + Tile<M, DP>::at(row + 8 * half, col >> 3) + (col & 7)));
+        const bf16x4 b = __builtin_bit_cast(bf16x4, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[4 * half + j] = b[j];
+    }
+    return a;
+}
 
 template <> struct Mma<__bf16> {
-    using Chunk = bf16x8;
+    using Global = __bf16;                              // element of the arrays
+    using Store = __bf16;                               // element of a tile
+    static constexpr int PLANES = 1, BYTES = 2;         // of an element in a tile or held row
+    static constexpr bool ROUNDS = true;                // the weights are rounded
+    using Chunk = bf16x8;                               // one 16-byte chunk a lane: 16 columns of 32 rows
     struct Weights { bf16x8 w[2]; };                    // a 32-row block of P, rounded to bf16: half a step of 2^-8 relative a weight
-    static __device__ __forceinline__ f32x16 dot(Chunk a, Chunk b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Chunk load(const Global* p) { return *reinterpret_cast<const Chunk*>(p); }
+    static __device__ __forceinline__ f32x16 dot(const Store* a, Chunk b, f32x16 c, int) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(a), b, c, 0, 0, 0);
+    }
     static __device__ __forceinline__ Weights pack(const f32x16& p) {
         Weights r;
 #pragma unroll
@@ -85,24 +113,18 @@ template <> struct Mma<__bf16> {
     static __device__ __forceinline__ f32x16 weigh(const __bf16* tile, int row0, int col0, const Weights& p, f32x16 acc) {
         const int l = tile_lane<DP>(), row = row0 + 4 * (l >> 5) + ((l & 15) >> 2), col = col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            bf16x8 a;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int r = row + 16 * s + 8 * half;
-                const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + Tile<__bf16, DP>::at(r, col >> 3) + (col & 7)));
-                const bf16x4 b = __builtin_bit_cast(bf16x4, v);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) a[4 * half + j] = b[j];
-            }
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p.w[s], acc, 0, 0, 0);
-        }
+        for (int s = 0; s < 2; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(column_chunk<__bf16, DP>(tile, row + 16 * s, col), p.w[s], acc, 0, 0, 0);
         return acc;
     }
     static __device__ __forceinline__ Chunk negate(Chunk a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) a[i] = -a[i];
         return a;
+    }
+    static __device__ __forceinline__ float product(Chunk a, Chunk b, float c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c = fmaf((float)a[i], (float)b[i], c);
+        return c;
     }
     static __device__ __forceinline__ void store4(__bf16* p, float a, float b, float c, float d) {
         bf16x4 v;
@@ -112,9 +134,15 @@ template <> struct Mma<__bf16> {
 };
 
 template <> struct Mma<float> {
-    using Chunk = f32x4;
+    using Global = float;
+    using Store = float;
+    static constexpr int PLANES = 1, BYTES = 4;
+    static constexpr bool ROUNDS = false;
+    using Chunk = f32x4;                                // 8 columns of 32 rows
     struct Weights { f32x16 w; };
-    static __device__ __forceinline__ f32x16 dot(Chunk a, Chunk b, f32x16 c) {
+    static __device__ __forceinline__ Chunk load(const Global* p) { return *reinterpret_cast<const Chunk*>(p); }
+    static __device__ __forceinline__ f32x16 dot(const Store* p, Chunk b, f32x16 c, int) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
         return c;
@@ -129,60 +157,161 @@ template <> struct Mma<float> {
         return acc;
     }
     static __device__ __forceinline__ Chunk negate(Chunk a) { return -a; }
+    static __device__ __forceinline__ float product(Chunk a, Chunk b, float c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = fmaf(a[i], b[i], c);
+        return c;
+    }
+    static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d}; }
+};
+
+struct Planes { bf16x8 h, m, l; };
+// x = h + m + l, each the nearest bf16 of what is left: the subtractions are exact
+__device__ __forceinline__ Planes planes_of(const float (&x)[8]) {
+    Planes p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        p.h[i] = (__bf16)x[i];
+        const float r = x[i] - (float)p.h[i];
+        p.m[i] = (__bf16)r;
+        p.l[i] = (__bf16)(r - (float)p.m[i]);
+    }
+    return p;
+}
+// the six products, smallest first
+__device__ __forceinline__ f32x16 six(const Planes& a, const Planes& b, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.m, b.m, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.l, b.h, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.l, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.m, b.h, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.m, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.h, b.h, c, 0, 0, 0);
+}
+
+template <> struct Mma<Split> {
+    using Global = float;
+    using Store = __bf16;
+    static constexpr int PLANES = 3, BYTES = 6;
+    static constexpr bool ROUNDS = false;
+    using Chunk = Planes;                               // 16 columns of 32 rows
+    struct Weights { Planes w[2]; };
+    static __device__ __forceinline__ Chunk load(const Global* p) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(p + 4 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
+        }
+        return planes_of(x);
+    }
+    static __device__ __forceinline__ f32x16 dot(const Store* a, const Chunk& b, f32x16 c, int plane) {
+        return six(Planes{*reinterpret_cast<const bf16x8*>(a), *reinterpret_cast<const bf16x8*>(a + plane), *reinterpret_cast<const bf16x8*>(a + 2 * plane)}, b, c);
+    }
+    static __device__ __forceinline__ Weights pack(const f32x16& p) {
+        Weights r;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = p[8 * s + i];
+            r.w[s] = planes_of(x);
+        }
+        return r;
+    }
+    template <int DP>
+    static __device__ __forceinline__ f32x16 weigh(const __bf16* tile, int row0, int col0, const Weights& p, f32x16 acc) {
+        const int l = tile_lane<DP>(), row = row0 + 4 * (l >> 5) + ((l & 15) >> 2), col = col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            acc = six(Planes{column_chunk<Split, DP>(tile, row + 16 * s, col), column_chunk<Split, DP>(tile + DP, row + 16 * s, col),
+                             column_chunk<Split, DP>(tile + 2 * DP, row + 16 * s, col)}, p.w[s], acc);
+        return acc;
+    }
+    static __device__ __forceinline__ Chunk negate(Chunk a) {
+        a.h = Mma<__bf16>::negate(a.h);
+        a.m = Mma<__bf16>::negate(a.m);
+        a.l = Mma<__bf16>::negate(a.l);
+        return a;
+    }
+    static __device__ __forceinline__ float product(const Chunk& a, const Chunk& b, float c) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            c = fmaf(((float)a.h[i] + (float)a.m[i]) + (float)a.l[i], ((float)b.h[i] + (float)b.m[i]) + (float)b.l[i], c);
+        return c;
+    }
     static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d}; }
 };
 
 // 32 rows in registers, one a lane (both halves together hold a row's chunks): the B operand of the scores
-template <typename T, int DP>
+template <typename M, int DP>
 struct RowFrags {
-    static constexpr int STEPS = Tile<T, DP>::CHUNKS / 2;
-    typename Mma<T>::Chunk c[STEPS];
+    using T = typename Mma<M>::Global;
+    static constexpr int STEPS = Tile<M, DP>::CHUNKS / 2;
+    typename Mma<M>::Chunk c[STEPS];
     __device__ __forceinline__ void load(const T* row, int chunks, bool on) {          // `on`: the row exists; the rest is zero
         const int g = (threadIdx.x >> 5) & 1;
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
-            c[s] = typename Mma<T>::Chunk{};
-            if (on && 2 * s + g < chunks) c[s] = *reinterpret_cast<const typename Mma<T>::Chunk*>(row + (2 * s + g) * Tile<T, DP>::PER);
+            c[s] = typename Mma<M>::Chunk{};
+            if (on && 2 * s + g < chunks) c[s] = Mma<M>::load(row + (2 * s + g) * Tile<M, DP>::PER);
         }
     }
     __device__ __forceinline__ void negate() {
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) c[s] = Mma<T>::negate(c[s]);
+        for (int s = 0; s < STEPS; ++s) c[s] = Mma<M>::negate(c[s]);
     }
 };
 
 // S of tile rows [row0, row0 + 32) against held rows
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 scores(const T* tile, int row0, const RowFrags<T, DP>& held) {
+template <typename M, int DP>
+__device__ __forceinline__ f32x16 scores(const typename Mma<M>::Store* tile, int row0, const RowFrags<M, DP>& held) {
     const int l = tile_lane<DP>(), row = row0 + (l & 31), g = l >> 5;
     f32x16 s = {};
 #pragma unroll
-    for (int k = 0; k < RowFrags<T, DP>::STEPS; ++k)
-        s = Mma<T>::dot(*reinterpret_cast<const typename Mma<T>::Chunk*>(tile + Tile<T, DP>::at(row, 2 * k + g)), held.c[k], s);
+    for (int k = 0; k < RowFrags<M, DP>::STEPS; ++k) s = Mma<M>::dot(tile + Tile<M, DP>::at(row, 2 * k + g), held.c[k], s, DP);
     return s;
 }
 
 // ROWS rows of an array on their way into a tile, by THREADS threads: fetched into registers while the tile before is in use
-template <typename T, int DP, int ROWS, int THREADS>
+template <typename M, int DP, int ROWS, int THREADS>
 struct Staged {
-    static constexpr int CHUNKS = Tile<T, DP>::CHUNKS, N = ROWS * CHUNKS / THREADS;
+    using T = typename Mma<M>::Global;
+    using S = typename Mma<M>::Store;
+    static constexpr int CHUNKS = Tile<M, DP>::CHUNKS, PER = Tile<M, DP>::PER, N = ROWS * CHUNKS / THREADS, LOADS = PER * (int)sizeof(T) / 16;
     static_assert(N >= 1 && ROWS * CHUNKS % THREADS == 0, "a tile is a whole number of chunks a thread");
-    f32x4 v[N];
+    f32x4 v[N][LOADS];
     // rows [first, first + ROWS) of those below `end`; the rest is zero
     __device__ __forceinline__ void fetch(const T* base, int64_t ld, int64_t first, int64_t end, int chunks, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = tid + i * THREADS, r = at / CHUNKS, c = at % CHUNKS;
-            v[i] = f32x4{};
-            if (first + r < end && c < chunks) v[i] = *reinterpret_cast<const f32x4*>(base + (first + r) * ld + c * Tile<T, DP>::PER);
+            const bool on = first + r < end && c < chunks;
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                v[i][j] = f32x4{};
+                if (on) v[i][j] = *reinterpret_cast<const f32x4*>(base + (first + r) * ld + c * PER + j * (16 / (int)sizeof(T)));
+            }
         }
     }
     // rows whose bit is not set become zero, whatever the array holds there
-    __device__ __forceinline__ void store(T* tile, int tid, uint64_t rows = ~0ull) const {
+    __device__ __forceinline__ void store(S* tile, int tid, uint64_t rows = ~0ull) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = tid + i * THREADS, r = at / CHUNKS, c = at % CHUNKS;
-            *reinterpret_cast<f32x4*>(tile + Tile<T, DP>::at(r, c)) = (rows >> r & 1) ? v[i] : f32x4{};
+            const bool on = rows >> r & 1;
+            S* to = tile + Tile<M, DP>::at(r, c);
+            if constexpr (LOADS == 1) {
+                *reinterpret_cast<f32x4*>(to) = on ? v[i][0] : f32x4{};
+            } else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = on ? v[i][e >> 2][e & 3] : 0.f;
+                const Planes p = planes_of(x);
+                *reinterpret_cast<bf16x8*>(to) = p.h;
+                *reinterpret_cast<bf16x8*>(to + DP) = p.m;
+                *reinterpret_cast<bf16x8*>(to + 2 * DP) = p.l;
+            }
         }
     }
 };
@@ -191,16 +320,16 @@ struct Staged {
 __device__ __forceinline__ uint64_t lane_bits(uint64_t rows) { return rows >> (4 * ((threadIdx.x >> 5) & 1)); }
 
 // Running softmax of a wave's 32 columns: m (base 2) and this half's share of the sum, the weighted sum as O^T blocks.
-template <typename T, int DP>
+template <typename M, int DP>
 struct Softmax {
     float m = -INFINITY, l = 0.f;
     f32x16 acc[DP / 32] = {};
 
-    // Takes one 32 x NB*32 step's scores: t = fma(s, c, b), hidden entries -inf already where c = 1, b = 0.  Returns the weights in s.
-    // The running maximum moves only when a score passes it by 2^8: weights up to 256 lose nothing in either type, and most steps
-    // then skip the rescaling of the accumulators.
+    // The running maximum takes in one 32 x NB*32 step's scores, t = fma(s, c, b); returns b - maximum for weights().
+    // It moves only when a score passes it by 2^8: weights up to 256 lose nothing in either type, and most steps then skip the rescaling of
+    // the accumulators.
     template <int NB>
-    __device__ __forceinline__ void step(f32x16 (&s)[NB], float c, float b) {
+    __device__ __forceinline__ float raise(const f32x16 (&s)[NB], float c, float b) {
         float top = s[0][0];
 #pragma unroll
         for (int k = 0; k < NB; ++k)
@@ -217,7 +346,11 @@ struct Softmax {
             }
             m = mn;
         }
-        const float off = b - (m == -INFINITY ? 0.f : m);
+        return b - (m == -INFINITY ? 0.f : m);
+    }
+    // s becomes the weights 2^(s c + off), whose sum l takes in
+    template <int NB>
+    __device__ __forceinline__ void weights(f32x16 (&s)[NB], float c, float off) {
         float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NB; ++k)
@@ -229,20 +362,22 @@ struct Softmax {
         l += (part[0] + part[1]) + (part[2] + part[3]);
     }
     template <int NB>
-    __device__ __forceinline__ void weigh(const T* tile, const f32x16 (&p)[NB]) {
+    __device__ __forceinline__ void step(f32x16 (&s)[NB], float c, float b) { weights<NB>(s, c, raise<NB>(s, c, b)); }
+    template <int NB>
+    __device__ __forceinline__ void weigh(const typename Mma<M>::Store* tile, const f32x16 (&p)[NB]) {
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const auto w = Mma<T>::pack(p[k]);
+            const auto w = Mma<M>::pack(p[k]);
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(tile, 32 * k, 32 * d, w, acc[d]);
+            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(tile, 32 * k, 32 * d, w, acc[d]);
         }
     }
 };
 
 // The results of a block's four waves on the same 32 rows meet in shared memory: `join` 4 x 32 rows of DP + 4 floats (no two rows start at the
 // same bank), `stats` 4 x 32 pairs (maximum, sum).  Afterwards thread t holds row t / 8's maximum, sum and columns [t % 8 * DP/8, + DP/8).
-template <typename T, int DP>
-__device__ __forceinline__ void join_waves(const Softmax<T, DP>& o, float* join, float* stats, float& m, float& l, float (&w)[DP / 8]) {
+template <typename M, int DP>
+__device__ __forceinline__ void join_waves(const Softmax<M, DP>& o, float* join, float* stats, float& m, float& l, float (&w)[DP / 8]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = tid >> 3;
     __syncthreads();                                                    // every wave is done with the tiles
     const float sum = both_sum(o.l);

@@ -7,6 +7,7 @@
 // no cancellation however sure the model is, nor has loss = log1p(e) where the label is the row's largest.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "seq_mma.h"
 
@@ -32,47 +33,47 @@ struct VocabParts {
     int64_t each;                   // vocabulary rows of a split, a multiple of the tile
 };
 
+// Operand kind: float arrays in planes (seq_mma.h) up to 128 wide, beyond that the planes of 32 rows and their accumulators pass the registers.
 template <typename T, int DP>
-struct VocabTile { static constexpr int ROWS = sizeof(T) * DP <= 256 ? 64 : 32, NB = ROWS / 32, SIZE = ROWS * DP; };
+using VocabKind = std::conditional_t<std::is_same_v<T, float> && DP <= 128, Split, T>;
 
-// One step of a wave's 32 rows against NB * 32 table rows from v0 on: scores, bias, hidden columns (behind the table, the row's label).
-// `bt`: log2(e) b of the tile's rows, in shared memory, or null.
-template <typename T, int DP, int NB, bool DX>
-__device__ __forceinline__ void vocab_step(const T* tile, const float* bt, const RowFrags<T, DP>& x, int64_t v0, int64_t v1, int64_t label,
-                                           Softmax<T, DP>& o) {
+template <typename T, int DP>
+struct VocabTile {
+    using M = VocabKind<T, DP>;
+    static constexpr int WIDTH = Mma<M>::BYTES * DP, ROWS = WIDTH <= 384 ? 64 : 32, NB = ROWS / 32, SIZE = ROWS * Tile<M, DP>::STRIDE;
+    static constexpr size_t bytes = (size_t)ROWS * WIDTH;
+};
+
+// Bias and hidden columns (behind the table, the row's label) of a wave's 32 rows' scores against NB * 32 table rows from v0 on; returns the factor
+// that is left to the exponent.  `bt`: log2(e) b of the tile's rows, in shared memory, or null.
+template <int NB>
+__device__ __forceinline__ float adjust(f32x16 (&s)[NB], const float* bt, int64_t v0, int64_t v1, int64_t label) {
     const int half = (threadIdx.x >> 5) & 1;
-    f32x16 s[NB];
-#pragma unroll
-    for (int k = 0; k < NB; ++k) s[k] = scores<T, DP>(tile, 32 * k, x);
     const int64_t own = label - v0;
-    float c = LOG2E;
     const bool hide = v0 + 32 * NB > v1 || __any(own >= 0 && own < 32 * NB);
-    if (bt != nullptr || hide) {
-        uint64_t seen = v1 - v0 >= 64 ? ~0ull : (1ull << (v1 - v0)) - 1;
-        if (own >= 0 && own < 64) seen &= ~(1ull << own);
-        seen = lane_bits(seen);
+    if (bt == nullptr && !hide) return LOG2E;
+    uint64_t seen = v1 - v0 >= 64 ? ~0ull : (1ull << (v1 - v0)) - 1;
+    if (own >= 0 && own < 64) seen &= ~(1ull << own);
+    seen = lane_bits(seen);
+#pragma unroll
+    for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 add = bt != nullptr ? *reinterpret_cast<const f32x4*>(bt + 32 * k + 8 * i + 4 * half) : f32x4{};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[k][4 * i + j] = fmaf(s[k][4 * i + j], LOG2E, add[j]);
+        }
+    if (hide) {
 #pragma unroll
         for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 add = bt != nullptr ? *reinterpret_cast<const f32x4*>(bt + 32 * k + 8 * i + 4 * half) : f32x4{};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[k][4 * i + j] = fmaf(s[k][4 * i + j], LOG2E, add[j]);
-            }
-        if (hide) {
-#pragma unroll
-            for (int k = 0; k < NB; ++k)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[k][r] = (seen >> (32 * k + reg_row(r)) & 1) ? s[k][r] : -INFINITY;
-        }
-        c = 1.f;
+            for (int r = 0; r < 16; ++r) s[k][r] = (seen >> (32 * k + reg_row(r)) & 1) ? s[k][r] : -INFINITY;
     }
-    o.template step<NB>(s, c, 0.f);
-    if (DX) o.template weigh<NB>(tile, s);
+    return 1.f;
 }
 
-template <typename T, int DP, bool DX>
-__device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, int64_t n, bool on, const Softmax<T, DP>& o) {
+template <typename M, int DP, bool DX>
+__device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, int64_t n, bool on, const Softmax<M, DP>& o) {
     const int lane = threadIdx.x & 63, half = lane >> 5;
     const float e = both_sum(o.l);
     if (!on) return;
@@ -87,23 +88,27 @@ __device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, 
                     f32x4{o.acc[k][4 * i], o.acc[k][4 * i + 1], o.acc[k][4 * i + 2], o.acc[k][4 * i + 3]};
 }
 
-// 4 waves of 32 rows share the table's tiles, double-buffered
+// 4 waves of 32 rows share the table's tiles, three buffers: while a tile is weighed, the scores of the next one are formed under its exponents and
+// the one after that is on its way.
 template <typename T, int DP, bool DX>
-__global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= (DX ? 256 : 512) ? 2 : 1)) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
+__global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 : 512) ? 2 : 1)) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Ti = VocabTile<T, DP>;
-    T* tiles = reinterpret_cast<T*>(lds);
-    float* bias = reinterpret_cast<float*>(tiles + 2 * Ti::SIZE);                       // [2][ROWS]
+    using M = VocabKind<T, DP>;
+    using S = typename Mma<M>::Store;
+    constexpr int NB = Ti::NB;
+    S* tiles = reinterpret_cast<S*>(lds);
+    float* bias = reinterpret_cast<float*>(tiles + 3 * Ti::SIZE);                       // [3][ROWS]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int rb = blockIdx.x % row_blocks, sp = blockIdx.x / row_blocks;
     const int64_t n = (int64_t)rb * 128 + wave * 32 + (lane & 31), v0 = sp * p.each, v1 = min(a.V, v0 + p.each);
-    const int chunks = a.D / Tile<T, DP>::PER;
+    const int chunks = a.D / Tile<M, DP>::PER;
     const bool on = n < a.N, busy = rb * 128 + wave * 32 < a.N;
-    RowFrags<T, DP> x;
+    RowFrags<M, DP> x;
     x.load((const T*)a.x + n * a.x_ld, chunks, on);
     const int64_t label = on ? a.labels[n] : -1;
-    Softmax<T, DP> o;
-    Staged<T, DP, Ti::ROWS, VS_THREADS> ws;
+    Softmax<M, DP> o;
+    Staged<M, DP, Ti::ROWS, VS_THREADS> ws;
     float bv = 0.f;
     auto fetch = [&](int64_t v) {
         ws.fetch((const T*)a.w, a.w_ld, v, v1, chunks, tid);
@@ -113,43 +118,63 @@ __global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= (DX ? 256 : 512) ? 2
         ws.store(tiles + buf * Ti::SIZE, tid);
         if (a.b != nullptr && tid < Ti::ROWS) bias[buf * Ti::ROWS + tid] = bv;
     };
-    if (v0 < v1) {
+    if (v0 < v1) {                                                                      // (rows behind v1 are zeros)
         fetch(v0);
         store(0);
+        fetch(v0 + Ti::ROWS);
+        store(1);
     }
     __syncthreads();
-    int buf = 0;
-    for (int64_t v = v0; v < v1; v += Ti::ROWS, buf ^= 1) {
-        const bool more = v + Ti::ROWS < v1;
-        if (more) fetch(v + Ti::ROWS);
-        if (busy) vocab_step<T, DP, Ti::NB, DX>(tiles + buf * Ti::SIZE, a.b != nullptr ? bias + buf * Ti::ROWS : nullptr, x, v, v1, label, o);
-        if (more) store(buf ^ 1);
+    f32x16 sc[NB];
+#pragma unroll
+    for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(tiles, 32 * k, x);
+    int now = 0;
+    for (int64_t v = v0; v < v1; v += Ti::ROWS) {
+        const int next = now == 2 ? 0 : now + 1, then = next == 2 ? 0 : next + 1;
+        const bool more = v + 2 * Ti::ROWS < v1;
+        if (more) fetch(v + 2 * Ti::ROWS);
+        if (busy) {
+            const float c = adjust<NB>(sc, a.b != nullptr ? bias + now * Ti::ROWS : nullptr, v, v1, label);
+            const float off = o.template raise<NB>(sc, c, 0.f);
+            f32x16 ahead[NB];
+#pragma unroll
+            for (int k = 0; k < NB; ++k) ahead[k] = scores<M, DP>(tiles + next * Ti::SIZE, 32 * k, x);
+            o.template weights<NB>(sc, c, off);
+            if (DX) o.template weigh<NB>(tiles + now * Ti::SIZE, sc);
+
+#pragma unroll
+            for (int k = 0; k < NB; ++k) sc[k] = ahead[k];
+        }
+        if (more) store(then);
         __syncthreads();
+        now = next;
     }
-    write_parts<T, DP, DX>(p, sp, a.N, n, on, o);
+    write_parts<M, DP, DX>(p, sp, a.N, n, on, o);
 }
 
 // Up to 32 rows: every wave takes tiles of its own, the four join before they leave their part.
 template <typename T, int DP>
 struct FewLds {
-    static constexpr size_t tiles = 4 * 32 * DP * sizeof(T), join = 4 * 32 * (DP + 4) * sizeof(float), first = tiles > join ? tiles : join;
+    static constexpr size_t tiles = 4 * 32 * (size_t)VocabTile<T, DP>::WIDTH, join = 4 * 32 * (DP + 4) * sizeof(float), first = tiles > join ? tiles : join;
     static constexpr size_t all = first + 4 * 32 * 2 * sizeof(float) + 4 * 32 * sizeof(float);      // + statistics + bias
 };
 template <typename T, int DP, bool DX>
-__global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void vocab_few_kernel(VocabView a, VocabParts p) {
+__global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1)) void vocab_few_kernel(VocabView a, VocabParts p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sp = blockIdx.x;
-    T* tile = reinterpret_cast<T*>(lds) + wave * 32 * DP;
+    using M = VocabKind<T, DP>;
+    using S = typename Mma<M>::Store;
+    S* tile = reinterpret_cast<S*>(lds) + wave * 32 * Tile<M, DP>::STRIDE;
     float* stats = reinterpret_cast<float*>(lds + FewLds<T, DP>::first);
     float* bias = stats + 4 * 32 * 2 + wave * 32;
     const int64_t n = lane & 31, v0 = sp * p.each, v1 = min(a.V, v0 + p.each);
-    const int chunks = a.D / Tile<T, DP>::PER;
+    const int chunks = a.D / Tile<M, DP>::PER;
     const bool on = n < a.N;
-    RowFrags<T, DP> x;
+    RowFrags<M, DP> x;
     x.load((const T*)a.x + n * a.x_ld, chunks, on);
     const int64_t label = on ? a.labels[n] : -1;
-    Softmax<T, DP> o;
-    Staged<T, DP, 32, 64> ws;
+    Softmax<M, DP> o;
+    Staged<M, DP, 32, 64> ws;
     float bv = 0.f;
     auto fetch = [&](int64_t v) {
         ws.fetch((const T*)a.w, a.w_ld, v, v1, chunks, lane);
@@ -164,11 +189,14 @@ __global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void v
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (v + 128 < v1) fetch(v + 128);
-        vocab_step<T, DP, 1, DX>(tile, a.b != nullptr ? bias : nullptr, x, v, v1, label, o);
+        f32x16 sc[1] = {scores<M, DP>(tile, 0, x)};
+        const float c = adjust<1>(sc, a.b != nullptr ? bias : nullptr, v, v1, label);
+        o.template step<1>(sc, c, 0.f);
+        if (DX) o.template weigh<1>(tile, sc);
     }
     if (DX) {
         float m, e, w[DP / 8];
-        join_waves<T, DP>(o, reinterpret_cast<float*>(lds), stats, m, e, w);
+        join_waves<M, DP>(o, reinterpret_cast<float*>(lds), stats, m, e, w);
         const int row = threadIdx.x >> 3, part = threadIdx.x & 7;
         if (row >= a.N) return;
         const int64_t at = (int64_t)sp * a.N + row;
@@ -246,23 +274,25 @@ __global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, Voc
 // ---- dw, db: 32 table rows a wave, over the rows of x ---------------------------------------------------------------------------------
 // With more than one split (a short vocabulary): part [splits][V][DP], part_b [splits][V], joined by vocab_dw_join_kernel.
 template <typename T, int DP>
-__global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
+__global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1)) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
                                                               int splits, int each, int table_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Ti = VocabTile<T, DP>;
-    T* tiles = reinterpret_cast<T*>(lds);
+    using M = VocabKind<T, DP>;
+    using S = typename Mma<M>::Store;
+    S* tiles = reinterpret_cast<S*>(lds);
     float* stats = reinterpret_cast<float*>(tiles + 2 * Ti::SIZE);                      // [2][-log2(e) lse, row scale, label][ROWS]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
     const int tb = blockIdx.x % table_blocks, sp = blockIdx.x / table_blocks;
     const int64_t w0 = (int64_t)tb * 128 + wave * 32, v = w0 + (lane & 31);
-    const int chunks = a.D / Tile<T, DP>::PER, n0 = sp * each, n1 = min(a.N, n0 + each);
+    const int chunks = a.D / Tile<M, DP>::PER, n0 = sp * each, n1 = min(a.N, n0 + each);
     const bool on = v < a.V;
-    RowFrags<T, DP> w;
+    RowFrags<M, DP> w;
     w.load((const T*)a.w + v * a.w_ld, chunks, on);
     const float bv = on && a.b != nullptr ? LOG2E * a.b[v] : 0.f;
     f32x16 acc[DP / 32] = {};
     float sum = 0.f;
-    Staged<T, DP, Ti::ROWS, VS_THREADS> xs;
+    Staged<M, DP, Ti::ROWS, VS_THREADS> xs;
     float lv = 0.f, cv = 0.f;
     int label = -1;
     auto fetch = [&](int n) {
@@ -291,14 +321,14 @@ __global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void v
     for (int n = n0; n < n1; n += Ti::ROWS, buf ^= 1) {
         const bool more = n + Ti::ROWS < n1;
         if (more) fetch(n + Ti::ROWS);
-        const T* xt = tiles + buf * Ti::SIZE;
+        const S* xt = tiles + buf * Ti::SIZE;
         const float* st = stats + buf * 3 * Ti::ROWS;
         const int32_t* lt = reinterpret_cast<const int32_t*>(st) + 2 * Ti::ROWS;
         const int64_t there = lane < Ti::ROWS ? (int64_t)lt[lane] - w0 : -1;
         const bool hot = __any(there >= 0 && there < 32);                               // a row's label is one of the wave's table rows
 #pragma unroll
         for (int k = 0; k < Ti::NB; ++k) {
-            f32x16 p = scores<T, DP>(xt, 32 * k, w);
+            f32x16 p = scores<M, DP>(xt, 32 * k, w);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 ml = *reinterpret_cast<const f32x4*>(st + 32 * k + 8 * i + 4 * half);
@@ -323,9 +353,9 @@ __global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void v
                 for (int r = 0; r < 16; ++r) part4[r & 3] += p[r];
                 sum += (part4[0] + part4[1]) + (part4[2] + part4[3]);
             }
-            const auto g = Mma<T>::pack(p);
+            const auto g = Mma<M>::pack(p);
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<T>::template weigh<DP>(xt, 32 * k, 32 * d, g, acc[d]);
+            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(xt, 32 * k, 32 * d, g, acc[d]);
         }
         if (more) store(buf ^ 1);
         __syncthreads();
@@ -350,7 +380,7 @@ __global__ __launch_bounds__(VS_THREADS, (sizeof(T) * DP <= 256 ? 2 : 1)) void v
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (32 * d + 8 * i < a.D)
-                Mma<T>::store4(to + 32 * d + 8 * i, a.scale * acc[d][4 * i], a.scale * acc[d][4 * i + 1], a.scale * acc[d][4 * i + 2],
+                Mma<M>::store4(to + 32 * d + 8 * i, a.scale * acc[d][4 * i], a.scale * acc[d][4 * i + 1], a.scale * acc[d][4 * i + 2],
                                a.scale * acc[d][4 * i + 3]);
 }
 
@@ -420,7 +450,7 @@ static int launch_fwd(const VocabView& a, float* loss, float* lse, void* dx, int
         vocab_few_kernel<T, DP, DX><<<f.splits, VS_THREADS, FewLds<T, DP>::all, st>>>(a, p);
     else
         vocab_rows_kernel<T, DP, DX><<<(unsigned)(f.row_blocks * f.splits), VS_THREADS,
-                                       2 * (VocabTile<T, DP>::SIZE * sizeof(T) + VocabTile<T, DP>::ROWS * sizeof(float)), st>>>(a, p, f.row_blocks);
+                                       3 * (VocabTile<T, DP>::bytes + VocabTile<T, DP>::ROWS * sizeof(float)), st>>>(a, p, f.row_blocks);
     DCTR_LAUNCH_CHECK();
     vocab_join_kernel<T, DP, DX><<<a.N, VS_THREADS, 0, st>>>(a, p, loss, lse, (T*)dx, dx_ld, status);
     DCTR_LAUNCH_CHECK();
@@ -432,7 +462,7 @@ static int launch_dw(const VocabView& a, const float* lse, void* dw, int64_t dw_
     const VocabWPlan w = plan_dw(a.N, a.V);
     float *part = ws, *part_b = ws + (int64_t)w.splits * a.V * DP;
     DCTR_REQUIRE((int64_t)w.table_blocks * w.splits <= INT32_MAX, "vocab softmax: too many blocks for one launch");
-    const size_t lds = 2 * (VocabTile<T, DP>::SIZE * sizeof(T) + 3 * VocabTile<T, DP>::ROWS * sizeof(float));
+    const size_t lds = 2 * (VocabTile<T, DP>::bytes + 3 * VocabTile<T, DP>::ROWS * sizeof(float));
     vocab_dw_kernel<T, DP><<<(unsigned)(w.table_blocks * w.splits), VS_THREADS, lds, st>>>(a, lse, (T*)dw, dw_ld, db, part, part_b, w.splits, w.each,
                                                                                            w.table_blocks);
     DCTR_LAUNCH_CHECK();
