@@ -90,6 +90,14 @@ __device__ __forceinline__ int bucket_of(const RelBuckets& r, int d) {
 }
 __device__ __forceinline__ int rel_reach(const RelBuckets& r) { return r.n > 1 ? r.edge[r.n - 2] - r.edge[0] + 2 * REL_PAD : 0; }
 
+// log2(e) x a head's bias of the two far buckets, read once: a load within the tile loop would wait for the tiles under way
+struct FarBias { float before, behind; };
+__device__ __forceinline__ FarBias far_bias(const AttnView& a, int h) {
+    FarBias f{0.f, 0.f};
+    if (a.rel.n > 0) f = {LOG2E * a.bias[h], LOG2E * a.bias[(int64_t)(a.rel.n - 1) * a.heads + h]};
+    return f;
+}
+
 inline int rel_reach(const dctr_attention* a) {         // entries of a table over distances
     return a->n_buckets > 1 ? a->boundaries[a->n_buckets - 2] - a->boundaries[0] + 2 * REL_PAD : 0;
 }

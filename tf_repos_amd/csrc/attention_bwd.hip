@@ -30,7 +30,7 @@ __device__ __forceinline__ void lds_add(float* cell, float x) { __hip_atomic_fet
 
 // part: [head][segment * row_blocks + row block][n_buckets] shares of the bias gradient, or null; delta [total_q, heads]
 template <typename T, int DP, int FORM>
-__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
+__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
                                                                  T* dq, int64_t dq_ld, float* delta, float* part, int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Q = QuerySide<T, DP, FORM>;
@@ -101,27 +101,28 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
     const bool busy = wrow < s.nq;
     const int wend = a.causal ? s.start + min(wrow + 32, s.nq) : keys;
 
+    FarBias fars = far_bias(a, h);
     f32x16 acc[DP / 32] = {}, pk[ROUNDED ? DP / 32 : 1] = {};
     float far_ds[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, pdp = 0.f;     // [below the first boundary, from the last one on]
-    Staged<M, DP, Q::KEYS, Q::THREADS> ks, vs;
+    std::conditional_t<OWN, Staged<M, DP, Q::KEYS, Q::THREADS>, Loader<M, DP, Q::KEYS, Q::THREADS>> ks, vs;
     uint64_t bits = 0;                                                  // kept keys of the tile
     uint8_t kept = 0;
-    auto fetch = [&](int j0) {
-        ks.fetch(K, a.k_ld, j0, s.nk, chunks, loader);
-        vs.fetch(V, a.v_ld, j0, s.nk, chunks, loader);
+    auto fetch = [&](int j0, int buf) {
+        ks.fetch(kt + buf * TILE, K, a.k_ld, j0, s.nk, chunks, loader);
+        vs.fetch(vt + buf * TILE, V, a.v_ld, j0, s.nk, chunks, loader);
         kept = lane < Q::KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
-    auto store = [&](int buf) {
+    auto land = [&](int buf) {
         bits = __ballot(kept != 0);
-        ks.store(kt + buf * TILE, loader, bits);
-        vs.store(vt + buf * TILE, loader, bits);
+        ks.land(kt + buf * TILE, loader, bits);
+        vs.land(vt + buf * TILE, loader, bits);
     };
     // p and dp of the tile at j0; returns whether it is near, `side` its far side otherwise
     auto pair = [&](const S* kb, const S* vb, int j0, uint64_t now, f32x16 (&p)[NB], f32x16 (&dp)[NB], int& cell, int& side) {
         const int d0 = j0 - s.start - wrow;                             // the tile's first key from the wave's first query
         const bool near = near_tile(a.rel, d0 - 31, d0 + 32 * NB - 1);
         const int fb = a.rel.n > 0 && !near ? far_bucket(a.rel, d0 - 31) : 0;
-        const float far = (a.rel.n > 0 && !near ? LOG2E * a.bias[fb * a.heads + h] : 0.f);
+        const float far = near ? 0.f : fb > 0 ? fars.behind : fars.before;
         side = fb > 0;
         cell = near ? d0 - (lane & 31) + 4 * half - a.rel.edge[0] + REL_PAD : 0;
         const bool cut = a.causal && d0 + 32 * NB - 1 > 0;
@@ -134,8 +135,8 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
         seen = lane_bits(seen);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            p[k] = scores<M, DP>(kb, 32 * k, q);
-            dp[k] = scores<M, DP>(vb, 32 * k, go);
+            p[k] = scores<M, DP, (attn_width<T, DP> > 192)>(kb, 32 * k, q);
+            dp[k] = scores<M, DP, (attn_width<T, DP> > 192)>(vb, 32 * k, go);
         }
         if (near || hide) {
 #pragma unroll
@@ -167,20 +168,26 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
         constexpr int STEP = FORM == SPLIT ? 4 : 1;
         if (FORM == SPLIT) t += wave;
         meet();
-        if (t < last) fetch(t * Q::KEYS);
+        if (t < last) fetch(t * Q::KEYS, 0);
         if (!second) {                                                  // under the first tile's loads
             for (int u = FORM == SOLO ? lane : tid; u < reach; u += FORM == SOLO ? 64 : BWD_THREADS)
                 lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
             if (part != nullptr)
                 for (int u = FORM == SOLO ? lane : tid; u < (FORM == SOLO ? 2 : 8) * reach; u += FORM == SOLO ? 64 : BWD_THREADS) cells[u] = 0.f;
             if (FORM == SPLIT) __syncthreads();
+            q.wait();
+            go.wait();
+            settle(minus_lse);
+            settle(dl);
+            settle(fars.before);
+            settle(fars.behind);
         }
-        if (t < last) store(0);
+        if (t < last) land(0);
         meet();
         for (int n = 0; t < last; t += STEP, ++n) {
             const int j0 = t * Q::KEYS, buf = Q::BUFS == 2 ? n & 1 : 0;
             const uint64_t now = bits;
-            if (t + STEP < last) fetch(j0 + STEP * Q::KEYS);
+            if (t + STEP < last) fetch(j0 + STEP * Q::KEYS, Q::BUFS == 2 ? (n + 1) & 1 : 0);
             if (busy && j0 < wend) {
                 const S *kb = kt + buf * TILE, *vb = vt + buf * TILE;
                 f32x16 p[NB], dp[NB];
@@ -221,7 +228,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
                 }
             }
             if (Q::BUFS == 1) meet();
-            if (t + STEP < last) store(Q::BUFS == 2 ? (n + 1) & 1 : 0);
+            if (t + STEP < last) land(Q::BUFS == 2 ? (n + 1) & 1 : 0);
             meet();
         }
     };
@@ -342,7 +349,7 @@ struct KeySide {
 };
 
 template <typename T, int DP, bool ALONE>
-__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout,
+__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout,
                                                                                                    int64_t dout_ld, T* dk, int64_t dk_ld, T* dv, int64_t dv_ld,
                                                                                                    int key_blocks, BiasShares shares, int blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -390,11 +397,11 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
     const int first = a.causal ? max(0, key0 - s.start) / QT : 0;
     const int tiles = max(0, (s.nq + QT - 1) / QT - first);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
-    Staged<M, DP, QT, Kd::THREADS> qs, gs;
+    std::conditional_t<ALONE, Staged<M, DP, QT, Kd::THREADS>, Loader<M, DP, QT, Kd::THREADS>> qs, gs;
     float lv = -INFINITY, dv_ = 0.f;
-    auto fetch = [&](int h, int i0) {
-        qs.fetch((const T*)a.q + s.q0 * a.q_ld + (int64_t)h * a.dim, a.q_ld, i0, s.nq, chunks, loader);
-        gs.fetch(dout + s.q0 * dout_ld + (int64_t)h * a.dim, dout_ld, i0, s.nq, chunks, loader);
+    auto fetch = [&](int h, int i0, int buf) {
+        qs.fetch(qt + buf * TILE, (const T*)a.q + s.q0 * a.q_ld + (int64_t)h * a.dim, a.q_ld, i0, s.nq, chunks, loader);
+        gs.fetch(gt + buf * TILE, dout + s.q0 * dout_ld + (int64_t)h * a.dim, dout_ld, i0, s.nq, chunks, loader);
         lv = -INFINITY;
         dv_ = 0.f;
         if (loader < QT && i0 + loader < s.nq) {
@@ -403,9 +410,9 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
             dv_ = delta[(s.q0 + i0 + loader) * a.heads + h];
         }
     };
-    auto store = [&](int buf) {
-        qs.store(qt + buf * TILE, loader);
-        gs.store(gt + buf * TILE, loader);
+    auto land = [&](int i0, int buf) {
+        qs.land(qt + buf * TILE, loader, first_rows(s.nq - i0));
+        gs.land(gt + buf * TILE, loader, first_rows(s.nq - i0));
         if (loader < QT) {
             stats[buf * 2 * QT + loader] = lv;
             stats[buf * 2 * QT + QT + loader] = dv_;
@@ -414,13 +421,18 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
     for (int h = g * a.group; h < (g + 1) * a.group; ++h) {
         if (tiles == 0) break;
         meet();
-        fetch(h, first * QT);
+        fetch(h, first * QT, 0);
         for (int u = first_u; u < reach; u += step_u) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
-        store(0);
+        FarBias fars = far_bias(a, h);
+        k.wait();
+        v.wait();
+        settle(fars.before);
+        settle(fars.behind);
+        land(first * QT, 0);
         meet();
         for (int t = 0; t < tiles; ++t) {
             const int i0 = (first + t) * QT;
-            if (!ALONE && t + 1 < tiles) fetch(h, i0 + QT);             // (ALONE: the other waves cover the loads, the registers go further)
+            if (!ALONE && t + 1 < tiles) fetch(h, i0 + QT, (t + 1) & 1);             // (ALONE: the other waves cover the loads, the registers go further)
             const int buf = Kd::BUFS == 2 ? t & 1 : 0;
             const S *qb = qt + buf * TILE, *gb = gt + buf * TILE;
             const float* st = stats + buf * 2 * QT;
@@ -432,9 +444,9 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
                     const int d0 = wkey - s.start - r0;                 // the wave's first key from the step's first query
                     if (a.causal && d0 - 31 > 0) continue;              // its last query is before the wave's first key
                     const bool near = near_tile(a.rel, d0 - 31, d0 + 31);
-                    const float far = a.rel.n > 0 && !near ? LOG2E * a.bias[far_bucket(a.rel, d0 - 31) * a.heads + h] : 0.f;
+                    const float far = near ? 0.f : far_bucket(a.rel, d0 - 31) > 0 ? fars.behind : fars.before;
                     const bool cut = a.causal && d0 + 31 > 0;
-                    f32x16 p = scores<M, DP>(qb, 32 * n, k), dp = scores<M, DP>(gb, 32 * n, v);
+                    f32x16 p = scores<M, DP, (attn_width<T, DP> > 192)>(qb, 32 * n, k), dp = scores<M, DP>(gb, 32 * n, v);
                     f32x4 ml[4], dl[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -467,8 +479,8 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 128 ? 2 : 1)) vo
                 }
             if (ALONE) meet();
             if (t + 1 < tiles) {
-                if (ALONE) fetch(h, i0 + QT);
-                store(ALONE ? 0 : (t + 1) & 1);
+                if (ALONE) fetch(h, i0 + QT, 0);
+                land(i0 + QT, ALONE ? 0 : (t + 1) & 1);
             }
             meet();
         }

@@ -61,36 +61,40 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) v
     const int wend = a.causal ? s.start + min(wrow + 32, s.nq) : keys;  // keys from here on are hidden from the whole wave
 
     Softmax<M, DP> o;
-    Staged<M, DP, ROWS_KEYS, ROWS_THREADS> ks, vs;
+    Loader<M, DP, ROWS_KEYS, ROWS_THREADS> ks, vs;
     uint8_t kept = 1;
     uint64_t bits = 0;
-    auto fetch = [&](int j0) {
-        ks.fetch(K, a.k_ld, j0, s.nk, chunks, tid);
-        vs.fetch(V, a.v_ld, j0, s.nk, chunks, tid);
+    auto fetch = [&](int j0, int buf) {
+        ks.fetch(kt + buf * TILE, K, a.k_ld, j0, s.nk, chunks, tid);
+        vs.fetch(vt + buf * TILE, V, a.v_ld, j0, s.nk, chunks, tid);
         kept = lane < ROWS_KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
-    auto store = [&](int buf) {
+    auto land = [&](int buf) {
         bits = __ballot(kept != 0);
-        ks.store(kt + buf * TILE, tid, bits);
-        vs.store(vt + buf * TILE, tid, bits);
+        ks.land(kt + buf * TILE, tid, bits);
+        vs.land(vt + buf * TILE, tid, bits);
     };
-    if (tiles > 0) fetch(0);
+    if (tiles > 0) fetch(0, 0);
     const int reach = rel_reach(a.rel);                                 // (under the first tile's loads)
     for (int u = tid; u < reach; u += ROWS_THREADS) lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
-    if (tiles > 0) store(0);
+    FarBias fars = far_bias(a, h);
+    q.wait();
+    settle(fars.before);
+    settle(fars.behind);
+    if (tiles > 0) land(0);
     __syncthreads();
     for (int t = 0; t < tiles; ++t) {
         const int j0 = t * ROWS_KEYS;
         const uint64_t now = bits;
-        if (t + 1 < tiles) fetch(j0 + ROWS_KEYS);
+        if (t + 1 < tiles) fetch(j0 + ROWS_KEYS, (t + 1) & 1);
         if (busy && j0 < wend) {
             const S* kb = kt + (t & 1) * TILE;
             f32x16 sc[NB];
 #pragma unroll
-            for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(kb, 32 * k, q);
+            for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP, (attn_width<T, DP> > 192)>(kb, 32 * k, q);
             const int d0 = j0 - s.start - wrow;                         // distance of the tile's first key from the wave's first query
             const bool near = near_tile(a.rel, d0 - 31, d0 + ROWS_KEYS - 1);
-            const float far = a.rel.n > 0 && !near ? LOG2E * a.bias[far_bucket(a.rel, d0 - 31) * a.heads + h] : 0.f;
+            const float far = near ? 0.f : far_bucket(a.rel, d0 - 31) > 0 ? fars.behind : fars.before;
             const bool cut = a.causal && d0 + ROWS_KEYS - 1 > 0;
             float c = scale, add = far;
             if (near || cut || now != ~0ull >> (64 - ROWS_KEYS)) {
@@ -115,7 +119,7 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) v
             o.template step<NB>(sc, c, add);
             o.template weigh<NB>(vt + (t & 1) * TILE, sc);
         }
-        if (t + 1 < tiles) store((t + 1) & 1);
+        if (t + 1 < tiles) land((t + 1) & 1);
         __syncthreads();
     }
     if (row < s.nq) write_rows<T, M, DP>(a, o, s.q0 + row, h, out, out_ld, lse);
@@ -220,8 +224,8 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
     Staged<M, DP, SPLIT_KEYS, 64> ks, vs;
     uint8_t kept = 0;
     auto fetch = [&](int j0) {
-        ks.fetch(K, a.k_ld, j0, s.nk, chunks, lane);
-        vs.fetch(V, a.v_ld, j0, s.nk, chunks, lane);
+        ks.fetch(kt, K, a.k_ld, j0, s.nk, chunks, lane);
+        vs.fetch(vt, V, a.v_ld, j0, s.nk, chunks, lane);
         kept = lane < SPLIT_KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
     int t = SOLO ? (none ? t1 : 0) : t0 + wave;
@@ -242,13 +246,13 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
         const uint64_t now = __ballot(kept != 0);
         // the tile is this wave's own: its reads of the last step are behind these writes in program order
         __builtin_amdgcn_wave_barrier();
-        ks.store(kt, lane, now);
-        vs.store(vt, lane, now);
+        ks.land(kt, lane, now);
+        vs.land(vt, lane, now);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (t + STEP < t1) fetch((t + STEP) * SPLIT_KEYS);
         f32x16 sc[1];
-        sc[0] = scores<M, DP>(kt, 0, q);
+        sc[0] = scores<M, DP, (attn_width<T, DP> > 192)>(kt, 0, q);
         const int dmin = j0 - s.start - i1, dmax = j0 + SPLIT_KEYS - 1 - s.start - i0;
         const bool near = near_tile(a.rel, dmin, dmax);
         const float far = a.rel.n > 0 && !near ? table[far_bucket(a.rel, dmin) * wide + col] : 0.f;

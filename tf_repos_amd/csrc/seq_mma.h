@@ -16,6 +16,8 @@
 // Tiles: DP (a power of two >= the row's width, the rest zero) elements a row, 16-byte chunk c of row r at chunk c ^ swz(r).  A row read takes
 // one chunk of 32 consecutive rows, a column read (ds_read_b64_tr_b16) 64 bytes of 4 consecutive rows: swz spreads both over all 64 banks.
 #pragma once
+#include <type_traits>
+
 #include <hip/hip_bf16.h>
 
 #include "common.h"
@@ -243,6 +245,18 @@ template <> struct Mma<Split> {
     static __device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) { *reinterpret_cast<f32x4*>(p) = f32x4{a, b, c, d}; }
 };
 
+// Waits for a value's load here and not at its first use: within a loop that wait would hold up the tile loads under way (which the compiler does
+// not see) on every turn.
+__device__ __forceinline__ void settle(float& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void settle(int& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void settle(f32x4& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void settle(bf16x8& x) {
+    f32x4 y = __builtin_bit_cast(f32x4, x);
+    settle(y);
+    x = __builtin_bit_cast(bf16x8, y);
+}
+__device__ __forceinline__ void settle(Planes& x) { settle(x.h); settle(x.m); settle(x.l); }
+
 // 32 rows in registers, one a lane (both halves together hold a row's chunks): the B operand of the scores
 template <typename M, int DP>
 struct RowFrags {
@@ -261,15 +275,30 @@ struct RowFrags {
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) c[s] = Mma<M>::negate(c[s]);
     }
+    __device__ __forceinline__ void wait() {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) settle(c[s]);
+    }
 };
 
-// S of tile rows [row0, row0 + 32) against held rows
-template <typename M, int DP>
+// S of tile rows [row0, row0 + 32) against held rows.  LEAD: four reads of the tile before the first product and one behind each from there on.
+// For kernels of one wave a SIMD, which nothing else covers: the compiler spares registers there and has each read waited for.
+template <typename M, int DP, bool LEAD = false>
 __device__ __forceinline__ f32x16 scores(const typename Mma<M>::Store* tile, int row0, const RowFrags<M, DP>& held) {
     const int l = tile_lane<DP>(), row = row0 + (l & 31), g = l >> 5;
     f32x16 s = {};
 #pragma unroll
     for (int k = 0; k < RowFrags<M, DP>::STEPS; ++k) s = Mma<M>::dot(tile + Tile<M, DP>::at(row, 2 * k + g), held.c[k], s, DP);
+    if constexpr (LEAD) {
+        constexpr int P = Mma<M>::PLANES, PRODUCTS = P == 3 ? 6 : sizeof(typename Mma<M>::Store) == 2 ? 1 : 4;
+        constexpr int AHEAD = RowFrags<M, DP>::STEPS < 4 ? RowFrags<M, DP>::STEPS : 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * P, 0);
+#pragma unroll
+        for (int k = 0; k < RowFrags<M, DP>::STEPS; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+            if (k + AHEAD < RowFrags<M, DP>::STEPS) __builtin_amdgcn_sched_group_barrier(0x100, P, 0);
+        }
+    }
     return s;
 }
 
@@ -282,7 +311,7 @@ struct Staged {
     static_assert(N >= 1 && ROWS * CHUNKS % THREADS == 0, "a tile is a whole number of chunks a thread");
     f32x4 v[N][LOADS];
     // rows [first, first + ROWS) of those below `end`; the rest is zero
-    __device__ __forceinline__ void fetch(const T* base, int64_t ld, int64_t first, int64_t end, int chunks, int tid) {
+    __device__ __forceinline__ void fetch(S*, const T* base, int64_t ld, int64_t first, int64_t end, int chunks, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = tid + i * THREADS, r = at / CHUNKS, c = at % CHUNKS;
@@ -295,7 +324,7 @@ struct Staged {
         }
     }
     // rows whose bit is not set become zero, whatever the array holds there
-    __device__ __forceinline__ void store(S* tile, int tid, uint64_t rows = ~0ull) const {
+    __device__ __forceinline__ void land(S* tile, int tid, uint64_t rows) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = tid + i * THREADS, r = at / CHUNKS, c = at % CHUNKS;
@@ -315,6 +344,43 @@ struct Staged {
         }
     }
 };
+
+// The same straight into the tile (no registers: held back there, the compiler parks them in the accumulator file and waits for the loads to do
+// so).  A wave's load fills 64 consecutive 16-byte slots, so the swizzle is in the addresses that it reads.  Rows behind the end are read as the
+// last one and columns behind the row's width as its last chunk: the first become zero on landing, the second meet zeros in the held rows.
+template <typename M, int DP, int ROWS, int THREADS>
+struct Direct {
+    using T = typename Mma<M>::Global;
+    static constexpr int CHUNKS = Tile<M, DP>::CHUNKS, PER = Tile<M, DP>::PER, N = ROWS * CHUNKS / THREADS;
+    static_assert(N >= 1 && ROWS * CHUNKS % THREADS == 0 && THREADS % 64 == 0 && Mma<M>::PLANES == 1, "a wave's load is 64 slots of a tile of one plane");
+    __device__ __forceinline__ void fetch(T* tile, const T* base, int64_t ld, int64_t first, int64_t end, int chunks, int tid) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = tid + i * THREADS, r = at / CHUNKS, c = (at % CHUNKS) ^ Tile<M, DP>::swz(r);
+            const int64_t row = first + r < end ? first + r : end - 1;
+            const T* from = base + row * ld + (c < chunks ? c : chunks - 1) * PER;
+            const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)(tile + (at & ~63) * PER);
+            uint32_t m0;                                                // (kept: the register is the compiler's)
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                         : "=&s"(m0) : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(from) : "memory");
+        }
+    }
+    // to be called before the barrier behind which the tile is read; rows whose bit is not set become zero
+    __device__ __forceinline__ void land(T* tile, int tid, uint64_t rows) const {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if ((rows | (ROWS < 64 ? ~0ull << (ROWS & 63) : 0)) == ~0ull) return;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = tid + i * THREADS;
+            if (!(rows >> (at / CHUNKS) & 1)) *reinterpret_cast<f32x4*>(tile + at * PER) = f32x4{};
+        }
+    }
+};
+
+template <typename M, int DP, int ROWS, int THREADS>
+struct Loader : std::conditional_t<Mma<M>::PLANES == 1, Direct<M, DP, ROWS, THREADS>, Staged<M, DP, ROWS, THREADS>> {};
+
+__device__ __forceinline__ uint64_t first_rows(int64_t n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
 
 // bits of 64 consecutive tile rows as register r of 32-row block `blk` sees them: bit reg_row(r) + 32 blk of the shifted word
 __device__ __forceinline__ uint64_t lane_bits(uint64_t rows) { return rows >> (4 * ((threadIdx.x >> 5) & 1)); }

@@ -97,6 +97,8 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 :
     using M = VocabKind<T, DP>;
     using S = typename Mma<M>::Store;
     constexpr int NB = Ti::NB;
+    // (not where a second step's scores are what takes the kernel past two waves a SIMD: bf16 of 128, 213 us against 166 at 1024 x 100000)
+    constexpr bool AHEAD = !(DX && Ti::WIDTH == 256);
     S* tiles = reinterpret_cast<S*>(lds);
     float* bias = reinterpret_cast<float*>(tiles + 3 * Ti::SIZE);                       // [3][ROWS]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -106,46 +108,58 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 :
     const bool on = n < a.N, busy = rb * 128 + wave * 32 < a.N;
     RowFrags<M, DP> x;
     x.load((const T*)a.x + n * a.x_ld, chunks, on);
-    const int64_t label = on ? a.labels[n] : -1;
+    int label = on ? a.labels[n] : -1;
     Softmax<M, DP> o;
-    Staged<M, DP, Ti::ROWS, VS_THREADS> ws;
+    Loader<M, DP, Ti::ROWS, VS_THREADS> ws;
     float bv = 0.f;
-    auto fetch = [&](int64_t v) {
-        ws.fetch((const T*)a.w, a.w_ld, v, v1, chunks, tid);
+    auto fetch = [&](int64_t v, int buf) {
+        ws.fetch(tiles + buf * Ti::SIZE, (const T*)a.w, a.w_ld, v, v1, chunks, tid);
         if (a.b != nullptr && tid < Ti::ROWS) bv = v + tid < v1 ? LOG2E * a.b[v + tid] : 0.f;
     };
-    auto store = [&](int buf) {
-        ws.store(tiles + buf * Ti::SIZE, tid);
+    auto land = [&](int64_t v, int buf) {
+        ws.land(tiles + buf * Ti::SIZE, tid, first_rows(v1 - v));
         if (a.b != nullptr && tid < Ti::ROWS) bias[buf * Ti::ROWS + tid] = bv;
     };
+    x.wait();
+    settle(label);
     if (v0 < v1) {                                                                      // (rows behind v1 are zeros)
-        fetch(v0);
-        store(0);
-        fetch(v0 + Ti::ROWS);
-        store(1);
+        fetch(v0, 0);
+        land(v0, 0);
+        fetch(v0 + Ti::ROWS, 1);
+        land(v0 + Ti::ROWS, 1);
     }
     __syncthreads();
     f32x16 sc[NB];
+    if (AHEAD) {
 #pragma unroll
-    for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(tiles, 32 * k, x);
+        for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(tiles, 32 * k, x);
+    }
     int now = 0;
     for (int64_t v = v0; v < v1; v += Ti::ROWS) {
         const int next = now == 2 ? 0 : now + 1, then = next == 2 ? 0 : next + 1;
         const bool more = v + 2 * Ti::ROWS < v1;
-        if (more) fetch(v + 2 * Ti::ROWS);
+        if (more) fetch(v + 2 * Ti::ROWS, then);
         if (busy) {
+            if (!AHEAD) {
+#pragma unroll
+                for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(tiles + now * Ti::SIZE, 32 * k, x);
+            }
             const float c = adjust<NB>(sc, a.b != nullptr ? bias + now * Ti::ROWS : nullptr, v, v1, label);
             const float off = o.template raise<NB>(sc, c, 0.f);
             f32x16 ahead[NB];
+            if (AHEAD) {
 #pragma unroll
-            for (int k = 0; k < NB; ++k) ahead[k] = scores<M, DP>(tiles + next * Ti::SIZE, 32 * k, x);
+                for (int k = 0; k < NB; ++k) ahead[k] = scores<M, DP>(tiles + next * Ti::SIZE, 32 * k, x);
+            }
             o.template weights<NB>(sc, c, off);
             if (DX) o.template weigh<NB>(tiles + now * Ti::SIZE, sc);
 
+            if (AHEAD) {
 #pragma unroll
-            for (int k = 0; k < NB; ++k) sc[k] = ahead[k];
+                for (int k = 0; k < NB; ++k) sc[k] = ahead[k];
+            }
         }
-        if (more) store(then);
+        if (more) land(v + 2 * Ti::ROWS, then);
         __syncthreads();
         now = next;
     }
@@ -177,14 +191,14 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1
     Staged<M, DP, 32, 64> ws;
     float bv = 0.f;
     auto fetch = [&](int64_t v) {
-        ws.fetch((const T*)a.w, a.w_ld, v, v1, chunks, lane);
+        ws.fetch(tile, (const T*)a.w, a.w_ld, v, v1, chunks, lane);
         if (a.b != nullptr && lane < 32) bv = v + lane < v1 ? LOG2E * a.b[v + lane] : 0.f;
     };
     int64_t v = v0 + 32 * wave;
     if (v < v1) fetch(v);
     for (; v < v1; v += 128) {
         __builtin_amdgcn_wave_barrier();
-        ws.store(tile, lane);
+        ws.land(tile, lane, ~0ull);
         if (a.b != nullptr && lane < 32) bias[lane] = bv;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -289,38 +303,41 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1
     const bool on = v < a.V;
     RowFrags<M, DP> w;
     w.load((const T*)a.w + v * a.w_ld, chunks, on);
-    const float bv = on && a.b != nullptr ? LOG2E * a.b[v] : 0.f;
+    float bv = on && a.b != nullptr ? LOG2E * a.b[v] : 0.f;
+    w.wait();
+    settle(bv);
     f32x16 acc[DP / 32] = {};
     float sum = 0.f;
-    Staged<M, DP, Ti::ROWS, VS_THREADS> xs;
+    Loader<M, DP, Ti::ROWS, VS_THREADS> xs;
     float lv = 0.f, cv = 0.f;
     int label = -1;
-    auto fetch = [&](int n) {
-        xs.fetch((const T*)a.x, a.x_ld, n, n1, chunks, tid);
+    auto fetch = [&](int n, int buf) {
+        xs.fetch(tiles + buf * Ti::SIZE, (const T*)a.x, a.x_ld, n, n1, chunks, tid);
         const int r = n + lane;                                                         // (every wave: the rows' bits)
-        label = lane < Ti::ROWS && r < n1 ? a.labels[r] : -1;
-        if (label >= a.V) label = -1;
-        lv = label >= 0 ? -LOG2E * lse[r] : -INFINITY;                                  // no label: p = 2^-inf = 0
-        if (a.row_scale != nullptr) cv = label >= 0 ? a.row_scale[r] : 0.f;
+        const bool there = lane < Ti::ROWS && r < n1;
+        label = there ? a.labels[r] : -1;                                               // (all looked at on landing: nothing waits here)
+        lv = there ? lse[r] : 0.f;
+        if (a.row_scale != nullptr) cv = there ? a.row_scale[r] : 0.f;
     };
-    auto store = [&](int buf) {
-        xs.store(tiles + buf * Ti::SIZE, tid, __ballot(label >= 0));
+    auto land = [&](int buf) {
+        const bool labelled = label >= 0 && label < a.V;
+        xs.land(tiles + buf * Ti::SIZE, tid, __ballot(labelled));
         if (wave == 0 && lane < Ti::ROWS) {
             float* st = stats + buf * 3 * Ti::ROWS + lane;
-            st[0] = lv;
-            st[Ti::ROWS] = cv;
-            reinterpret_cast<int32_t*>(st)[2 * Ti::ROWS] = label;
+            st[0] = labelled ? -LOG2E * lv : -INFINITY;                                 // no label: p = 2^-inf = 0
+            st[Ti::ROWS] = labelled ? cv : 0.f;
+            reinterpret_cast<int32_t*>(st)[2 * Ti::ROWS] = labelled ? label : -1;
         }
     };
     if (n0 < n1) {
-        fetch(n0);
-        store(0);
+        fetch(n0, 0);
+        land(0);
     }
     __syncthreads();
     int buf = 0;
     for (int n = n0; n < n1; n += Ti::ROWS, buf ^= 1) {
         const bool more = n + Ti::ROWS < n1;
-        if (more) fetch(n + Ti::ROWS);
+        if (more) fetch(n + Ti::ROWS, buf ^ 1);
         const S* xt = tiles + buf * Ti::SIZE;
         const float* st = stats + buf * 3 * Ti::ROWS;
         const int32_t* lt = reinterpret_cast<const int32_t*>(st) + 2 * Ti::ROWS;
@@ -357,7 +374,7 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(xt, 32 * k, 32 * d, g, acc[d]);
         }
-        if (more) store(buf ^ 1);
+        if (more) land(buf ^ 1);
         __syncthreads();
     }
     sum = both_sum(sum);
