@@ -18,19 +18,51 @@ enum { ROWS = 0, SPLIT = 1, SOLO = 2 };
 template <typename T, int DP, int FORM>
 struct QuerySide {
     using M = AttnKind<T, DP>;
-    static constexpr int NB = FORM == ROWS && attn_width<T, DP> <= 256 ? 2 : 1, KEYS = 32 * NB, BUFS = FORM == ROWS ? 2 : 1, THREADS = FORM == ROWS ? 256 : 64;
+    static constexpr int NB = FORM == ROWS && attn_width<T, DP> <= 256 ? 2 : 1, KEYS = 32 * NB, BUFS = FORM == ROWS || sizeof(T) == 2 ? 2 : 1, THREADS = FORM == ROWS ? 256 : 64;
     static constexpr int TILE = KEYS * Tile<M, DP>::STRIDE, ITEM_ROWS = FORM == ROWS ? 128 : 32;
     static constexpr size_t tiles = (FORM == ROWS ? 1 : 4) * 2 * BUFS * KEYS * attn_width<T, DP>, join = FORM == SPLIT ? 4 * 32 * (DP + 4) * sizeof(float) : 0;
     static constexpr size_t first = tiles > join ? tiles : join;
 };
 
-// Sums of ds by distance.  A near tile adds every element to its distance's cell: of one half-wave and register no two lanes (queries) share a
-// distance, so each half of each wave has cells of its own and the order of every cell's sum is the program's.
-__device__ __forceinline__ void lds_add(float* cell, float x) { __hip_atomic_fetch_add(cell, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+// Sums of a 32 x 32 block of ds by distance, into the wave's cells (`cells`: that of the block's first key and first query).  A block's rows go to
+// shared memory each shifted by its own number, so that equal distances stand in one column; the columns' sums are then added to the cells.  16 queries
+// at a time: 16 x 48 floats, of which a row always writes the same 32 and the rest stays zero.  (Float atomics to the cells took 64 and more cycles an
+// instruction: 104 us of a 254 us pass over 8 x 2048 causal steps, 8 heads.)  The order of every sum is the program's.
+constexpr int SKEW = 16 * 48;
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+__device__ __forceinline__ void add_diagonals(float* skew, const f32x16& x, float* cells) {
+    const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 15, quad = lane & 15, group = lane >> 4;
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+        wave_order();
+        if ((group & 1) == pass) {
+            float* to = skew + row * 47 + 15 + 4 * half;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) to[reg_row(r)] = x[r];
+        }
+        wave_order();
+        f32x4 sum = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += *reinterpret_cast<const f32x4*>(skew + (4 * group + j) * 48 + 4 * min(quad, 11));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t y = __float_as_uint(sum[e]);
+            const auto z = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+            const uint32_t even = z[0], odd = z[1];
+            sum[e] = both_sum(__uint_as_float(even) + __uint_as_float(odd));
+        }
+        const float mine = group == 0 ? sum[0] : group == 1 ? sum[1] : group == 2 ? sum[2] : sum[3];
+        const int c = 4 * quad + group;
+        if (c < 47) cells[c - 15 - 16 * pass] += mine;
+    }
+}
 
 // part: [head][segment * row_blocks + row block][n_buckets] shares of the bias gradient, or null; delta [total_q, heads]
 template <typename T, int DP, int FORM>
-__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
+__global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == ROWS && attn_width<T, DP> == 384) ? 2 : 1)) void attn_bwd_q_kernel(AttnView a, const T* out, int64_t out_ld, const float* lse, const T* dout, int64_t dout_ld,
                                                                  T* dq, int64_t dq_ld, float* delta, float* part, int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Q = QuerySide<T, DP, FORM>;
@@ -43,7 +75,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     constexpr bool ROUNDED = Mma<M>::ROUNDS;
     constexpr bool OWN = FORM != ROWS;                                  // tiles of a wave's own
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-    S* kt = reinterpret_cast<S*>(lds) + (OWN ? wave * 2 * TILE : 0);
+    S* kt = reinterpret_cast<S*>(lds) + (OWN ? wave * 2 * Q::BUFS * TILE : 0);
     S* vt = kt + Q::BUFS * TILE;
     const int64_t items = (int64_t)row_blocks * a.heads * a.n_seg, at_item = FORM == SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     const int item = (int)min(at_item, items - 1);
@@ -70,10 +102,11 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     const int chunks = a.dim / Tile<M, DP>::PER;
     const float scale = a.scale * LOG2E;
     const int reach = rel_reach(a.rel);
-    // SOLO: every wave's own table and 2 x reach cells; else one table, [4 waves][2 halves][reach] cells; 2 x 4 far sums
-    float* lut = reinterpret_cast<float*>(lds + Q::first) + (FORM == SOLO ? wave * 3 * reach : 0);
+    // skewed blocks, a wave each; SOLO: every wave's own table and cells; else one table, [4 waves][reach] cells; 2 x 4 far sums
+    float* skew = reinterpret_cast<float*>(lds + Q::first) + wave * SKEW;
+    float* lut = reinterpret_cast<float*>(lds + Q::first) + 4 * SKEW + (FORM == SOLO ? wave * 2 * reach : 0);
     float* cells = lut + reach;
-    float* mine = cells + (FORM == SOLO ? half : 2 * wave + half) * reach;
+    float* mine = cells + (FORM == SOLO ? 0 : wave * reach);
     const int loader = OWN ? lane : tid;
 
     RowFrags<M, DP> q, go;
@@ -104,7 +137,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     FarBias fars = far_bias(a, h);
     f32x16 acc[DP / 32] = {}, pk[ROUNDED ? DP / 32 : 1] = {};
     float far_ds[2] = {0.f, 0.f}, far_p[2] = {0.f, 0.f}, pdp = 0.f;     // [below the first boundary, from the last one on]
-    std::conditional_t<OWN, Staged<M, DP, Q::KEYS, Q::THREADS>, Loader<M, DP, Q::KEYS, Q::THREADS>> ks, vs;
+    std::conditional_t<Q::BUFS == 2, Loader<M, DP, Q::KEYS, Q::THREADS>, Staged<M, DP, Q::KEYS, Q::THREADS>> ks, vs;
     uint64_t bits = 0;                                                  // kept keys of the tile
     uint8_t kept = 0;
     auto fetch = [&](int j0, int buf) {
@@ -117,6 +150,8 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
         ks.land(kt + buf * TILE, loader, bits);
         vs.land(vt + buf * TILE, loader, bits);
     };
+    // cell of the distance between a block's first key and the wave's first query
+    auto block_cell = [&](int key) { return key - s.start - wrow - a.rel.edge[0] + REL_PAD; };
     // p and dp of the tile at j0; returns whether it is near, `side` its far side otherwise
     auto pair = [&](const S* kb, const S* vb, int j0, uint64_t now, f32x16 (&p)[NB], f32x16 (&dp)[NB], int& cell, int& side) {
         const int d0 = j0 - s.start - wrow;                             // the tile's first key from the wave's first query
@@ -173,7 +208,9 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
             for (int u = FORM == SOLO ? lane : tid; u < reach; u += FORM == SOLO ? 64 : BWD_THREADS)
                 lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
             if (part != nullptr)
-                for (int u = FORM == SOLO ? lane : tid; u < (FORM == SOLO ? 2 : 8) * reach; u += FORM == SOLO ? 64 : BWD_THREADS) cells[u] = 0.f;
+                for (int u = FORM == SOLO ? lane : tid; u < (FORM == SOLO ? 1 : 4) * reach; u += FORM == SOLO ? 64 : BWD_THREADS) cells[u] = 0.f;
+            if (part != nullptr && reach > 0)
+                for (int u = lane; u < SKEW; u += 64) skew[u] = 0.f;
             if (FORM == SPLIT) __syncthreads();
             q.wait();
             go.wait();
@@ -195,13 +232,23 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
                 const bool near = pair(kb, vb, j0, now, p, dp, cell, side);
                 if (!second) {
                     if (ROUNDED || (part != nullptr && !near)) {
-                        float x = 0.f, y = 0.f;
+                        float x[2] = {0.f, 0.f};
 #pragma unroll
                         for (int k = 0; k < NB; ++k)
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) { x = fmaf(p[k][r], dp[k][r], x); y += p[k][r]; }
-                        pdp += x;
-                        if (!near) { far_ds[side] += x; far_p[side] += y; }
+                            for (int r = 0; r < 16; ++r) x[r & 1] = fmaf(p[k][r], dp[k][r], x[r & 1]);
+                        pdp += x[0] + x[1];
+                        if (part != nullptr && !near) {
+                            float y[2] = {0.f, 0.f};
+#pragma unroll
+                            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) y[r & 1] += p[k][r];
+                            far_ds[0] += side ? 0.f : x[0] + x[1];
+                            far_ds[1] += side ? x[0] + x[1] : 0.f;
+                            far_p[0] += side ? 0.f : y[0] + y[1];
+                            far_p[1] += side ? y[0] + y[1] : 0.f;
+                        }
                     }
 #pragma unroll
                     for (int k = 0; k < NB; ++k) {
@@ -213,18 +260,18 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
                         }
 #pragma unroll
                         for (int r = 0; r < 16; ++r) p[k][r] *= dp[k][r] - dl;
-                        if (!ROUNDED && part != nullptr && near)
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) lds_add(mine + cell + 32 * k + reg_row(r), p[k][r]);
+                        if (!ROUNDED && part != nullptr && near) add_diagonals(skew, p[k], mine + block_cell(j0 + 32 * k));
                         const auto w = Mma<M>::pack(p[k]);
 #pragma unroll
                         for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(kb, 32 * k, 32 * d, w, acc[d]);
                     }
                 } else if (near) {
 #pragma unroll
-                    for (int k = 0; k < NB; ++k)
+                    for (int k = 0; k < NB; ++k) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) lds_add(mine + cell + 32 * k + reg_row(r), p[k][r] * (dp[k][r] - dl));
+                        for (int r = 0; r < 16; ++r) p[k][r] *= dp[k][r] - dl;
+                        add_diagonals(skew, p[k], mine + block_cell(j0 + 32 * k));
+                    }
                 }
             }
             if (Q::BUFS == 1) meet();
@@ -254,8 +301,8 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
         float far_sum[2];
 #pragma unroll
         for (int side = 0; side < 2; ++side) far_sum[side] = wave_sum(fmaf(-dl, far_p[side], far_ds[side]));
-        constexpr int WAYS = FORM == SOLO ? 2 : 8;
-        float* fars = cells + 8 * reach;                                // (not SOLO's)
+        constexpr int WAYS = FORM == SOLO ? 1 : 4;
+        float* fars = cells + 4 * reach;                                // (not SOLO's)
         if (FORM != SOLO && lane == 0) {
             fars[wave] = far_sum[0];
             fars[4 + wave] = far_sum[1];
@@ -340,46 +387,52 @@ __device__ __forceinline__ void sum_shares(const BiasShares& x, int n, int heads
 }
 
 // ---- key side ------------------------------------------------------------------------------------------------------------------------
-// A block's waves take 32 keys each and share the tiles of queries; ALONE: a wave has 32 keys, and 32-query tiles, to itself.
-template <typename T, int DP, bool ALONE>
+// Key-side forms: KEY_ROWS a block's waves take 32 keys each and share the tiles of queries; KEY_SPLIT the waves take 32-query tiles of their own for
+// the same 32 keys and add up at the end; KEY_SOLO a wave has 32 keys to itself.
+enum { KEY_ROWS = 0, KEY_SPLIT = 1, KEY_SOLO = 2 };
+template <typename T, int DP, int FORM>
 struct KeySide {
     using M = AttnKind<T, DP>;
-    static constexpr int QT = !ALONE && attn_width<T, DP> <= 256 ? 64 : 32, TILE = QT * Tile<M, DP>::STRIDE, BUFS = ALONE ? 1 : 2, THREADS = ALONE ? 64 : 256;      // queries of a tile
-    static constexpr size_t tiles = (ALONE ? 4 : 1) * 2 * BUFS * QT * attn_width<T, DP>, stats = (ALONE ? 4 : 1) * BUFS * 2 * QT * sizeof(float);
+    static constexpr bool OWN = FORM != KEY_ROWS;
+    static constexpr int QT = !OWN && attn_width<T, DP> <= 256 ? 64 : 32, TILE = QT * Tile<M, DP>::STRIDE, THREADS = OWN ? 64 : 256;      // queries of a tile
+    static constexpr int BUFS = !OWN || sizeof(T) == 2 ? 2 : 1;         // (planes pass through registers: there the other waves cover the loads)
+    static constexpr size_t tiles = (OWN ? 4 : 1) * 2 * BUFS * QT * attn_width<T, DP>, stats = (OWN ? 4 : 1) * BUFS * 2 * QT * sizeof(float);
+    static_assert(FORM != KEY_SPLIT || tiles >= 4 * 32 * (DP + 4) * sizeof(float), "the waves' sums meet in the tiles' place");
 };
 
-template <typename T, int DP, bool ALONE>
+template <typename T, int DP, int FORM>
 __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout,
                                                                                                    int64_t dout_ld, T* dk, int64_t dk_ld, T* dv, int64_t dv_ld,
                                                                                                    int key_blocks, BiasShares shares, int blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    using Kd = KeySide<T, DP, ALONE>;
+    using Kd = KeySide<T, DP, FORM>;
     using M = AttnKind<T, DP>;
     using S = typename Mma<M>::Store;
-    constexpr int QT = Kd::QT, TILE = Kd::TILE;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, kv_heads = a.heads / a.group, loader = ALONE ? lane : tid;
-    S* qt = reinterpret_cast<S*>(lds) + (ALONE ? wave * 2 * TILE : 0);
-    S* gt = qt + Kd::BUFS * TILE;
-    float* stats = reinterpret_cast<float*>(lds + Kd::tiles) + (ALONE ? wave * 2 * QT : 0);       // [buffer][-log2(e) lse, delta][QT]
+    constexpr int QT = Kd::QT, TILE = Kd::TILE, BUFS = Kd::BUFS, STEP = FORM == KEY_SPLIT ? 4 : 1;
+    constexpr bool OWN = Kd::OWN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, kv_heads = a.heads / a.group, loader = OWN ? lane : tid;
+    S* qt = reinterpret_cast<S*>(lds) + (OWN ? wave * 2 * BUFS * TILE : 0);
+    S* gt = qt + BUFS * TILE;
+    float* stats = reinterpret_cast<float*>(lds + Kd::tiles) + (OWN ? wave * BUFS * 2 * QT : 0);  // [buffer][-log2(e) lse, delta][QT]
     if ((int)blockIdx.x >= blocks) {
         sum_shares(shares, a.rel.n, a.heads, blockIdx.x - blocks, reinterpret_cast<float*>(lds));
         return;
     }
-    const int64_t items = (int64_t)key_blocks * kv_heads * a.n_seg, at_item = ALONE ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-    if (at_item >= items) return;                                       // (ALONE has no barriers)
+    const int64_t items = (int64_t)key_blocks * kv_heads * a.n_seg, at_item = FORM == KEY_SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    if (at_item >= items) return;                                       // (KEY_SOLO has no barriers)
     const int item = (int)at_item, kb = item % key_blocks, g = item / key_blocks % kv_heads, b = item / key_blocks / kv_heads;
     const Segment s = load_segment(a, b);
-    const int key0 = kb * (ALONE ? 32 : 128);
+    const int key0 = kb * (OWN ? 32 : 128);
     if (key0 >= s.nk) return;
-    const int wkey = key0 + (ALONE ? 0 : wave * 32), key = wkey + (lane & 31);
+    const int wkey = key0 + (OWN ? 0 : wave * 32), key = wkey + (lane & 31);
     const int chunks = a.dim / Tile<M, DP>::PER;
     const float scale = a.scale * LOG2E;
-    const int reach = rel_reach(a.rel), first_u = ALONE ? lane : tid, step_u = Kd::THREADS;
-    float* lut = reinterpret_cast<float*>(lds + Kd::tiles + Kd::stats) + (ALONE ? wave * 2 * reach : 0);
+    const int reach = rel_reach(a.rel), first_u = OWN ? lane : tid, step_u = Kd::THREADS;
+    float* lut = reinterpret_cast<float*>(lds + Kd::tiles + Kd::stats) + (OWN ? wave * 2 * reach : 0);
     int32_t* buckets = reinterpret_cast<int32_t*>(lut + reach);         // of every distance
     for (int u = first_u; u < reach; u += step_u) buckets[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u);
     auto meet = [&] {
-        if (ALONE) {
+        if (OWN) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
         } else {
@@ -397,16 +450,15 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     const int first = a.causal ? max(0, key0 - s.start) / QT : 0;
     const int tiles = max(0, (s.nq + QT - 1) / QT - first);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
-    std::conditional_t<ALONE, Staged<M, DP, QT, Kd::THREADS>, Loader<M, DP, QT, Kd::THREADS>> qs, gs;
-    float lv = -INFINITY, dv_ = 0.f;
+    std::conditional_t<BUFS == 2, Loader<M, DP, QT, Kd::THREADS>, Staged<M, DP, QT, Kd::THREADS>> qs, gs;
+    float lv = -INFINITY, dv_ = 0.f;                                    // as loaded: nothing waits for them before the tile lands
     auto fetch = [&](int h, int i0, int buf) {
         qs.fetch(qt + buf * TILE, (const T*)a.q + s.q0 * a.q_ld + (int64_t)h * a.dim, a.q_ld, i0, s.nq, chunks, loader);
         gs.fetch(gt + buf * TILE, dout + s.q0 * dout_ld + (int64_t)h * a.dim, dout_ld, i0, s.nq, chunks, loader);
         lv = -INFINITY;
         dv_ = 0.f;
         if (loader < QT && i0 + loader < s.nq) {
-            const float L = lse[(s.q0 + i0 + loader) * a.heads + h];
-            lv = L == -INFINITY ? -INFINITY : -LOG2E * L;               // p = 2^-inf = 0 for a row that saw nothing, and behind the last row
+            lv = lse[(s.q0 + i0 + loader) * a.heads + h];
             dv_ = delta[(s.q0 + i0 + loader) * a.heads + h];
         }
     };
@@ -414,26 +466,27 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
         qs.land(qt + buf * TILE, loader, first_rows(s.nq - i0));
         gs.land(gt + buf * TILE, loader, first_rows(s.nq - i0));
         if (loader < QT) {
-            stats[buf * 2 * QT + loader] = lv;
+            stats[buf * 2 * QT + loader] = lv == -INFINITY ? -INFINITY : -LOG2E * lv;        // p = 2^-inf = 0 for a row that saw nothing, and behind the last row
             stats[buf * 2 * QT + QT + loader] = dv_;
         }
     };
     for (int h = g * a.group; h < (g + 1) * a.group; ++h) {
         if (tiles == 0) break;
+        int t = FORM == KEY_SPLIT ? wave : 0;
         meet();
-        fetch(h, first * QT, 0);
+        if (t < tiles) fetch(h, (first + t) * QT, 0);
         for (int u = first_u; u < reach; u += step_u) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
         FarBias fars = far_bias(a, h);
         k.wait();
         v.wait();
         settle(fars.before);
         settle(fars.behind);
-        land(first * QT, 0);
+        if (t < tiles) land((first + t) * QT, 0);
         meet();
-        for (int t = 0; t < tiles; ++t) {
-            const int i0 = (first + t) * QT;
-            if (!ALONE && t + 1 < tiles) fetch(h, i0 + QT, (t + 1) & 1);             // (ALONE: the other waves cover the loads, the registers go further)
-            const int buf = Kd::BUFS == 2 ? t & 1 : 0;
+        for (int turn = 0; t < tiles; t += STEP, ++turn) {
+            const int i0 = (first + t) * QT, then = i0 + STEP * QT, buf = BUFS == 2 ? turn & 1 : 0;
+            const bool more = t + STEP < tiles;
+            if (BUFS == 2 && more) fetch(h, then, buf ^ 1);
             const S *qb = qt + buf * TILE, *gb = gt + buf * TILE;
             const float* st = stats + buf * 2 * QT;
             if (busy)
@@ -477,19 +530,50 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
                         ak[d] = Mma<M>::template weigh<DP>(qb, 32 * n, 32 * d, wd, ak[d]);
                     }
                 }
-            if (ALONE) meet();
-            if (t + 1 < tiles) {
-                if (ALONE) fetch(h, i0 + QT, 0);
-                land(i0 + QT, ALONE ? 0 : (t + 1) & 1);
+            if (BUFS == 1) meet();
+            if (more) {
+                if (BUFS == 1) fetch(h, then, 0);
+                land(then, BUFS == 2 ? buf ^ 1 : 0);
             }
             meet();
         }
     }
-    if (key >= s.nk) return;
     if (!on) {                                                          // (0, also where an infinite dout has met the zeros in its place)
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) ak[d] = av[d] = f32x16{};
     }
+    if (FORM == KEY_SPLIT) {                                            // the four waves' sums meet, dk's and then dv's
+        float* join = reinterpret_cast<float*>(lds);
+        const int r = tid >> 3, c0 = (tid & 7) * (DP / 8);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const f32x16& x = which == 0 ? ak[d] : av[d];
+                    *reinterpret_cast<f32x4*>(join + (wave * 32 + (lane & 31)) * (DP + 4) + 32 * d + 8 * e + 4 * half) =
+                        f32x4{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
+                }
+            __syncthreads();
+            if (key0 + r < s.nk) {
+                const float by = which == 0 ? a.scale : 1.f;
+                T* to = (which == 0 ? dk + (s.k0 + key0 + r) * dk_ld : dv + (s.k0 + key0 + r) * dv_ld) + (int64_t)g * a.dim + c0;
+#pragma unroll
+                for (int d = 0; d < DP / 8; d += 4) {
+                    if (c0 + d >= a.dim) break;
+                    f32x4 x = *reinterpret_cast<f32x4*>(join + r * (DP + 4) + c0 + d);
+#pragma unroll
+                    for (int w = 1; w < 4; ++w) x += *reinterpret_cast<f32x4*>(join + (w * 32 + r) * (DP + 4) + c0 + d);
+                    x *= by;
+                    Mma<T>::store4(to + d, x[0], x[1], x[2], x[3]);
+                }
+            }
+        }
+        return;
+    }
+    if (key >= s.nk) return;
     T* tk = dk + (s.k0 + key) * dk_ld + (int64_t)g * a.dim + 4 * half;
     T* tv = dv + (s.k0 + key) * dv_ld + (int64_t)g * a.dim + 4 * half;
 #pragma unroll
@@ -503,14 +587,24 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
+#ifndef QUERY_ROWS_FROM
+#define QUERY_ROWS_FROM 0
+#define KEY_ROWS_FROM 200
+#endif
 static int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
-// Short query lists leave three of four row waves idle: there the waves share the keys instead, or are items of their own (not for f32 heads
-// wider than 64, whose registers do not suffice).
+// Which form: a wave to an item where they are many and short; else rows where those blocks fill the chip, or the waves share an item's other side.
+// (f32 heads wider than 64 have the rows form only, as bias tables beyond 256 distances between first and last boundary: registers, shared memory.)
+static bool rows_only(const dctr_attention* a) { return (a->dtype == DCTR_TYPE_F32 && a->head_dim > 64) || rel_reach(a) > 512; }
 static int query_form(const dctr_attention* a) {
-    if (a->max_q > 64 || (a->dtype == DCTR_TYPE_F32 && a->head_dim > 64)) return ROWS;
-    return attn_solo(a, (int64_t)ceil_div(a->max_q, 32) * a->heads * a->n_seg) ? SOLO : SPLIT;
+    if (rows_only(a)) return ROWS;
+    if (a->max_q <= 64 && attn_solo(a, (int64_t)ceil_div(a->max_q, 32) * a->heads * a->n_seg)) return SOLO;
+    return a->max_q <= 64 || (a->total_q / 128 + a->n_seg) * a->heads < QUERY_ROWS_FROM ? SPLIT : ROWS;
 }
-static bool keys_alone(const dctr_attention* a) { return a->max_q <= 128 && attn_solo(a, (int64_t)ceil_div(a->max_k, 32) * a->kv_heads * a->n_seg); }
+static int key_form(const dctr_attention* a) {
+    if (rows_only(a)) return KEY_ROWS;
+    if (a->max_q <= 128 && attn_solo(a, (int64_t)ceil_div(a->max_k, 32) * a->kv_heads * a->n_seg)) return KEY_SOLO;
+    return (a->total_k / 128 + a->n_seg) * a->kv_heads < KEY_ROWS_FROM ? KEY_SPLIT : KEY_ROWS;
+}
 static int row_blocks_of(const dctr_attention* a) { return ceil_div(a->max_q, query_form(a) == ROWS ? 128 : 32); }
 
 // delta, then the bias gradient's shares
@@ -524,22 +618,22 @@ static int launch_q(const dctr_attention* a, const AttnView& v, const AttnGrads&
     const int64_t items = (int64_t)row_blocks * a->heads * a->n_seg, blocks = FORM == SOLO ? (items + 3) / 4 : items;
     DCTR_REQUIRE(items <= INT32_MAX, "attention: too many blocks for one launch");
     if (blocks == 0) return DCTR_OK;
-    const size_t lds = QuerySide<T, DP, FORM>::first + sizeof(float) * ((FORM == SOLO ? 12 : 9) * rel_reach(a) + 8);
+    const size_t lds = QuerySide<T, DP, FORM>::first + sizeof(float) * (4 * SKEW + (FORM == SOLO ? 8 : 5) * rel_reach(a) + 8);
     attn_bwd_q_kernel<T, DP, FORM><<<(unsigned)blocks, BWD_THREADS, lds, st>>>(v, (const T*)x.out, x.out_ld, x.lse, (const T*)x.dout, x.dout_ld, (T*)x.dq, x.dq_ld,
                                                                                delta, part, row_blocks);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
 
-template <typename T, int DP, bool ALONE>
+template <typename T, int DP, int FORM>
 static int launch_kv(const dctr_attention* a, const AttnView& v, const AttnGrads& x, const float* delta, const float* part, hipStream_t st) {
-    using Kd = KeySide<T, DP, ALONE>;
-    const int key_blocks = ceil_div(a->max_k, ALONE ? 32 : 128), sums = part != nullptr ? a->heads : 0;
-    const int64_t items = (int64_t)key_blocks * a->kv_heads * a->n_seg, blocks = ALONE ? (items + 3) / 4 : items;
+    using Kd = KeySide<T, DP, FORM>;
+    const int key_blocks = ceil_div(a->max_k, Kd::OWN ? 32 : 128), sums = part != nullptr ? a->heads : 0;
+    const int64_t items = (int64_t)key_blocks * a->kv_heads * a->n_seg, blocks = FORM == KEY_SOLO ? (items + 3) / 4 : items;
     DCTR_REQUIRE(items + a->heads <= INT32_MAX, "attention: too many blocks for one launch");
     if (blocks + sums == 0) return DCTR_OK;
-    const size_t lds = std::max(Kd::tiles + Kd::stats + sizeof(float) * (ALONE ? 8 : 2) * rel_reach(a), BWD_THREADS * sizeof(float));
-    attn_bwd_kv_kernel<T, DP, ALONE><<<(unsigned)(blocks + sums), BWD_THREADS, lds, st>>>(
+    const size_t lds = std::max(Kd::tiles + Kd::stats + sizeof(float) * (Kd::OWN ? 8 : 2) * rel_reach(a), BWD_THREADS * sizeof(float));
+    attn_bwd_kv_kernel<T, DP, FORM><<<(unsigned)(blocks + sums), BWD_THREADS, lds, st>>>(
         v, x.lse, delta, (const T*)x.dout, x.dout_ld, (T*)x.dk, x.dk_ld, (T*)x.dv, x.dv_ld, key_blocks,
         BiasShares{part, (int64_t)a->n_seg * row_blocks_of(a), x.dbias}, (int)blocks);
     DCTR_LAUNCH_CHECK();
@@ -557,8 +651,10 @@ static int launch_bwd(const dctr_attention* a, const AttnView& v, const AttnGrad
         DCTR_TRY((launch_q<T, DP, wide ? ROWS : SPLIT>(a, v, x, delta, part, st)));
     else
         DCTR_TRY((launch_q<T, DP, wide ? ROWS : SOLO>(a, v, x, delta, part, st)));
-    if (!wide && keys_alone(a)) return launch_kv<T, DP, !wide>(a, v, x, delta, part, st);
-    return launch_kv<T, DP, false>(a, v, x, delta, part, st);
+    const int keys = key_form(a);
+    if (keys == KEY_ROWS || wide) return launch_kv<T, DP, KEY_ROWS>(a, v, x, delta, part, st);
+    if (keys == KEY_SPLIT) return launch_kv<T, DP, wide ? KEY_ROWS : KEY_SPLIT>(a, v, x, delta, part, st);
+    return launch_kv<T, DP, wide ? KEY_ROWS : KEY_SOLO>(a, v, x, delta, part, st);
 }
 
 template <typename T>

@@ -27,10 +27,10 @@ __device__ __forceinline__ void write_rows(const AttnView& a, const Softmax<M, D
 
 constexpr int ROWS_THREADS = 256;
 template <typename T, int DP>
-constexpr int rows_keys = attn_width<T, DP> <= 384 ? 64 : 32;           // keys of a tile
+constexpr int rows_keys = attn_width<T, DP> <= 256 ? 64 : 32;           // keys of a tile
 
 template <typename T, int DP>
-__global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) void attn_rows_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status,
+__global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) void attn_rows_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status,
                                                                                                             int row_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using M = AttnKind<T, DP>;

@@ -354,6 +354,7 @@ struct Direct {
     static constexpr int CHUNKS = Tile<M, DP>::CHUNKS, PER = Tile<M, DP>::PER, N = ROWS * CHUNKS / THREADS;
     static_assert(N >= 1 && ROWS * CHUNKS % THREADS == 0 && THREADS % 64 == 0 && Mma<M>::PLANES == 1, "a wave's load is 64 slots of a tile of one plane");
     __device__ __forceinline__ void fetch(T* tile, const T* base, int64_t ld, int64_t first, int64_t end, int chunks, int tid) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");              // this wave's reads of what the tile held are answered (others': a barrier ago)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int at = tid + i * THREADS, r = at / CHUNKS, c = (at % CHUNKS) ^ Tile<M, DP>::swz(r);
