@@ -90,6 +90,15 @@ __device__ __forceinline__ int bucket_of(const RelBuckets& r, int d) {
 }
 __device__ __forceinline__ int rel_reach(const RelBuckets& r) { return r.n > 1 ? r.edge[r.n - 2] - r.edge[0] + 2 * REL_PAD : 0; }
 
+// The entries of such a table that distances in [dmin, dmax] can ask for: short lists do without the rest.
+struct RelRange { int lo, hi; };
+__device__ __forceinline__ RelRange rel_range(const RelBuckets& r, int64_t dmin, int64_t dmax) {
+    const int reach = rel_reach(r);
+    if (reach == 0) return {0, 0};
+    const int64_t zero = (int64_t)REL_PAD - r.edge[0];
+    return {(int)cut_to(dmin + zero, 0, reach), (int)cut_to(dmax + zero + 1, 0, reach)};
+}
+
 // log2(e) x a head's bias of the two far buckets, read once: a load within the tile loop would wait for the tiles under way
 struct FarBias { float before, behind; };
 __device__ __forceinline__ FarBias far_bias(const AttnView& a, int h) {

@@ -131,6 +131,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     int keys = s.nk;
     if (a.causal) keys = max(0, min(keys, s.start + min(row0 + Q::ITEM_ROWS, s.nq)));
     const int tiles = (keys + Q::KEYS - 1) / Q::KEYS;
+    const RelRange range = rel_range(a.rel, (int64_t)0 - s.start - (row0 + Q::ITEM_ROWS - 1), (int64_t)tiles * Q::KEYS - 1 - s.start - row0);
     const bool busy = wrow < s.nq;
     const int wend = a.causal ? s.start + min(wrow + 32, s.nq) : keys;
 
@@ -205,10 +206,10 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
         meet();
         if (t < last) fetch(t * Q::KEYS, 0);
         if (!second) {                                                  // under the first tile's loads
-            for (int u = FORM == SOLO ? lane : tid; u < reach; u += FORM == SOLO ? 64 : BWD_THREADS)
+            for (int u = range.lo + (FORM == SOLO ? lane : tid); u < range.hi; u += FORM == SOLO ? 64 : BWD_THREADS)
                 lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
             if (part != nullptr)
-                for (int u = FORM == SOLO ? lane : tid; u < (FORM == SOLO ? 1 : 4) * reach; u += FORM == SOLO ? 64 : BWD_THREADS) cells[u] = 0.f;
+                for (int u = range.lo + lane; u < range.hi; u += 64) mine[u] = 0.f;
             if (part != nullptr && reach > 0)
                 for (int u = lane; u < SKEW; u += 64) skew[u] = 0.f;
             if (FORM == SPLIT) __syncthreads();
@@ -313,18 +314,19 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
             far_sum[1] = (fars[4] + fars[5]) + (fars[6] + fars[7]);
         }
         // every distance's cells, then a wave a bucket
-        for (int u = FORM == SOLO ? lane : tid; u < reach; u += FORM == SOLO ? 64 : BWD_THREADS) {
-            float x = cells[u];
+        if (WAYS > 1)
+            for (int u = range.lo + tid; u < range.hi; u += BWD_THREADS) {
+                float x = cells[u];
 #pragma unroll
-            for (int w = 1; w < WAYS; ++w) x += cells[w * reach + u];
-            cells[u] = x;
-        }
+                for (int w = 1; w < WAYS; ++w) x += cells[w * reach + u];
+                cells[u] = x;
+            }
         if (FORM == SOLO) meet(); else __syncthreads();
         for (int u = FORM == SOLO ? 0 : wave; u < a.rel.n; u += FORM == SOLO ? 1 : 4) {
             float x = 0.f;
             if (reach > 0) {
                 const int lo = u == 0 ? 0 : a.rel.edge[u - 1] - a.rel.edge[0] + REL_PAD, hi = u + 1 == a.rel.n ? reach : a.rel.edge[u] - a.rel.edge[0] + REL_PAD;
-                for (int d = lo + lane; d < hi; d += 64) x += cells[d];
+                for (int d = max(lo, range.lo) + lane; d < min(hi, range.hi); d += 64) x += cells[d];
                 x = wave_sum(x);
             }
             if (u == 0) x += far_sum[0];
@@ -430,7 +432,6 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     const int reach = rel_reach(a.rel), first_u = OWN ? lane : tid, step_u = Kd::THREADS;
     float* lut = reinterpret_cast<float*>(lds + Kd::tiles + Kd::stats) + (OWN ? wave * 2 * reach : 0);
     int32_t* buckets = reinterpret_cast<int32_t*>(lut + reach);         // of every distance
-    for (int u = first_u; u < reach; u += step_u) buckets[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u);
     auto meet = [&] {
         if (OWN) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -449,6 +450,8 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     // queries that see one of the block's keys: [first, nq)
     const int first = a.causal ? max(0, key0 - s.start) / QT : 0;
     const int tiles = max(0, (s.nq + QT - 1) / QT - first);
+    const RelRange range = rel_range(a.rel, (int64_t)key0 - s.start - ((int64_t)(first + tiles) * QT - 1), (int64_t)key0 + 127 - s.start - (int64_t)first * QT);
+    for (int u = range.lo + first_u; u < range.hi; u += step_u) buckets[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
     std::conditional_t<BUFS == 2, Loader<M, DP, QT, Kd::THREADS>, Staged<M, DP, QT, Kd::THREADS>> qs, gs;
     float lv = -INFINITY, dv_ = 0.f;                                    // as loaded: nothing waits for them before the tile lands
@@ -475,7 +478,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
         int t = FORM == KEY_SPLIT ? wave : 0;
         meet();
         if (t < tiles) fetch(h, (first + t) * QT, 0);
-        for (int u = first_u; u < reach; u += step_u) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
+        for (int u = range.lo + first_u; u < range.hi; u += step_u) lut[u] = LOG2E * a.bias[buckets[u] * a.heads + h];
         FarBias fars = far_bias(a, h);
         k.wait();
         v.wait();

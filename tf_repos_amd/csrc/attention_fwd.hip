@@ -75,8 +75,8 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) v
         vs.land(vt + buf * TILE, tid, bits);
     };
     if (tiles > 0) fetch(0, 0);
-    const int reach = rel_reach(a.rel);                                 // (under the first tile's loads)
-    for (int u = tid; u < reach; u += ROWS_THREADS) lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
+    const RelRange range = rel_range(a.rel, (int64_t)0 - s.start - (row0 + 127), (int64_t)tiles * ROWS_KEYS - 1 - s.start - row0);      // (under the first loads)
+    for (int u = range.lo + tid; u < range.hi; u += ROWS_THREADS) lut[u] = LOG2E * a.bias[bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * a.heads + h];
     FarBias fars = far_bias(a, h);
     q.wait();
     settle(fars.before);
@@ -237,8 +237,10 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
     float* table = reinterpret_cast<float*>(lut + reach) + (SOLO ? wave * a.rel.n * wide : 0);      // [n_buckets][wide]
     for (int u = SOLO ? lane : tid; u < a.rel.n * wide; u += SOLO ? 64 : 256)
         table[u] = LOG2E * a.bias[u / wide * a.heads + g * a.group + (a.group <= 32 ? u % wide : (r0 + u % wide) % a.group)];
-    if (SOLO ? reach > 0 : near_tile(a.rel, t0 * SPLIT_KEYS - s.start - i1, t1 * SPLIT_KEYS - 1 - s.start - i0))
-        for (int u = tid; u < reach; u += 256) lut[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * wide;
+    // (SOLO's waves fill one table for the whole range)
+    const RelRange range = SOLO ? RelRange{0, reach} : rel_range(a.rel, (int64_t)t0 * SPLIT_KEYS - s.start - i1, (int64_t)t1 * SPLIT_KEYS - 1 - s.start - i0);
+    if (SOLO || near_tile(a.rel, t0 * SPLIT_KEYS - s.start - i1, t1 * SPLIT_KEYS - 1 - s.start - i0))
+        for (int u = range.lo + tid; u < range.hi; u += 256) lut[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u) * wide;
     if (a.rel.n > 0) __syncthreads();
     if (SOLO && none) return;
     for (; t < t1; t += STEP) {
