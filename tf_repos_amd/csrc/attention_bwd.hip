@@ -79,7 +79,9 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     S* vt = kt + Q::BUFS * TILE;
     const int64_t items = (int64_t)row_blocks * a.heads * a.n_seg, at_item = FORM == SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     const int item = (int)min(at_item, items - 1);
-    const int rb = item % row_blocks, h = item / row_blocks % a.heads, b = item / row_blocks / a.heads;
+    // (SOLO: row block slowest, so that a block's waves are alike long)
+    const int rb = FORM == SOLO ? item / a.heads / a.n_seg : item % row_blocks, h = FORM == SOLO ? item % a.heads : item / row_blocks % a.heads;
+    const int b = FORM == SOLO ? item / a.heads % a.n_seg : item / row_blocks / a.heads;
     const Segment s = load_segment(a, b);
     const int row0 = rb * Q::ITEM_ROWS;
     float* share = part != nullptr ? part + ((int64_t)h * a.n_seg * row_blocks + (int64_t)b * row_blocks + rb) * a.rel.n : nullptr;
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
                                acc[k][4 * i + 3] * a.scale);
 }
 
-// One block a head, behind the key side's blocks: thread = (slice of the shares, bucket), slices added in order.
+// One block a head, before the key side's blocks: thread = (slice of the shares, bucket), slices added in order.
 struct BiasShares { const float* part; int64_t shares; float* dbias; };
 __device__ __forceinline__ void sum_shares(const BiasShares& x, int n, int heads, int h, float* red) {
     const int slices = BWD_THREADS / n, u = threadIdx.x % n, sl = threadIdx.x / n;
@@ -405,7 +407,7 @@ struct KeySide {
 template <typename T, int DP, int FORM>
 __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) void attn_bwd_kv_kernel(AttnView a, const float* lse, const float* delta, const T* dout,
                                                                                                    int64_t dout_ld, T* dk, int64_t dk_ld, T* dv, int64_t dv_ld,
-                                                                                                   int key_blocks, BiasShares shares, int blocks) {
+                                                                                                   int key_blocks, BiasShares shares, int sums) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     using Kd = KeySide<T, DP, FORM>;
     using M = AttnKind<T, DP>;
@@ -416,13 +418,16 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     S* qt = reinterpret_cast<S*>(lds) + (OWN ? wave * 2 * BUFS * TILE : 0);
     S* gt = qt + BUFS * TILE;
     float* stats = reinterpret_cast<float*>(lds + Kd::tiles) + (OWN ? wave * BUFS * 2 * QT : 0);  // [buffer][-log2(e) lse, delta][QT]
-    if ((int)blockIdx.x >= blocks) {
-        sum_shares(shares, a.rel.n, a.heads, blockIdx.x - blocks, reinterpret_cast<float*>(lds));
+    if ((int)blockIdx.x < sums) {                                       // (first: behind the others they would be the launch's tail)
+        sum_shares(shares, a.rel.n, a.heads, blockIdx.x, reinterpret_cast<float*>(lds));
         return;
     }
-    const int64_t items = (int64_t)key_blocks * kv_heads * a.n_seg, at_item = FORM == KEY_SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+    const int block = blockIdx.x - sums;
+    const int64_t items = (int64_t)key_blocks * kv_heads * a.n_seg, at_item = FORM == KEY_SOLO ? (int64_t)block * 4 + wave : block;
     if (at_item >= items) return;                                       // (KEY_SOLO has no barriers)
-    const int item = (int)at_item, kb = item % key_blocks, g = item / key_blocks % kv_heads, b = item / key_blocks / kv_heads;
+    const int item = (int)at_item;                                      // (KEY_SOLO: key block slowest)
+    const int kb = FORM == KEY_SOLO ? item / kv_heads / a.n_seg : item % key_blocks, g = FORM == KEY_SOLO ? item % kv_heads : item / key_blocks % kv_heads;
+    const int b = FORM == KEY_SOLO ? item / kv_heads % a.n_seg : item / key_blocks / kv_heads;
     const Segment s = load_segment(a, b);
     const int key0 = kb * (OWN ? 32 : 128);
     if (key0 >= s.nk) return;
@@ -638,7 +643,7 @@ static int launch_kv(const dctr_attention* a, const AttnView& v, const AttnGrads
     const size_t lds = std::max(Kd::tiles + Kd::stats + sizeof(float) * (Kd::OWN ? 8 : 2) * rel_reach(a), BWD_THREADS * sizeof(float));
     attn_bwd_kv_kernel<T, DP, FORM><<<(unsigned)(blocks + sums), BWD_THREADS, lds, st>>>(
         v, x.lse, delta, (const T*)x.dout, x.dout_ld, (T*)x.dk, x.dk_ld, (T*)x.dv, x.dv_ld, key_blocks,
-        BiasShares{part, (int64_t)a->n_seg * row_blocks_of(a), x.dbias}, (int)blocks);
+        BiasShares{part, (int64_t)a->n_seg * row_blocks_of(a), x.dbias}, sums);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }

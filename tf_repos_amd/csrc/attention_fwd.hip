@@ -195,8 +195,11 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
     float* stats = reinterpret_cast<float*>(lds + L::first);
     const int64_t items = (int64_t)cut.row_blocks * kv_heads * a.n_seg, at_item = SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     int rb, g, b, sp = 0, item;
-    if (SOLO || cut.splits == 1) {
+    if (SOLO) {                                                         // (row block slowest: a block's waves are alike long)
         item = (int)min(at_item, items - 1);
+        g = item % kv_heads, b = item / kv_heads % a.n_seg, rb = item / kv_heads / a.n_seg;
+    } else if (cut.splits == 1) {
+        item = (int)at_item;
         rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
     } else {
         rb = blockIdx.x % cut.row_blocks, g = blockIdx.x / cut.row_blocks % kv_heads;
