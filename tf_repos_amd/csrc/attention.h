@@ -107,6 +107,15 @@ __device__ __forceinline__ FarBias far_bias(const AttnView& a, int h) {
     return f;
 }
 
+// Item (segment, head, block of its rows) of a launch whose blocks of rows go slowest: the first of every segment, then the second, ...  Consecutive
+// workgroups go to the eight XCDs in turn; the segments move on by one a round, or a long one among short ones would have all its work on one XCD
+// (16 segments x 2 heads: 441 us against 139).
+struct Item { int head, seg, nth; };
+__device__ __forceinline__ Item item_of(int item, int heads, int n_seg) {
+    const int nth = item / heads / n_seg;
+    return {item % heads, (item / heads % n_seg + nth) % n_seg, nth};
+}
+
 inline int rel_reach(const dctr_attention* a) {         // entries of a table over distances
     return a->n_buckets > 1 ? a->boundaries[a->n_buckets - 2] - a->boundaries[0] + 2 * REL_PAD : 0;
 }

@@ -79,9 +79,9 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     S* vt = kt + Q::BUFS * TILE;
     const int64_t items = (int64_t)row_blocks * a.heads * a.n_seg, at_item = FORM == SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     const int item = (int)min(at_item, items - 1);
-    // (SOLO: row block slowest, so that a block's waves are alike long)
-    const int rb = FORM == SOLO ? item / a.heads / a.n_seg : item % row_blocks, h = FORM == SOLO ? item % a.heads : item / row_blocks % a.heads;
-    const int b = FORM == SOLO ? item / a.heads % a.n_seg : item / row_blocks / a.heads;
+    // Row block slowest.  ROWS, SPLIT: the last first, which a causal mask makes the longest; SOLO: a block's waves are alike long.
+    const Item it = item_of(item, a.heads, a.n_seg);
+    const int h = it.head, b = it.seg, rb = FORM == SOLO ? it.nth : row_blocks - 1 - it.nth;
     const Segment s = load_segment(a, b);
     const int row0 = rb * Q::ITEM_ROWS;
     float* share = part != nullptr ? part + ((int64_t)h * a.n_seg * row_blocks + (int64_t)b * row_blocks + rb) * a.rel.n : nullptr;
@@ -425,9 +425,8 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     const int block = blockIdx.x - sums;
     const int64_t items = (int64_t)key_blocks * kv_heads * a.n_seg, at_item = FORM == KEY_SOLO ? (int64_t)block * 4 + wave : block;
     if (at_item >= items) return;                                       // (KEY_SOLO has no barriers)
-    const int item = (int)at_item;                                      // (KEY_SOLO: key block slowest)
-    const int kb = FORM == KEY_SOLO ? item / kv_heads / a.n_seg : item % key_blocks, g = FORM == KEY_SOLO ? item % kv_heads : item / key_blocks % kv_heads;
-    const int b = FORM == KEY_SOLO ? item / kv_heads % a.n_seg : item / key_blocks / kv_heads;
+    const Item it = item_of((int)at_item, kv_heads, a.n_seg);           // (under a causal mask the first key blocks are the longest)
+    const int g = it.head, b = it.seg, kb = it.nth;
     const Segment s = load_segment(a, b);
     const int key0 = kb * (OWN ? 32 : 128);
     if (key0 >= s.nk) return;

@@ -39,7 +39,9 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) v
     S *kt = reinterpret_cast<S*>(lds), *vt = kt + 2 * TILE;
     float* lut = reinterpret_cast<float*>(vt + 2 * TILE);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int rb = blockIdx.x % row_blocks, h = blockIdx.x / row_blocks % a.heads, b = blockIdx.x / row_blocks / a.heads;
+    // last row blocks of every head first: under a causal mask they are the longest, and each compute unit begins with one of them
+    const Item it = item_of(blockIdx.x, a.heads, a.n_seg);
+    const int h = it.head, b = it.seg, rb = row_blocks - 1 - it.nth;
     const Segment s = load_segment(a, b);
     if (rb == 0 && h == 0 && tid == 0) flag_segment(a, b, status);
     const int row0 = rb * 128;
@@ -197,7 +199,8 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
     int rb, g, b, sp = 0, item;
     if (SOLO) {                                                         // (row block slowest: a block's waves are alike long)
         item = (int)min(at_item, items - 1);
-        g = item % kv_heads, b = item / kv_heads % a.n_seg, rb = item / kv_heads / a.n_seg;
+        const Item it = item_of(item, kv_heads, a.n_seg);
+        g = it.head, b = it.seg, rb = it.nth;
     } else if (cut.splits == 1) {
         item = (int)at_item;
         rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
