@@ -99,6 +99,11 @@ __device__ __forceinline__ RelRange rel_range(const RelBuckets& r, int64_t dmin,
     return {(int)cut_to(dmin + zero, 0, reach), (int)cut_to(dmax + zero + 1, 0, reach)};
 }
 
+// Keys that are not kept, as numbers to add to a tile's scores (0, -inf): one read for four keys and no vector work beyond the fma that is there.
+__device__ __forceinline__ f32x4 hidden4(const float* hidden, int k, int i) {      // rows of registers 4 i .. 4 i + 3 of block k
+    return *reinterpret_cast<const f32x4*>(hidden + 32 * k + 8 * i + 4 * ((threadIdx.x >> 5) & 1));
+}
+
 // log2(e) x a head's bias of the two far buckets, read once: a load within the tile loop would wait for the tiles under way
 struct FarBias { float before, behind; };
 __device__ __forceinline__ FarBias far_bias(const AttnView& a, int h) {

@@ -19,7 +19,7 @@ template <typename T, int DP, int FORM>
 struct QuerySide {
     using M = AttnKind<T, DP>;
     static constexpr int NB = FORM == ROWS && attn_width<T, DP> <= 256 ? 2 : 1, KEYS = 32 * NB, BUFS = FORM == ROWS || sizeof(T) == 2 ? 2 : 1, THREADS = FORM == ROWS ? 256 : 64;
-    static constexpr int TILE = KEYS * Tile<M, DP>::STRIDE, ITEM_ROWS = FORM == ROWS ? 128 : 32;
+    static constexpr int HIDDEN = (FORM == ROWS ? 1 : 4) * BUFS * KEYS, TILE = KEYS * Tile<M, DP>::STRIDE, ITEM_ROWS = FORM == ROWS ? 128 : 32;
     static constexpr size_t tiles = (FORM == ROWS ? 1 : 4) * 2 * BUFS * KEYS * attn_width<T, DP>, join = FORM == SPLIT ? 4 * 32 * (DP + 4) * sizeof(float) : 0;
     static constexpr size_t first = tiles > join ? tiles : join;
 };
@@ -105,8 +105,9 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     const float scale = a.scale * LOG2E;
     const int reach = rel_reach(a.rel);
     // skewed blocks, a wave each; SOLO: every wave's own table and cells; else one table, [4 waves][reach] cells; 2 x 4 far sums
-    float* skew = reinterpret_cast<float*>(lds + Q::first) + wave * SKEW;
-    float* lut = reinterpret_cast<float*>(lds + Q::first) + 4 * SKEW + (FORM == SOLO ? wave * 2 * reach : 0);
+    float* hidden = reinterpret_cast<float*>(lds + Q::first) + (OWN ? wave * Q::BUFS * Q::KEYS : 0);     // [buffer][KEYS]
+    float* skew = reinterpret_cast<float*>(lds + Q::first) + Q::HIDDEN + wave * SKEW;
+    float* lut = reinterpret_cast<float*>(lds + Q::first) + Q::HIDDEN + 4 * SKEW + (FORM == SOLO ? wave * 2 * reach : 0);
     float* cells = lut + reach;
     float* mine = cells + (FORM == SOLO ? 0 : wave * reach);
     const int loader = OWN ? lane : tid;
@@ -150,13 +151,14 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     };
     auto land = [&](int buf) {
         bits = __ballot(kept != 0);
+        if (loader < Q::KEYS) hidden[buf * Q::KEYS + loader] = kept != 0 ? 0.f : -INFINITY;
         ks.land(kt + buf * TILE, loader, bits);
         vs.land(vt + buf * TILE, loader, bits);
     };
     // cell of the distance between a block's first key and the wave's first query
     auto block_cell = [&](int key) { return key - s.start - wrow - a.rel.edge[0] + REL_PAD; };
     // p and dp of the tile at j0; returns whether it is near, `side` its far side otherwise
-    auto pair = [&](const S* kb, const S* vb, int j0, uint64_t now, f32x16 (&p)[NB], f32x16 (&dp)[NB], int& cell, int& side) {
+    auto pair = [&](const S* kb, const S* vb, const float* hide, int j0, uint64_t now, f32x16 (&p)[NB], f32x16 (&dp)[NB], int& cell, int& side) {
         const int d0 = j0 - s.start - wrow;                             // the tile's first key from the wave's first query
         const bool near = near_tile(a.rel, d0 - 31, d0 + 32 * NB - 1);
         const int fb = a.rel.n > 0 && !near ? far_bucket(a.rel, d0 - 31) : 0;
@@ -169,14 +171,13 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
             const int last = row + s.start - j0;
             seen &= last < 0 ? 0ull : last >= 63 ? ~0ull : (2ull << last) - 1;
         }
-        const bool hide = __any((uint32_t)(seen >> (32 * (NB - 1))) != ~0u || (uint32_t)seen != ~0u);
         seen = lane_bits(seen);
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
             p[k] = scores<M, DP, (attn_width<T, DP> > 192)>(kb, 32 * k, q);
             dp[k] = scores<M, DP, (attn_width<T, DP> > 192)>(vb, 32 * k, go);
         }
-        if (near || hide) {
+        if (near || cut) {
 #pragma unroll
             for (int k = 0; k < NB; ++k)
 #pragma unroll
@@ -184,6 +185,16 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
                     const int at = 32 * k + reg_row(r);
                     const float x = fmaf(p[k][r], scale, near ? lut[cell + at] : far) + minus_lse;
                     p[k][r] = (seen >> at & 1) ? __builtin_amdgcn_exp2f(x) : 0.f;
+                }
+        } else if (now != ~0ull >> (64 - Q::KEYS)) {
+            const float off = far + minus_lse;
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 x = hidden4(hide, k, i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) p[k][4 * i + j] = __builtin_amdgcn_exp2f(fmaf(p[k][4 * i + j], scale, x[j]) + off);
                 }
         } else {
             const float off = far + minus_lse;
@@ -232,7 +243,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
                 const S *kb = kt + buf * TILE, *vb = vt + buf * TILE;
                 f32x16 p[NB], dp[NB];
                 int cell, side;
-                const bool near = pair(kb, vb, j0, now, p, dp, cell, side);
+                const bool near = pair(kb, vb, hidden + buf * Q::KEYS, j0, now, p, dp, cell, side);
                 if (!second) {
                     if (ROUNDED || (part != nullptr && !near)) {
                         float x[2] = {0.f, 0.f};
@@ -448,7 +459,6 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     RowFrags<M, DP> k, v;
     k.load((const T*)a.k + (s.k0 + key) * a.k_ld + (int64_t)g * a.dim, chunks, on);
     v.load((const T*)a.v + (s.k0 + key) * a.v_ld + (int64_t)g * a.dim, chunks, on);
-    const bool all_on = __all(on);
     const bool busy = __any(on);
 
     // queries that see one of the block's keys: [first, nq)
@@ -504,7 +514,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
                     const int d0 = wkey - s.start - r0;                 // the wave's first key from the step's first query
                     if (a.causal && d0 - 31 > 0) continue;              // its last query is before the wave's first key
                     const bool near = near_tile(a.rel, d0 - 31, d0 + 31);
-                    const float far = near ? 0.f : far_bucket(a.rel, d0 - 31) > 0 ? fars.behind : fars.before;
+                    const float far = !on ? -INFINITY : near ? 0.f : far_bucket(a.rel, d0 - 31) > 0 ? fars.behind : fars.before;      // a key: a lane
                     const bool cut = a.causal && d0 + 31 > 0;
                     f32x16 p = scores<M, DP, (attn_width<T, DP> > 192)>(qb, 32 * n, k), dp = scores<M, DP>(gb, 32 * n, v);
                     f32x4 ml[4], dl[4];
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
                         ml[i] = *reinterpret_cast<const f32x4*>(st + 32 * n + 8 * i + 4 * half);
                         dl[i] = *reinterpret_cast<const f32x4*>(st + QT + 32 * n + 8 * i + 4 * half);
                     }
-                    if (near || cut || !all_on) {
+                    if (near || cut) {
                         const int from = key - s.start - r0;            // first query of the step that sees the key
                         uint32_t seen = !on ? 0u : !cut || from <= 0 ? ~0u : from > 31 ? 0u : ~0u << from;
                         seen >>= 4 * half;
@@ -625,7 +635,7 @@ static int launch_q(const dctr_attention* a, const AttnView& v, const AttnGrads&
     const int64_t items = (int64_t)row_blocks * a->heads * a->n_seg, blocks = FORM == SOLO ? (items + 3) / 4 : items;
     DCTR_REQUIRE(items <= INT32_MAX, "attention: too many blocks for one launch");
     if (blocks == 0) return DCTR_OK;
-    const size_t lds = QuerySide<T, DP, FORM>::first + sizeof(float) * (4 * SKEW + (FORM == SOLO ? 8 : 5) * rel_reach(a) + 8);
+    const size_t lds = QuerySide<T, DP, FORM>::first + sizeof(float) * (QuerySide<T, DP, FORM>::HIDDEN + 4 * SKEW + (FORM == SOLO ? 8 : 5) * rel_reach(a) + 8);
     attn_bwd_q_kernel<T, DP, FORM><<<(unsigned)blocks, BWD_THREADS, lds, st>>>(v, (const T*)x.out, x.out_ld, x.lse, (const T*)x.dout, x.dout_ld, (T*)x.dq, x.dq_ld,
                                                                                delta, part, row_blocks);
     DCTR_LAUNCH_CHECK();

@@ -37,7 +37,8 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) v
     using S = typename Mma<M>::Store;
     constexpr int ROWS_KEYS = rows_keys<T, DP>, NB = ROWS_KEYS / 32, TILE = ROWS_KEYS * Tile<M, DP>::STRIDE;
     S *kt = reinterpret_cast<S*>(lds), *vt = kt + 2 * TILE;
-    float* lut = reinterpret_cast<float*>(vt + 2 * TILE);
+    float* hidden = reinterpret_cast<float*>(vt + 2 * TILE);            // [buffer][ROWS_KEYS]
+    float* lut = hidden + 2 * ROWS_KEYS;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // last row blocks of every head first: under a causal mask they are the longest, and each compute unit begins with one of them
     const Item it = item_of(blockIdx.x, a.heads, a.n_seg);
@@ -73,6 +74,7 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) v
     };
     auto land = [&](int buf) {
         bits = __ballot(kept != 0);
+        if (tid < ROWS_KEYS) hidden[buf * ROWS_KEYS + tid] = kept != 0 ? 0.f : -INFINITY;
         ks.land(kt + buf * TILE, tid, bits);
         vs.land(vt + buf * TILE, tid, bits);
     };
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) v
             const float far = near ? 0.f : far_bucket(a.rel, d0 - 31) > 0 ? fars.behind : fars.before;
             const bool cut = a.causal && d0 + ROWS_KEYS - 1 > 0;
             float c = scale, add = far;
-            if (near || cut || now != ~0ull >> (64 - ROWS_KEYS)) {
+            if (near || cut) {
                 uint64_t seen = now;
                 if (cut) {
                     const int last = row + s.start - j0;                // last key of the tile that this query sees
@@ -117,6 +119,17 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) v
                     }
                 c = 1.f;
                 add = 0.f;
+            } else if (now != ~0ull >> (64 - ROWS_KEYS)) {
+                const float* hide = hidden + (t & 1) * ROWS_KEYS;
+#pragma unroll
+                for (int k = 0; k < NB; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 x = hidden4(hide, k, i);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sc[k][4 * i + j] = fmaf(sc[k][4 * i + j], scale, x[j]);
+                    }
+                c = 1.f;
             }
             o.template step<NB>(sc, c, add);
             o.template weigh<NB>(vt + (t & 1) * TILE, sc);
@@ -135,7 +148,7 @@ constexpr int SPLIT_KEYS = 32, SPLIT_TILES = 16;                       // keys o
 template <typename T, int DP>
 struct SplitLds {
     static constexpr size_t tiles = 4 * 2 * SPLIT_KEYS * attn_width<T, DP>, join = 4 * 32 * (DP + 4) * sizeof(float);
-    static constexpr size_t first = tiles > join ? tiles : join, stats = 4 * 32 * 2 * sizeof(float);
+    static constexpr size_t first = tiles > join ? tiles : join, stats = 4 * 32 * 2 * sizeof(float);        // statistics, or (while the tiles last) hidden keys
 };
 
 template <typename T, int DP>
@@ -195,6 +208,7 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
     S* kt = reinterpret_cast<S*>(lds) + wave * 2 * TILE;
     S* vt = kt + TILE;
     float* stats = reinterpret_cast<float*>(lds + L::first);
+    float* hidden = stats + wave * 64;                                  // (in the statistics' place)
     const int64_t items = (int64_t)cut.row_blocks * kv_heads * a.n_seg, at_item = SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     int rb, g, b, sp = 0, item;
     if (SOLO) {                                                         // (row block slowest: a block's waves are alike long)
@@ -239,7 +253,7 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
 
     // Bias, under the first loads: bucket of a distance, then its value for the row's head (an item's rows have min(group, 32) different ones).
     const int wide = min(a.group, 32), col = a.group <= 32 ? hg : r - r0, reach = rel_reach(a.rel);
-    int32_t* lut = reinterpret_cast<int32_t*>(stats + (SOLO ? 0 : 4 * 32 * 2));
+    int32_t* lut = reinterpret_cast<int32_t*>(stats + 4 * 32 * 2);
     float* table = reinterpret_cast<float*>(lut + reach) + (SOLO ? wave * a.rel.n * wide : 0);      // [n_buckets][wide]
     for (int u = SOLO ? lane : tid; u < a.rel.n * wide; u += SOLO ? 64 : 256)
         table[u] = LOG2E * a.bias[u / wide * a.heads + g * a.group + (a.group <= 32 ? u % wide : (r0 + u % wide) % a.group)];
@@ -256,6 +270,7 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
         __builtin_amdgcn_wave_barrier();
         ks.land(kt, lane, now);
         vs.land(vt, lane, now);
+        if (lane < SPLIT_KEYS) hidden[lane] = kept != 0 ? 0.f : -INFINITY;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (t + STEP < t1) fetch((t + STEP) * SPLIT_KEYS);
@@ -266,7 +281,7 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
         const float far = a.rel.n > 0 && !near ? table[far_bucket(a.rel, dmin) * wide + col] : 0.f;
         const bool hide = a.causal && dmax > 0;
         float c = scale, add = far;
-        if (near || hide || now != 0xFFFFFFFFull) {
+        if (near || hide) {
             uint64_t seen = now;
             if (hide) {
                 const int last = i + s.start - j0;
@@ -281,6 +296,14 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
             }
             c = 1.f;
             add = 0.f;
+        } else if (now != 0xFFFFFFFFull) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 x = hidden4(hidden, 0, i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sc[0][4 * i + j] = fmaf(sc[0][4 * i + j], scale, x[j]);
+            }
+            c = 1.f;
         }
         o.template step<1>(sc, c, add);
         o.template weigh<1>(vt, sc);
@@ -380,7 +403,7 @@ static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int
         const int row_blocks = ceil_div(a->max_q, 128);
         const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
         DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
-        const size_t lds = 4 * rows_keys<T, DP> * attn_width<T, DP> + rel_reach(a) * sizeof(float);
+        const size_t lds = 4 * rows_keys<T, DP> * attn_width<T, DP> + (2 * rows_keys<T, DP> + rel_reach(a)) * sizeof(float);
         attn_rows_kernel<T, DP><<<(unsigned)blocks, ROWS_THREADS, lds, st>>>(v, (T*)out, out_ld, lse, status, row_blocks);
         DCTR_LAUNCH_CHECK();
         return DCTR_OK;
@@ -390,7 +413,7 @@ static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int
     if (items == 0) return DCTR_OK;
     using L = SplitLds<T, DP>;
     if (cut.solo)
-        attn_split_kernel<T, DP, true><<<ceil_div(items, 4), 256, L::first + lut + 4 * table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
+        attn_split_kernel<T, DP, true><<<ceil_div(items, 4), 256, L::first + L::stats + lut + 4 * table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     else
         attn_split_kernel<T, DP, false><<<(unsigned)(cut.splits > 1 ? items / a->n_seg * cut.chunks : items), 256, L::first + L::stats + lut + table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     DCTR_LAUNCH_CHECK();
