@@ -455,8 +455,8 @@ typedef struct dctr_attention {
  *   d_q_offsets / d_k_offsets int32 [n_seg + 1]; d_q_start int32 [n_seg] or null; d_rel_bias f32 [n_buckets, heads]
  *   d_status int32[2] or null: [0] = 1, [1] = b if segment b's offsets leave the arrays, descend, or hold more than max_q / max_k rows
  *              (or its q_start is beyond +-DCTR_MAX_POSITION): such a segment is cut to what is within
- *   d_workspace: dctr_cross_attention_workspace_bytes(a, backward = 0 / 1) bytes, 16-byte aligned, overwritten; calls that may run at the same
- *              time (streams, captured graphs) need one each.  A handful of queries per segment (serving) splits long histories over blocks. */
+ *   d_workspace: dctr_cross_attention_workspace_bytes(a, backward) bytes (0: the forward's; 1: enough for the forward and the backward), 16-byte
+ *              aligned, overwritten; calls that may run at the same time (streams, captured graphs) need one each.  A handful of queries per segment (serving) splits long histories over blocks. */
 int dctr_cross_attention_workspace_bytes(const dctr_attention* a, int backward, int64_t* bytes);
 int dctr_cross_attention_fwd(const dctr_attention* a, const void* d_q, int q_ld, const void* d_k, int k_ld, const void* d_v, int v_ld,
                              const int32_t* d_q_offsets, const int32_t* d_k_offsets, const int32_t* d_q_start, const uint8_t* d_key_keep,
@@ -477,7 +477,7 @@ int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld,
  * scale = 1/batch for a mean).  d_x [N, D], d_w [V, D] and the gradients in `dtype`, rows 16-byte aligned, D a multiple of 8, 8..256.
  *   fwd: loss, lse and, d_dx not null, dL/dx [N, dx_ld] from the same pass over the table
  *   bwd_weights: dL/dw [V, dw_ld] and (may be null) dL/db f32 [V], overwritten; d_lse: the forward's
- * d_workspace: dctr_vocab_softmax_workspace_bytes(dtype, N, V, D, train) bytes (train = 0: fwd without dx), as above. */
+ * d_workspace: dctr_vocab_softmax_workspace_bytes(dtype, N, V, D, train) bytes (0: fwd without dx; 1: enough for all three), as above. */
 int dctr_vocab_softmax_workspace_bytes(int dtype, int N, int64_t V, int D, int train, int64_t* bytes);
 int dctr_vocab_softmax_fwd(int dtype, const void* d_x, int x_ld, const void* d_w, int w_ld, const float* d_b, const int32_t* d_labels, int N,
                            int64_t V, int D, const float* d_row_scale, float scale, float* d_loss, float* d_lse, void* d_dx, int dx_ld,

@@ -79,6 +79,19 @@ def test_attention_workspaces_refused():
         capi.check(capi.lib().dctr_cross_attention_workspace_bytes(None, 0, C.byref(size)))
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("dim", [16, 64, 96, 128])
+def test_a_training_workspace_covers_the_forward(dtype, dim):
+    for n_seg, max_q, max_k in ((1, 1, 100), (1, 3, 100000), (211, 9, 951), (40, 1, 16384), (512, 40, 200), (8, 2048, 2048)):
+        a = attention(dtype=dtype, n_seg=n_seg, heads=8, kv_heads=8, head_dim=dim, max_q=max_q, max_k=max_k, total_q=n_seg * max_q, total_k=n_seg * max_k)
+        sizes = []
+        for train in (0, 1):
+            size = C.c_int64()
+            capi.check(capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), train, C.byref(size)))
+            sizes.append(size.value)
+        assert sizes[1] >= sizes[0]
+
+
 def vfwd(dtype=0, x=A, x_ld=32, w=A, w_ld=32, labels=A, n=4, v=10, d=32, scale=1.0, loss=A, dx=A, dx_ld=32, ws=A, size=1 << 40):
     return capi.lib().dctr_vocab_softmax_fwd(dtype, x, x_ld, w, w_ld, None, labels, n, v, d, None, scale, loss, None, dx, dx_ld, None, ws, size, None)
 

@@ -63,7 +63,7 @@ static int make_view(const dctr_attention* a, const void* q, int q_ld, const voi
 }
 
 static int64_t workspace_bytes(const dctr_attention* a, int backward) {
-    return backward ? attn_bwd_workspace(a) : attn_fwd_workspace(a);
+    return std::max(attn_fwd_workspace(a), backward ? attn_bwd_workspace(a) : 0);
 }
 
 static int check_workspace(const dctr_attention* a, int backward, const void* ws, size_t bytes) {
