@@ -217,3 +217,25 @@ def test_short_segments_in_number(dtype, heads, kv_heads, dim, causal, dev):
 def test_long_histories_of_uneven_length_among_many(dtype, dev):
     k = [9000 if i == 5 else 3 * i for i in range(40)]
     run(AttentionCase(dtype, [1] * 40, k, 8, 2, 32, boundaries=[-64, -8, 0, 8], q_start=[max(0, n - 1) for n in k], seed=33), dev, ("out", "lse"))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_one_workspace_for_a_training_pass(dtype, dev):
+    """Few queries over long key lists: the forward splits the keys and needs more than the backward."""
+    case = AttentionCase(dtype, [3, 9, 0, 5], [900, 2000, 50, 1], 4, 2, 96, seed=34)
+    d = case.to(dev)
+    d["ws0"], d["bytes0"] = d["ws1"], d["bytes1"]
+    capi.check(case.forward(d))
+    capi.check(case.backward(d))
+    torch.cuda.synchronize()
+    case.check(d, BOTH)
+
+
+def test_bias_gradient_errors_lean_to_no_side(dev):
+    """A bucket's sum over thousands of rows adds up whatever each ds leans to.  Errors without a lean have either sign alike: of n sums (n / 2) +- 4
+    standard deviations (sqrt(n) / 2 each) are below the 64-bit value."""
+    q, k = ragged(35, 300, 40), ragged(36, 300, 200)
+    case = AttentionCase("f32", q, k, 4, 4, 16, boundaries=[-64, -40, -24, -16, -10, -6, -3, 0, 3, 6, 10, 16, 24, 40, 64], seed=35)
+    d = run(case, dev)
+    below = (d["db"].cpu().double() < case.reference()["db"][0]).sum().item()
+    assert abs(below - 32) <= 16, below

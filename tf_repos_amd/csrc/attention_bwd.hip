@@ -112,6 +112,10 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     float* mine = cells + (FORM == SOLO ? 0 : wave * reach);
     const int loader = OWN ? lane : tid;
 
+    // The matrix unit's sums of bf16 products lean to one side by a small part of a half step.  A row's <do, out> does not share that lean, so the bias
+    // gradient would add it up over thousands of rows (relative error 1.8e-6 over 512 segments of 40 x 200 by 4 heads of 16): every other row has its dO
+    // negated and dP's sign turned back, which leaves 3e-7.  (bf16 arrays: delta comes from the same dP, below.)
+    const float sign = ROUNDED || !(lane & 1) ? 1.f : -1.f;
     RowFrags<M, DP> q, go;
     q.load((const T*)a.q + (s.q0 + row) * a.q_ld + (int64_t)h * a.dim, chunks, row < s.nq);
     go.load(dout + (s.q0 + row) * dout_ld + (int64_t)h * a.dim, chunks, row < s.nq);
@@ -122,6 +126,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
 #pragma unroll
         for (int c = 0; c < RowFrags<M, DP>::STEPS; ++c) dl = Mma<M>::product(go.c[c], o.c[c], dl);
         dl = both_sum(dl);
+        if (!ROUNDED && (lane & 1)) go.negate();
         if (row < s.nq) {
             const float L = lse[(s.q0 + row) * a.heads + h];
             if (L != -INFINITY) minus_lse = -LOG2E * L;
@@ -245,7 +250,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
                 int cell, side;
                 const bool near = pair(kb, vb, hidden + buf * Q::KEYS, j0, now, p, dp, cell, side);
                 if (!second) {
-                    if (ROUNDED || (part != nullptr && !near)) {
+                    if (ROUNDED) {
                         float x[2] = {0.f, 0.f};
 #pragma unroll
                         for (int k = 0; k < NB; ++k)
@@ -273,8 +278,18 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
                                 pk[ROUNDED ? d : 0] = Mma<M>::template weigh<DP>(kb, 32 * k, 32 * d, w, pk[ROUNDED ? d : 0]);
                         }
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) p[k][r] *= dp[k][r] - dl;
-                        if (!ROUNDED && part != nullptr && near) add_diagonals(skew, p[k], mine + block_cell(j0 + 32 * k));
+                        for (int r = 0; r < 16; ++r) p[k][r] *= ROUNDED ? dp[k][r] - dl : fmaf(dp[k][r], sign, -dl);
+                        if (!ROUNDED && part != nullptr) {
+                            if (near) {
+                                add_diagonals(skew, p[k], mine + block_cell(j0 + 32 * k));
+                            } else {
+                                float x[2] = {0.f, 0.f};
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) x[r & 1] += p[k][r];
+                                far_ds[0] += side ? 0.f : x[0] + x[1];
+                                far_ds[1] += side ? x[0] + x[1] : 0.f;
+                            }
+                        }
                         const auto w = Mma<M>::pack(p[k]);
 #pragma unroll
                         for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(kb, 32 * k, 32 * d, w, acc[d]);
@@ -283,7 +298,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
 #pragma unroll
                     for (int k = 0; k < NB; ++k) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) p[k][r] *= dp[k][r] - dl;
+                        for (int r = 0; r < 16; ++r) p[k][r] *= ROUNDED ? dp[k][r] - dl : fmaf(dp[k][r], sign, -dl);
                         add_diagonals(skew, p[k], mine + block_cell(j0 + 32 * k));
                     }
                 }
@@ -314,7 +329,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
         if (ROUNDED && a.rel.n > 1) walk(true);                         // the near tiles again, for their distances' sums
         float far_sum[2];
 #pragma unroll
-        for (int side = 0; side < 2; ++side) far_sum[side] = wave_sum(fmaf(-dl, far_p[side], far_ds[side]));
+        for (int side = 0; side < 2; ++side) far_sum[side] = wave_sum(ROUNDED ? fmaf(-dl, far_p[side], far_ds[side]) : far_ds[side]);
         constexpr int WAYS = FORM == SOLO ? 1 : 4;
         float* fars = cells + 4 * reach;                                // (not SOLO's)
         if (FORM != SOLO && lane == 0) {
@@ -387,17 +402,17 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
 struct BiasShares { const float* part; int64_t shares; float* dbias; };
 __device__ __forceinline__ void sum_shares(const BiasShares& x, int n, int heads, int h, float* red) {
     const int slices = BWD_THREADS / n, u = threadIdx.x % n, sl = threadIdx.x / n;
-    float y = 0.f;
+    double y = 0.;                                                      // (thousands of shares)
     if (sl < slices) {
         const float* p = x.part + (int64_t)h * x.shares * n + u;
 #pragma unroll 8
         for (int64_t i = sl; i < x.shares; i += slices) y += p[i * n];
     }
-    red[threadIdx.x] = y;
+    red[threadIdx.x] = (float)y;
     __syncthreads();
     if (sl == 0) {
         for (int w = 1; w < slices; ++w) y += red[w * n + u];
-        x.dbias[u * heads + h] = y;
+        x.dbias[u * heads + h] = (float)y;
     }
 }
 
@@ -604,23 +619,21 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
-#ifndef QUERY_ROWS_FROM
-#define QUERY_ROWS_FROM 0
-#define KEY_ROWS_FROM 200
-#endif
 static int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
-// Which form: a wave to an item where they are many and short; else rows where those blocks fill the chip, or the waves share an item's other side.
+// Which form: a wave to an item where they are many and short; else rows where those blocks fill the chip, or the waves share an item's other side
+// (key side, 16 segments of up to 777 x 1531, 8 heads of 128 over 2: 106 blocks of rows, 194 us against 139; 4 of 1024 x 1024, 8 heads: 288 blocks,
+// a training pass of 176 us against 216).
 // (f32 heads wider than 64 have the rows form only, as bias tables beyond 256 distances between first and last boundary: registers, shared memory.)
 static bool rows_only(const dctr_attention* a) { return (a->dtype == DCTR_TYPE_F32 && a->head_dim > 64) || rel_reach(a) > 512; }
 static int query_form(const dctr_attention* a) {
     if (rows_only(a)) return ROWS;
     if (a->max_q <= 64 && attn_solo(a, (int64_t)ceil_div(a->max_q, 32) * a->heads * a->n_seg)) return SOLO;
-    return a->max_q <= 64 || (a->total_q / 128 + a->n_seg) * a->heads < QUERY_ROWS_FROM ? SPLIT : ROWS;
+    return a->max_q <= 64 || (a->total_q / 128 + a->n_seg) * a->heads < 100 ? SPLIT : ROWS;
 }
 static int key_form(const dctr_attention* a) {
     if (rows_only(a)) return KEY_ROWS;
     if (a->max_q <= 128 && attn_solo(a, (int64_t)ceil_div(a->max_k, 32) * a->kv_heads * a->n_seg)) return KEY_SOLO;
-    return (a->total_k / 128 + a->n_seg) * a->kv_heads < KEY_ROWS_FROM ? KEY_SPLIT : KEY_ROWS;
+    return (a->total_k / 128 + a->n_seg) * a->kv_heads < 200 ? KEY_SPLIT : KEY_ROWS;
 }
 static int row_blocks_of(const dctr_attention* a) { return ceil_div(a->max_q, query_form(a) == ROWS ? 128 : 32); }
 

@@ -377,10 +377,20 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnView a, T* out, int6
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
 static int padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 
+// Row form or the others.  Blocks of 128 rows that are too few for the compute units lose by two to three times to the split form, few rows sooner
+// (4 segments of 96 x 2000, heads of 64: 49 us against 19; of 512 x 2000: 49 against 24; but 1 of 2048 x 2048, 8 heads of 128: 67 against 129).  Where
+// there are enough, sharing the tiles pays from 128 rows on (64 segments of 128 x 300: 16.4 us against 20.4), for bf16 heads wider than 64 from 32 on
+// (96 x 300: 19 against 27; narrower heads: 14..17 both).
+static bool row_form(const dctr_attention* a, int64_t rows) {
+    const int64_t blocks = (a->total_q / 128 + a->n_seg) * a->heads, items = (rows + 31) / 32 * a->kv_heads * a->n_seg;
+    if (blocks < (rows <= 128 ? 256 : 100) && items <= 4096) return false;
+    return rows >= 128 || (rows > 32 && a->dtype == DCTR_TYPE_BF16 && a->head_dim > 64);
+}
+
 AttnSplit attn_split(const dctr_attention* a) {
     const int64_t rows = (int64_t)a->max_q * (a->heads / a->kv_heads);
     AttnSplit c{0, 0, 0, 0, false};
-    if (rows > 128) return c;
+    if (row_form(a, rows)) return c;
     c.row_blocks = (int)((rows + 31) / 32);
     c.splits = 1;
     const int64_t items = (int64_t)c.row_blocks * a->kv_heads * a->n_seg, tiles = (a->max_k + SPLIT_KEYS - 1) / SPLIT_KEYS;
