@@ -49,10 +49,8 @@ __device__ __forceinline__ void add_diagonals(float* skew, const f32x16& x, floa
         for (int j = 0; j < 4; ++j) sum += *reinterpret_cast<const f32x4*>(skew + (4 * group + j) * 48 + 4 * min(quad, 11));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t y = __float_as_uint(sum[e]);
-            const auto z = __builtin_amdgcn_permlane16_swap(y, y, false, false);
-            const uint32_t even = z[0], odd = z[1];
-            sum[e] = both_sum(__uint_as_float(even) + __uint_as_float(odd));
+            const Halves y = row_pair(sum[e]);
+            sum[e] = both_sum(y.lo + y.hi);
         }
         const float mine = group == 0 ? sum[0] : group == 1 ? sum[1] : group == 2 ? sum[2] : sum[3];
         const int c = 4 * quad + group;
@@ -327,39 +325,45 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     }
     if (part != nullptr) {
         if (ROUNDED && a.rel.n > 1) walk(true);                         // the near tiles again, for their distances' sums
+        // the outer buckets: the far tiles' sums and the wave's own cells of the near ones
         float far_sum[2];
 #pragma unroll
-        for (int side = 0; side < 2; ++side) far_sum[side] = wave_sum(ROUNDED ? fmaf(-dl, far_p[side], far_ds[side]) : far_ds[side]);
-        constexpr int WAYS = FORM == SOLO ? 1 : 4;
-        float* fars = cells + 4 * reach;                                // (not SOLO's)
-        if (FORM != SOLO && lane == 0) {
-            fars[wave] = far_sum[0];
-            fars[4 + wave] = far_sum[1];
-        }
-        if (FORM == SOLO) meet(); else __syncthreads();
-        if (FORM != SOLO) {
-            far_sum[0] = (fars[0] + fars[1]) + (fars[2] + fars[3]);
-            far_sum[1] = (fars[4] + fars[5]) + (fars[6] + fars[7]);
-        }
-        // every distance's cells, then a wave a bucket
-        if (WAYS > 1)
-            for (int u = range.lo + tid; u < range.hi; u += BWD_THREADS) {
-                float x = cells[u];
+        for (int side = 0; side < 2; ++side) far_sum[side] = ROUNDED ? fmaf(-dl, far_p[side], far_ds[side]) : far_ds[side];
+        const int inner = REL_PAD, outer = reach - REL_PAD;             // cells [inner, outer) are of the buckets between
+        wave_order();
+        for (int u = range.lo + lane; u < min(range.hi, inner); u += 64) far_sum[0] += mine[u];
+        for (int u = max(range.lo, outer) + lane; u < range.hi; u += 64) far_sum[1] += mine[u];
 #pragma unroll
-                for (int w = 1; w < WAYS; ++w) x += cells[w * reach + u];
-                cells[u] = x;
+        for (int side = 0; side < 2; ++side) far_sum[side] = wave_sum(far_sum[side]);
+        const int lo = max(range.lo, inner), hi = min(range.hi, outer);
+        if (FORM != SOLO) {
+            float* both = cells + 4 * reach;
+            if (lane == 0) {
+                both[wave] = far_sum[0];
+                both[4 + wave] = far_sum[1];
             }
-        if (FORM == SOLO) meet(); else __syncthreads();
-        for (int u = FORM == SOLO ? 0 : wave; u < a.rel.n; u += FORM == SOLO ? 1 : 4) {
+            __syncthreads();
+            far_sum[0] = (both[0] + both[1]) + (both[2] + both[3]);
+            far_sum[1] = (both[4] + both[5]) + (both[6] + both[7]);
+            for (int u = lo + tid; u < hi; u += BWD_THREADS)
+                cells[u] = (cells[u] + cells[reach + u]) + (cells[2 * reach + u] + cells[3 * reach + u]);
+            __syncthreads();
+        }
+        if (FORM == SOLO ? lane == 0 : tid == 0) {
+            share[0] = far_sum[0];
+            if (a.rel.n > 1) share[a.rel.n - 1] = far_sum[1];
+        }
+        // sixteen lanes a bucket
+        for (int u0 = FORM == SOLO ? 1 : 1 + 4 * wave; u0 < a.rel.n - 1; u0 += FORM == SOLO ? 4 : 16) {
+            int edge[5];
+#pragma unroll
+            for (int i = 0; i < 5; ++i) edge[i] = min(a.rel.edge[min(u0 - 1 + i, a.rel.n - 2)] - a.rel.edge[0] + REL_PAD, hi);
+            const int g = lane >> 4;
+            const int from = max(lo, g == 0 ? edge[0] : g == 1 ? edge[1] : g == 2 ? edge[2] : edge[3]), to = g == 0 ? edge[1] : g == 1 ? edge[2] : g == 2 ? edge[3] : edge[4];
             float x = 0.f;
-            if (reach > 0) {
-                const int lo = u == 0 ? 0 : a.rel.edge[u - 1] - a.rel.edge[0] + REL_PAD, hi = u + 1 == a.rel.n ? reach : a.rel.edge[u] - a.rel.edge[0] + REL_PAD;
-                for (int d = max(lo, range.lo) + lane; d < min(hi, range.hi); d += 64) x += cells[d];
-                x = wave_sum(x);
-            }
-            if (u == 0) x += far_sum[0];
-            if (u > 0 && u + 1 == a.rel.n) x += far_sum[1];
-            if (lane == 0) share[u] = x;
+            for (int d = from + (lane & 15); d < to; d += 16) x += cells[d];
+            x = row_sum(x);
+            if ((lane & 15) == 0 && u0 + g < a.rel.n - 1) share[u0 + g] = x;
         }
     }
 

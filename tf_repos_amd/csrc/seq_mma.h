@@ -479,15 +479,32 @@ __device__ __forceinline__ void join_waves(const Softmax<M, DP>& o, float* join,
     }
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+// Sums and maxima over 16 lanes (a DPP row: pairs, quads, mirrored halves) and over a wave; every lane has the result
+template <int CTRL>
+__device__ __forceinline__ float from_lane(float x) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ Halves row_pair(float x) {
+    const uint32_t a = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return {__uint_as_float(lo), __uint_as_float(hi)};
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x += from_lane<0xB1>(x);
+    x += from_lane<0x4E>(x);
+    x += from_lane<0x141>(x);
+    return x + from_lane<0x140>(x);
 }
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+    const Halves h = row_pair(row_sum(x));
+    return both_sum(h.lo + h.hi);
+}
+__device__ __forceinline__ float wave_max(float x) {
+    x = fmaxf(x, from_lane<0xB1>(x));
+    x = fmaxf(x, from_lane<0x4E>(x));
+    x = fmaxf(x, from_lane<0x141>(x));
+    x = fmaxf(x, from_lane<0x140>(x));
+    const Halves h = row_pair(x);
+    return both_max(fmaxf(h.lo, h.hi));
 }
 
 }  // namespace dctr
