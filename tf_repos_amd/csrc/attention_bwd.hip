@@ -147,12 +147,12 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     std::conditional_t<Q::BUFS == 2, Loader<M, DP, Q::KEYS, Q::THREADS>, Staged<M, DP, Q::KEYS, Q::THREADS>> ks, vs;
     uint64_t bits = 0;                                                  // kept keys of the tile
     uint8_t kept = 0;
-    auto fetch = [&](int j0, int buf) {
+    auto fetch = [&](int j0, int buf) __attribute__((always_inline)) {
         ks.fetch(kt + buf * TILE, K, a.k_ld, j0, s.nk, chunks, loader);
         vs.fetch(vt + buf * TILE, V, a.v_ld, j0, s.nk, chunks, loader);
         kept = lane < Q::KEYS && j0 + lane < s.nk ? (a.keep != nullptr ? a.keep[s.k0 + j0 + lane] : 1) : 0;
     };
-    auto land = [&](int buf) {
+    auto land = [&](int buf) __attribute__((always_inline)) {
         bits = __ballot(kept != 0);
         if (loader < Q::KEYS) hidden[buf * Q::KEYS + loader] = kept != 0 ? 0.f : -INFINITY;
         ks.land(kt + buf * TILE, loader, bits);
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
         return near;
     };
     // one walk over the tiles; `second`: only the near ones, for their cells
-    auto walk = [&](bool second) {
+    auto walk = [&](bool second) __attribute__((always_inline)) {
         int t = 0, last = tiles;
         if (second) {                                                   // tiles before and behind these are far for every row of the block
             const int64_t from = (int64_t)a.rel.edge[0] + s.start + row0 - (Q::KEYS - 1);
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     // queries that see one of the block's keys: [first, nq)
     const int first = a.causal ? max(0, key0 - s.start) / QT : 0;
     const int tiles = max(0, (s.nq + QT - 1) / QT - first);
-    const RelRange range = rel_range(a.rel, (int64_t)key0 - s.start - ((int64_t)(first + tiles) * QT - 1), (int64_t)key0 + 127 - s.start - (int64_t)first * QT);
+    const RelRange range = rel_range(a.rel, (int64_t)key0 - s.start - ((int64_t)(first + tiles) * QT - 1), (int64_t)key0 + (OWN ? 31 : 127) - s.start - (int64_t)first * QT);
     for (int u = range.lo + first_u; u < range.hi; u += step_u) buckets[u] = bucket_of(a.rel, a.rel.edge[0] - REL_PAD + u);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
     std::conditional_t<BUFS == 2, Loader<M, DP, QT, Kd::THREADS>, Staged<M, DP, QT, Kd::THREADS>> qs, gs;
