@@ -53,13 +53,22 @@ __device__ __forceinline__ float both_sum(float x) { const Halves h = halves(x);
 __device__ __forceinline__ constexpr int reg_row(int r) { return 8 * (r >> 2) + (r & 3); }      // + 4 * (lane >> 5)
 
 // The lane, for the addresses of a tile's reads.  At the widest rows the compiler would keep every address of the loop in a register of its own
-// and spill the accumulators for them: there it is told nothing, and forms them again a tile (one exclusive or each).
+// and spill the accumulators for them: there it is told nothing, and forms them again a tile, one exclusive or each (flipped; from row, chunk and
+// swizzle anew they were four instructions each, half of all of a wave that shares its SIMD with no other).
 template <int DP>
 __device__ __forceinline__ int tile_lane() {
     int l = threadIdx.x & 63;
     if (DP > 128) asm volatile("" : "+v"(l));
     return l;
 }
+
+// p with some of the bits flipped that its offset in a row of a tile takes (rows of a power of two bytes, the tile at a multiple of it)
+template <typename S>
+__device__ __forceinline__ const S* flipped(const S* p, int bits) {
+    typedef __attribute__((address_space(3))) const S lds_S;
+    return (const S*)(lds_S*)(uintptr_t)((uint32_t)(uintptr_t)(lds_S*)p ^ (uint32_t)bits);
+}
+constexpr int TILE_ALIGN = 1024;                        // of shared memory that holds tiles of rows this wide
 
 struct Split {};
 template <typename M> struct Mma;
@@ -285,10 +294,17 @@ struct RowFrags {
 // For kernels of one wave a SIMD, which nothing else covers: the compiler spares registers there and has each read waited for.
 template <typename M, int DP, bool LEAD = false>
 __device__ __forceinline__ f32x16 scores(const typename Mma<M>::Store* tile, int row0, const RowFrags<M, DP>& held) {
+    static_assert(DP <= 128 || Mma<M>::PLANES == 1, "a row's bytes are a power of two");
     const int l = tile_lane<DP>(), row = row0 + (l & 31), g = l >> 5;
+    const auto* first = tile + Tile<M, DP>::at(row, g);
     f32x16 s = {};
 #pragma unroll
-    for (int k = 0; k < RowFrags<M, DP>::STEPS; ++k) s = Mma<M>::dot(tile + Tile<M, DP>::at(row, 2 * k + g), held.c[k], s, DP);
+    for (int k = 0; k < RowFrags<M, DP>::STEPS; ++k) {
+        if constexpr (DP > 128)
+            s = Mma<M>::dot(flipped(first, 32 * k), held.c[k], s, DP);
+        else
+            s = Mma<M>::dot(tile + Tile<M, DP>::at(row, 2 * k + g), held.c[k], s, DP);
+    }
     if constexpr (LEAD) {
         constexpr int P = Mma<M>::PLANES, PRODUCTS = P == 3 ? 6 : sizeof(typename Mma<M>::Store) == 2 ? 1 : 4;
         constexpr int AHEAD = RowFrags<M, DP>::STEPS < 4 ? RowFrags<M, DP>::STEPS : 4;
@@ -300,6 +316,32 @@ __device__ __forceinline__ f32x16 scores(const typename Mma<M>::Store* tile, int
         }
     }
     return s;
+}
+
+// O of tile rows [row0, row0 + 32) with a block of weights, every column
+template <typename M, int DP>
+__device__ __forceinline__ void weigh_all(const typename Mma<M>::Store* tile, int row0, const typename Mma<M>::Weights& w, f32x16 (&acc)[DP / 32]) {
+    if constexpr (DP > 128 && std::is_same_v<M, __bf16>) {
+        const int l = tile_lane<DP>(), row = row0 + 4 * (l >> 5) + ((l & 15) >> 2);
+        const __bf16* first = tile + Tile<M, DP>::at(row, 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) + 4 * (l & 1);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                bf16x8 a;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {                  // (rows + 8: swz differs in the bit of two chunks)
+                    const __bf16* at = flipped(first, 64 * d + 32 * half) + (16 * s + 8 * half) * Tile<M, DP>::STRIDE;
+                    const bf16x4 b = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a[4 * half + j] = b[j];
+                }
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.w[s], acc[d], 0, 0, 0);
+            }
+    } else {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(tile, row0, 32 * d, w, acc[d]);
+    }
 }
 
 // ROWS rows of an array on their way into a tile, by THREADS threads: fetched into registers while the tile before is in use
@@ -434,9 +476,7 @@ struct Softmax {
     __device__ __forceinline__ void weigh(const typename Mma<M>::Store* tile, const f32x16 (&p)[NB]) {
 #pragma unroll
         for (int k = 0; k < NB; ++k) {
-            const auto w = Mma<M>::pack(p[k]);
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(tile, 32 * k, 32 * d, w, acc[d]);
+            weigh_all<M, DP>(tile, 32 * k, Mma<M>::pack(p[k]), acc);
         }
     }
 };

@@ -42,6 +42,7 @@ struct VocabTile {
     using M = VocabKind<T, DP>;
     static constexpr int WIDTH = Mma<M>::BYTES * DP, ROWS = WIDTH <= 384 ? 64 : 32, NB = ROWS / 32, SIZE = ROWS * Tile<M, DP>::STRIDE;
     static constexpr size_t bytes = (size_t)ROWS * WIDTH;
+    static constexpr bool LEAD = WIDTH == 512;                          // bf16 of 256, a wave a SIMD (rows of 2048 x 100000: 445 us, 430 with; f32 the same)
 };
 
 // Bias and hidden columns (behind the table, the row's label) of a wave's 32 rows' scores against NB * 32 table rows from v0 on; returns the factor
@@ -92,7 +93,7 @@ __device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, 
 // the one after that is on its way.
 template <typename T, int DP, bool DX>
 __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 : 512) ? 2 : 1)) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(TILE_ALIGN))) char lds[];
     using Ti = VocabTile<T, DP>;
     using M = VocabKind<T, DP>;
     using S = typename Mma<M>::Store;
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 :
     f32x16 sc[NB];
     if (AHEAD) {
 #pragma unroll
-        for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(tiles, 32 * k, x);
+        for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP, VocabTile<T, DP>::LEAD>(tiles, 32 * k, x);
     }
     int now = 0;
     for (int64_t v = v0; v < v1; v += Ti::ROWS) {
@@ -142,14 +143,14 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 :
         if (busy) {
             if (!AHEAD) {
 #pragma unroll
-                for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP>(tiles + now * Ti::SIZE, 32 * k, x);
+                for (int k = 0; k < NB; ++k) sc[k] = scores<M, DP, VocabTile<T, DP>::LEAD>(tiles + now * Ti::SIZE, 32 * k, x);
             }
             const float c = adjust<NB>(sc, a.b != nullptr ? bias + now * Ti::ROWS : nullptr, v, v1, label);
             const float off = o.template raise<NB>(sc, c, 0.f);
             f32x16 ahead[NB];
             if (AHEAD) {
 #pragma unroll
-                for (int k = 0; k < NB; ++k) ahead[k] = scores<M, DP>(tiles + next * Ti::SIZE, 32 * k, x);
+                for (int k = 0; k < NB; ++k) ahead[k] = scores<M, DP, VocabTile<T, DP>::LEAD>(tiles + next * Ti::SIZE, 32 * k, x);
             }
             o.template weights<NB>(sc, c, off);
             if (DX) o.template weigh<NB>(tiles + now * Ti::SIZE, sc);
@@ -174,7 +175,7 @@ struct FewLds {
 };
 template <typename T, int DP, bool DX>
 __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1)) void vocab_few_kernel(VocabView a, VocabParts p) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(TILE_ALIGN))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sp = blockIdx.x;
     using M = VocabKind<T, DP>;
     using S = typename Mma<M>::Store;
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (v + 128 < v1) fetch(v + 128);
-        f32x16 sc[1] = {scores<M, DP>(tile, 0, x)};
+        f32x16 sc[1] = {scores<M, DP, VocabTile<T, DP>::LEAD>(tile, 0, x)};
         const float c = adjust<1>(sc, a.b != nullptr ? bias : nullptr, v, v1, label);
         o.template step<1>(sc, c, 0.f);
         if (DX) o.template weigh<1>(tile, sc);
@@ -287,10 +288,11 @@ __global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, Voc
 
 // ---- dw, db: 32 table rows a wave, over the rows of x ---------------------------------------------------------------------------------
 // With more than one split (a short vocabulary): part [splits][V][DP], part_b [splits][V], joined by vocab_dw_join_kernel.
+// (bf16 of 256: two waves a SIMD at the price of 13 spilled registers, 2048 x 100000: 510 us -> 370; the rows kernel would spill 110: 430 -> 514)
 template <typename T, int DP>
-__global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1)) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
+__global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 || VocabTile<T, DP>::WIDTH == 512 ? 2 : 1)) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
                                                               int splits, int each, int table_blocks) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    extern __shared__ __attribute__((aligned(TILE_ALIGN))) char lds[];
     using Ti = VocabTile<T, DP>;
     using M = VocabKind<T, DP>;
     using S = typename Mma<M>::Store;
@@ -370,9 +372,7 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1
                 for (int r = 0; r < 16; ++r) part4[r & 3] += p[r];
                 sum += (part4[0] + part4[1]) + (part4[2] + part4[3]);
             }
-            const auto g = Mma<M>::pack(p);
-#pragma unroll
-            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(xt, 32 * k, 32 * d, g, acc[d]);
+            weigh_all<M, DP>(xt, 32 * k, Mma<M>::pack(p), acc);
         }
         if (more) land(buf ^ 1);
         __syncthreads();
