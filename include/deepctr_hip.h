@@ -439,7 +439,7 @@ typedef struct dctr_attention {
     int32_t n_seg;                     /* examples: segment b = rows [q_offsets[b], q_offsets[b+1]) x [k_offsets[b], k_offsets[b+1]) */
     int32_t heads, kv_heads;           /* query head h reads key head h / (heads / kv_heads)                                  */
     int32_t head_dim;                  /* a multiple of 8, 8..128; head h of a row is columns [h*head_dim, (h+1)*head_dim)     */
-    int32_t max_q, max_k;              /* no segment has more rows (the launches are sized by them)                           */
+    int32_t max_q, max_k;              /* no segment has more rows (the launches are sized by them); at most DCTR_MAX_POSITION  */
     int32_t causal;                    /* 1: a query sees the keys at positions <= its own only                               */
     int64_t total_q, total_k;          /* rows of the q / k, v arrays: offsets stay within them                               */
     float   scale;                     /* of the scores, e.g. 1/sqrt(head_dim)                                                */

@@ -79,6 +79,14 @@ def test_attention_workspaces_refused():
         capi.check(capi.lib().dctr_cross_attention_workspace_bytes(None, 0, C.byref(size)))
 
 
+@pytest.mark.parametrize("other", [dict(max_k=(1 << 28) + 1, total_k=1 << 30), dict(max_q=(1 << 28) + 1, total_q=1 << 30)])
+def test_attention_segments_beyond_the_positions_refused(other):
+    with pytest.raises(errors.InvalidArgumentError, match="at most"):
+        capi.check(fwd(attention(**other)))
+    with pytest.raises(errors.InvalidArgumentError, match="at most"):
+        capi.check(bwd(attention(**other)))
+
+
 @pytest.mark.parametrize("dtype", [0, 1])
 @pytest.mark.parametrize("dim", [16, 64, 96, 128])
 def test_a_training_workspace_covers_the_forward(dtype, dim):

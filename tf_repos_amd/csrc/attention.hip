@@ -21,6 +21,8 @@ static int check_attention(const dctr_attention* a) {
     DCTR_REQUIRE(a->dtype == DCTR_TYPE_F32 || a->dtype == DCTR_TYPE_BF16, "attention: unknown element type %d", a->dtype);
     DCTR_REQUIRE(a->n_seg >= 0 && a->max_q >= 0 && a->max_k >= 0 && a->total_q >= 0 && a->total_k >= 0, "attention: negative size");
     DCTR_REQUIRE(a->total_q <= INT32_MAX && a->total_k <= INT32_MAX, "attention: more rows than int32 offsets reach");
+    DCTR_REQUIRE(a->max_q <= DCTR_MAX_POSITION && a->max_k <= DCTR_MAX_POSITION, "attention: segments of %d x %d rows (at most %d)", a->max_q, a->max_k,
+                 DCTR_MAX_POSITION);                                    // (so that differences of positions and boundaries stay within 32 bits)
     DCTR_REQUIRE(a->heads >= 1 && a->heads <= 1024 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0,
                  "attention: %d heads (1..1024) over %d key heads (must divide them)", a->heads, a->kv_heads);
     DCTR_REQUIRE(a->head_dim >= 8 && a->head_dim <= 128 && a->head_dim % 8 == 0, "attention: head_dim %d (a multiple of 8, 8..128)", a->head_dim);
