@@ -472,7 +472,7 @@ int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld,
                              void* d_workspace, size_t workspace_bytes, void* stream);
 /* Softmax cross entropy of N rows against a vocabulary's table, without the [N, V] logits: z = x w^T + b (d_b f32 [V] or null),
  *     d_loss[n] = lse_n - z[n, label_n]      d_lse[n] = log sum_v exp(z_nv) (may be null)
- * d_labels int32 [N]; a negative label = a row without one: loss 0, no gradient; one >= V is treated the same and flagged in d_status
+ * N <= 2^30, V < 2^31.  d_labels int32 [N]; a negative label = a row without one: loss 0, no gradient; one >= V is treated the same and flagged in d_status
  * (int32[2] or null: [0] = 1, [1] = the label).  Gradients are of  sum_n scale * d_row_scale[n] * loss_n  (d_row_scale f32 [N] or null = 1;
  * scale = 1/batch for a mean).  d_x [N, D], d_w [V, D] and the gradients in `dtype`, rows 16-byte aligned, D a multiple of 8, 8..256.
  *   fwd: loss, lse and, d_dx not null, dL/dx [N, dx_ld] from the same pass over the table

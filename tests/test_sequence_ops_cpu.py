@@ -117,6 +117,12 @@ def test_vocab_softmax_arguments_refused(other):
         capi.check(vbwd(**other))
 
 
+def test_vocab_softmax_rows_beyond_32_bits_refused():
+    for call in (vfwd, vbwd):
+        with pytest.raises(errors.InvalidArgumentError, match="rows"):
+            capi.check(call(n=(1 << 30) + 1))
+
+
 @pytest.mark.parametrize("call,other", [(vfwd, dict(loss=None)), (vfwd, dict(dx_ld=8)), (vfwd, dict(dx=A + 4)), (vbwd, dict(lse=None)), (vbwd, dict(dw=None)),
                                         (vbwd, dict(dw_ld=31))])
 def test_vocab_softmax_outputs_refused(call, other):

@@ -509,7 +509,7 @@ static int fwd(const VocabView& a, float* loss, float* lse, void* dx, int64_t dx
 
 static int check_sizes(int dtype, int N, int64_t V, int D) {
     DCTR_REQUIRE(dtype == DCTR_TYPE_F32 || dtype == DCTR_TYPE_BF16, "vocab softmax: unknown element type %d", dtype);
-    DCTR_REQUIRE(N >= 0, "vocab softmax: %d rows", N);
+    DCTR_REQUIRE(N >= 0 && N <= 1 << 30, "vocab softmax: %d rows (0..2^30)", N);              // (row numbers and the tile behind the last stay in 32 bits)
     DCTR_REQUIRE(V >= 1 && V <= INT32_MAX, "vocab softmax: vocabulary of %lld (1..2^31-1)", (long long)V);
     DCTR_REQUIRE(D >= 8 && D <= 256 && D % 8 == 0, "vocab softmax: width %d (a multiple of 8, 8..256)", D);
     return DCTR_OK;
