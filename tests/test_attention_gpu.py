@@ -1,5 +1,6 @@
 """Ragged cross attention with a bucketed relative bias (dctr_cross_attention_fwd / _bwd) against its definition in 64 bits.  Bounds come from
 the arithmetic (tests/seq_util.py): f32 rounding of each score, exponent and sum, and for bf16 the rounding of the matrix operands and outputs."""
+import ctypes as C
 import math
 
 import pytest
@@ -239,3 +240,35 @@ def test_bias_gradient_errors_lean_to_no_side(dev):
     d = run(case, dev)
     below = (d["db"].cpu().double() < case.reference()["db"][0]).sum().item()
     assert abs(below - 32) <= 16, below
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("q,k", [([3, 40], [70, 33]), ([1, 1], [900, 5])])
+def test_rows_at_offsets_beyond_32_bits(dtype, q, k, dev):
+    """The segments are the last rows of arrays of more than 2^31 elements."""
+    case = AttentionCase(dtype, q, k, 2, 1, 32, boundaries=[-4, 0, 4], seed=37)
+    d = case.to(dev)
+    ld, total = 4096, (1 << 31) // 4096 + 2000
+    small = {n: d[n] for n in ("q", "do", "out", "dq", "k", "v", "dk", "dv")}
+    base = {n: total - x.shape[0] for n, x in small.items()}
+    for n, x in small.items():
+        whole = torch.empty(total, ld, dtype=x.dtype, device=dev)
+        whole[base[n]:, :x.shape[1]] = x
+        d[n] = whole
+    d["qo"], d["ko"] = d["qo"] + base["q"], d["ko"] + base["k"]
+    lse = torch.full((total, case.heads), 7.0, device=dev)
+    d["lse"] = lse
+    case.q_ld = case.k_ld = case.v_ld = ld
+    a = case.describe(total_q=total, total_k=total)
+    size = C.c_int64()
+    capi.check(capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), 1, C.byref(size)))
+    d["ws0"] = d["ws1"] = torch.full((size.value + 64,), 255, dtype=torch.uint8, device=dev)
+    d["bytes0"] = d["bytes1"] = size.value
+    capi.check(case.forward(d, a))
+    capi.check(case.backward(d, a))
+    torch.cuda.synchronize()
+    assert d["status"].tolist() == [0, 0]
+    for n, x in small.items():
+        d[n] = d[n][base[n]:, :x.shape[1]].clone()
+    d["lse"] = lse[base["q"]:]
+    case.check(d, BOTH)

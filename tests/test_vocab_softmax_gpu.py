@@ -186,3 +186,24 @@ def test_next_item_step(dtype, dev):
         want = want.detach()
         off = (got.detach().cpu().double() - want).norm() / want.norm()
         assert off <= most, float(off)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [5, 40])
+def test_a_table_beyond_32_bits(dtype, rows, dev):
+    """Rows of 8 at a stride of 4096: more than 2^31 elements between the first and the last."""
+    ld, vocab = 4096, (1 << 31) // 4096 + 3000
+    case = VocabCase(dtype, rows, vocab, 8, seed=40)
+    case.labels[:3] = torch.tensor([vocab - 1, vocab - 2, 0])
+    d = case.to(dev)
+    w = torch.empty(vocab, ld, dtype=d["w"].dtype, device=dev)
+    w[:, :8] = d["w"]
+    dw = torch.empty_like(w)
+    p, t, st = capi.ptr, capi.DTYPES[dtype], capi.current_stream()
+    ins = (t, p(d["x"]), 8, p(w), ld, p(d["b"]), p(d["labels"]), rows, vocab, 8, None, case.scale)
+    capi.check(capi.lib().dctr_vocab_softmax_fwd(*ins, p(d["loss"]), p(d["lse"]), p(d["dx"]), 8, p(d["status"]), p(d["ws1"]), d["bytes1"], st))
+    capi.check(capi.lib().dctr_vocab_softmax_bwd_weights(*ins, p(d["lse"]), p(dw), ld, p(d["db"]), p(d["ws1"]), d["bytes1"], st))
+    torch.cuda.synchronize()
+    assert d["status"].tolist() == [0, 0]
+    d["dw"] = dw[:, :8].clone()
+    case.check(d, ALL)
