@@ -463,8 +463,8 @@ int dctr_cross_attention_fwd(const dctr_attention* a, const void* d_q, int q_ld,
                              const float* d_rel_bias, void* d_out, int out_ld, float* d_lse, int32_t* d_status,
                              void* d_workspace, size_t workspace_bytes, void* stream);
 /* gradients of the same call: d_dout = dL/dout in; dL/dq, dL/dk, dL/dv (shared key heads: summed over their query heads) and dL/d rel_bias
- * [n_buckets, heads] f32 (null: not wanted) overwritten -- 0 where nothing contributes.  d_out, d_lse: the forward's.  Sums
- * run in a fixed order: the same call gives the same bits. */
+ * [n_buckets, heads] f32 (null: not wanted) overwritten -- 0 where nothing contributes.  d_out, d_lse: the forward's.  d_dout has
+ * to be finite in every row of a segment, also where the query saw no key.  Sums run in a fixed order: the same call gives the same bits. */
 int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld, const void* d_k, int k_ld, const void* d_v, int v_ld,
                              const int32_t* d_q_offsets, const int32_t* d_k_offsets, const int32_t* d_q_start, const uint8_t* d_key_keep,
                              const float* d_rel_bias, const void* d_out, int out_ld, const float* d_lse, const void* d_dout,
