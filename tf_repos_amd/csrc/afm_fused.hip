@@ -296,10 +296,10 @@ int afm_att_bwd(const float* pp, const float* W, const float* ba, const float* w
                 int64_t dbo_stride, int n_slabs, hipStream_t st) {
     DCTR_REQUIRE(afm_fused_supported(K, A), "fused AFM attention backward: K=%d / A=%d unsupported", K, A);
     // the slabs are accumulated with atomics: clear them first
-    DCTR_HIP_CHECK(hipMemsetAsync(dW_part, 0, sizeof(float) * ((size_t)(n_slabs - 1) * dW_stride + (size_t)K * A), st));
-    DCTR_HIP_CHECK(hipMemsetAsync(dba_part, 0, sizeof(float) * ((size_t)(n_slabs - 1) * dba_stride + A), st));
-    DCTR_HIP_CHECK(hipMemsetAsync(dwo_part, 0, sizeof(float) * ((size_t)(n_slabs - 1) * dwo_stride + A), st));
-    DCTR_HIP_CHECK(hipMemsetAsync(dbo_part, 0, sizeof(float) * ((size_t)(n_slabs - 1) * dbo_stride + 1), st));
+    DCTR_TRY(zero_words(dW_part, ((size_t)(n_slabs - 1) * dW_stride + (size_t)K * A), st));
+    DCTR_TRY(zero_words(dba_part, ((size_t)(n_slabs - 1) * dba_stride + A), st));
+    DCTR_TRY(zero_words(dwo_part, ((size_t)(n_slabs - 1) * dwo_stride + A), st));
+    DCTR_TRY(zero_words(dbo_part, ((size_t)(n_slabs - 1) * dbo_stride + 1), st));
     if (rows <= 0) return DCTR_OK;
     const int nch = (A + 31) / 32;
     const int NCH = nch <= 1 ? 1 : (nch <= 2 ? 2 : (nch <= 4 ? 4 : 8));

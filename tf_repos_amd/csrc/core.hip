@@ -1,5 +1,6 @@
 // Library-level entry points: error string, device selection, raw memory helpers.
 #include "common.h"
+#include "ops.h"
 
 namespace dctr {
 static thread_local char g_err[1024] = "";
@@ -25,6 +26,16 @@ void set_error(const char* fmt, ...) {
     va_end(ap);
 }
 const char* get_error() { return g_err; }
+
+__global__ __launch_bounds__(256) void zero_words_kernel(uint32_t* p, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0u;
+}
+int zero_words(void* p, size_t n, hipStream_t st) {
+    if (n == 0) return DCTR_OK;
+    zero_words_kernel<<<(unsigned)((n + 255) / 256 < 2048 ? (n + 255) / 256 : 2048), 256, 0, st>>>(static_cast<uint32_t*>(p), n);
+    DCTR_LAUNCH_CHECK();
+    return DCTR_OK;
+}
 }  // namespace dctr
 
 using namespace dctr;

@@ -933,7 +933,7 @@ int group_ids(Group* g, const int32_t* ids, int B, int F, hipStream_t st, bool z
         DCTR_LAUNCH_CHECK();
         return DCTR_OK;
     }
-    if (g->slots_clean) DCTR_HIP_CHECK(hipMemsetAsync(g->counters, 0, 32, st));
+    if (g->slots_clean) DCTR_TRY(zero_words(g->counters, 8, st));
     else group_reset_kernel<<<ceil_div(g->max_entries, 256), 256, 0, st>>>(g->slot, g->uniq, g->counters, (int)g->max_entries);
     if (n <= 0) { DCTR_LAUNCH_CHECK(); return DCTR_OK; }
     g->slots_clean = false;
@@ -951,7 +951,7 @@ int group_ids(Group* g, const int32_t* ids, int B, int F, hipStream_t st, bool z
     //  scatter has written the rows since)
     if (!zero_gemb) {
         if (!g->gemb_clean) {       // a plain scatter has written compact rows since: zero them all once, the fused path keeps them so
-            DCTR_HIP_CHECK(hipMemsetAsync(g->gemb, 0, (size_t)g->max_entries * g->K * 4, st));
+            DCTR_TRY(zero_words(g->gemb, (size_t)g->max_entries * g->K, st));
             g->gemb_clean = true;
         }
     } else { switch (KQ) {
@@ -1052,7 +1052,7 @@ int dctr_embed_scatter_apply(dctr_group_t g, int kind, const float* hyper, float
     }
     hipStream_t st = as_stream(stream);
     if (!G->gemb_clean) {           // a plain dctr_embed_scatter_bwd has used the compact rows since: the fused launch needs them zero
-        DCTR_HIP_CHECK(hipMemsetAsync(G->gemb, 0, (size_t)G->max_entries * G->K * 4, st));
+        DCTR_TRY(zero_words(G->gemb, (size_t)G->max_entries * G->K, st));
         G->gemb_clean = true;
     }
     return embed_scatter_apply(G, kind, nullptr, h, d_emb, d_emb_s0, d_emb_s1, d_lin, d_lin_s0, d_lin_s1, l2, d_sumsq,

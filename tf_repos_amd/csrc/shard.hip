@@ -188,7 +188,7 @@ int dctr_route_unique(dctr_group_t g, int world, int32_t* d_send_rows, int32_t* 
     Group* p = reinterpret_cast<Group*>(g);
     hipStream_t st = as_stream(stream);
     // d_counts: int32[2*world] = counts then cursors
-    DCTR_HIP_CHECK(hipMemsetAsync(d_counts, 0, sizeof(int32_t) * 2 * world, st));
+    DCTR_TRY(zero_words(d_counts, (size_t)2 * world, st));
     const int nb = ceil_div(p->max_entries, 256);
     route_count_kernel<<<nb, 256, 0, st>>>(p->uniq, p->counters, world, d_counts);
     route_fill_kernel<<<nb, 256, 0, st>>>(p->uniq, p->counters, world, d_counts, d_counts + world, d_send_rows, d_upos);
