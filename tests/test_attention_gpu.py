@@ -272,3 +272,10 @@ def test_rows_at_offsets_beyond_32_bits(dtype, q, k, dev):
         d[n] = d[n][base[n]:, :x.shape[1]].clone()
     d["lse"] = lse[base["q"]:]
     case.check(d, BOTH)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("boundaries", [list(range(-63, 64)), [8 * i - 504 for i in range(127)]])
+@pytest.mark.parametrize("q,k", [([130, 300, 7], [260, 300, 90]), ([20, 64, 1], [700, 64, 3]), ([30] * 300, [40] * 300)])
+def test_as_many_buckets_as_there_can_be(dtype, boundaries, q, k, dev):
+    run(AttentionCase(dtype, q, k, 4, 4, 16, causal=False, boundaries=boundaries, q_start=[max(0, m - n) for n, m in zip(q, k)], seed=41), dev)
