@@ -62,7 +62,7 @@ __device__ __forceinline__ int tile_lane() {
     return l;
 }
 
-// p with some of the bits flipped that its offset in a row of a tile takes (a plane's bytes of a row are a power of two, the tile stands at a multiple of it)
+// p with some of the bits flipped that its offset in a row of a tile takes (rows of a power of two bytes, the tile at a multiple of it)
 template <typename S>
 __device__ __forceinline__ const S* flipped(const S* p, int bits) {
     typedef __attribute__((address_space(3))) const S lds_S;
@@ -294,6 +294,7 @@ struct RowFrags {
 // For kernels of one wave a SIMD, which nothing else covers: the compiler spares registers there and has each read waited for.
 template <typename M, int DP, bool LEAD = false>
 __device__ __forceinline__ f32x16 scores(const typename Mma<M>::Store* tile, int row0, const RowFrags<M, DP>& held) {
+    static_assert(DP <= 128 || Mma<M>::PLANES == 1, "a row's bytes are a power of two");
     const int l = tile_lane<DP>(), row = row0 + (l & 31), g = l >> 5;
     const auto* first = tile + Tile<M, DP>::at(row, g);
     f32x16 s = {};
@@ -320,27 +321,22 @@ __device__ __forceinline__ f32x16 scores(const typename Mma<M>::Store* tile, int
 // O of tile rows [row0, row0 + 32) with a block of weights, every column
 template <typename M, int DP>
 __device__ __forceinline__ void weigh_all(const typename Mma<M>::Store* tile, int row0, const typename Mma<M>::Weights& w, f32x16 (&acc)[DP / 32]) {
-    if constexpr (DP > 128 && sizeof(typename Mma<M>::Store) == 2) {
+    if constexpr (DP > 128 && std::is_same_v<M, __bf16>) {
         const int l = tile_lane<DP>(), row = row0 + 4 * (l >> 5) + ((l & 15) >> 2);
         const __bf16* first = tile + Tile<M, DP>::at(row, 2 * ((l >> 4) & 1) + ((l & 3) >> 1)) + 4 * (l & 1);
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                bf16x8 a[Mma<M>::PLANES];
+                bf16x8 a;
 #pragma unroll
-                for (int half = 0; half < 2; ++half)                    // (rows + 8: swz differs in the bit of two chunks)
+                for (int half = 0; half < 2; ++half) {                  // (rows + 8: swz differs in the bit of two chunks)
+                    const __bf16* at = flipped(first, 64 * d + 32 * half) + (16 * s + 8 * half) * Tile<M, DP>::STRIDE;
+                    const bf16x4 b = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
 #pragma unroll
-                    for (int plane = 0; plane < Mma<M>::PLANES; ++plane) {
-                        const __bf16* at = flipped(first, 64 * d + 32 * half) + (16 * s + 8 * half) * Tile<M, DP>::STRIDE + plane * DP;
-                        const bf16x4 b = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) a[plane][4 * half + j] = b[j];
-                    }
-                if constexpr (Mma<M>::PLANES == 3)
-                    acc[d] = six(Planes{a[0], a[1], a[2]}, w.w[s], acc[d]);
-                else
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], w.w[s], acc[d], 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) a[4 * half + j] = b[j];
+                }
+                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.w[s], acc[d], 0, 0, 0);
             }
     } else {
 #pragma unroll

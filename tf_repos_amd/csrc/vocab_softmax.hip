@@ -33,11 +33,9 @@ struct VocabParts {
     int64_t each;                   // vocabulary rows of a split, a multiple of the tile
 };
 
-// Operand kind: float arrays in planes (seq_mma.h); the form for few rows, whose waves have tiles of their own, up to 128 wide (shared memory).
+// Operand kind: float arrays in planes (seq_mma.h) up to 128 wide, beyond that the planes of 32 rows and their accumulators pass the registers.
 template <typename T, int DP>
-using VocabKind = std::conditional_t<std::is_same_v<T, float>, Split, T>;
-template <typename T, int DP>
-using FewKind = std::conditional_t<std::is_same_v<T, float> && DP <= 128, Split, T>;
+using VocabKind = std::conditional_t<std::is_same_v<T, float> && DP <= 128, Split, T>;
 
 template <typename T, int DP>
 struct VocabTile {
@@ -93,7 +91,7 @@ __device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, 
 
 // 4 waves of 32 rows share the table's tiles, three buffers: while a tile is weighed, the scores of the next one are formed under its exponents and
 // the one after that is on its way.  Bound by the matrix unit and the exponents beside it: bf16 2048 x 1000000 x 64 with dx 749 us (700 TF/s of its two
-// products), 2048 x 100000 x 256 360 us (583: one wave a SIMD); f32 in planes 777 x 50021 x 200 365 us (the f32 instructions 623); f32 in planes 4096 x 117581 x 64 without dx, the whole call: 373 us (165 TF/s; a large
+// products), 2048 x 100000 x 256 430 us (490: one wave a SIMD); f32 in planes 4096 x 117581 x 64 without dx, the whole call: 373 us (165 TF/s; a large
 // f32 matrix product of the library runs at 154).
 template <typename T, int DP, bool DX>
 __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 : 512) ? 2 : 1)) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
@@ -103,7 +101,7 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 :
     using S = typename Mma<M>::Store;
     constexpr int NB = Ti::NB;
     // (not where a second step's scores are what takes the kernel past two waves a SIMD: bf16 of 128, 213 us against 166 at 1024 x 100000)
-    constexpr bool AHEAD = !(DX && (Ti::WIDTH == 256 || Ti::WIDTH == 1536));
+    constexpr bool AHEAD = !(DX && Ti::WIDTH == 256);
     S* tiles = reinterpret_cast<S*>(lds);
     float* bias = reinterpret_cast<float*>(tiles + 3 * Ti::SIZE);                       // [3][ROWS]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -173,17 +171,15 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 :
 
 // Up to 32 rows: every wave takes tiles of its own, the four join before they leave their part.
 template <typename T, int DP>
-constexpr int few_width = Mma<FewKind<T, DP>>::BYTES * DP;
-template <typename T, int DP>
 struct FewLds {
-    static constexpr size_t tiles = 4 * 32 * (size_t)few_width<T, DP>, join = 4 * 32 * (DP + 4) * sizeof(float), first = tiles > join ? tiles : join;
+    static constexpr size_t tiles = 4 * 32 * (size_t)VocabTile<T, DP>::WIDTH, join = 4 * 32 * (DP + 4) * sizeof(float), first = tiles > join ? tiles : join;
     static constexpr size_t all = first + 4 * 32 * 2 * sizeof(float) + 4 * 32 * sizeof(float);      // + statistics + bias
 };
 template <typename T, int DP, bool DX>
-__global__ __launch_bounds__(VS_THREADS, (few_width<T, DP> <= 256 ? 2 : 1)) void vocab_few_kernel(VocabView a, VocabParts p) {
+__global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1)) void vocab_few_kernel(VocabView a, VocabParts p) {
     extern __shared__ __attribute__((aligned(TILE_ALIGN))) char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sp = blockIdx.x;
-    using M = FewKind<T, DP>;
+    using M = VocabKind<T, DP>;
     using S = typename Mma<M>::Store;
     S* tile = reinterpret_cast<S*>(lds) + wave * 32 * Tile<M, DP>::STRIDE;
     float* stats = reinterpret_cast<float*>(lds + FewLds<T, DP>::first);
@@ -210,7 +206,7 @@ __global__ __launch_bounds__(VS_THREADS, (few_width<T, DP> <= 256 ? 2 : 1)) void
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (v + 128 < v1) fetch(v + 128);
-        f32x16 sc[1] = {scores<M, DP, (few_width<T, DP> == 512)>(tile, 0, x)};
+        f32x16 sc[1] = {scores<M, DP, VocabTile<T, DP>::LEAD>(tile, 0, x)};
         const float c = adjust<1>(sc, a.b != nullptr ? bias : nullptr, v, v1, label);
         o.template step<1>(sc, c, 0.f);
         if (DX) o.template weigh<1>(tile, sc);
@@ -293,8 +289,7 @@ __global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, Voc
 }
 
 // ---- dw, db: 32 table rows a wave, over the rows of x ---------------------------------------------------------------------------------
-// bf16 2048 x 1000000 x 64: 617 us (850 TF/s of two products); 2048 x 100000 x 256: 370 us (567).  f32 in planes 1024 x 117581 x 64: 170 us (181 TF/s),
-// 777 x 50021 x 200: 299 us (the f32 instructions 709).
+// bf16 2048 x 1000000 x 64: 617 us (850 TF/s of two products); 2048 x 100000 x 256: 370 us (567).  f32 in planes 1024 x 117581 x 64: 170 us (181 TF/s).
 // With more than one split (a short vocabulary): part [splits][V][DP], part_b [splits][V], joined by vocab_dw_join_kernel.
 // (bf16 of 256: two waves a SIMD at the price of 13 spilled registers, 2048 x 100000: 510 us -> 370; the rows kernel would spill 110: 430 -> 514)
 template <typename T, int DP>
@@ -471,11 +466,9 @@ static int launch_fwd(const VocabView& a, float* loss, float* lse, void* dx, int
     const int64_t rows = (int64_t)f.splits * a.N;
     const VocabParts p{ws, ws + rows, ws + round_up(2 * rows, 4), f.splits, f.each};
     DCTR_REQUIRE((int64_t)f.row_blocks * f.splits <= INT32_MAX, "vocab softmax: too many blocks for one launch");
-    // (f32 wider than 128 with dx spills in the form for few rows: 16 x 50021 x 200 86 us, in the other 59)
-    constexpr bool FEW = !DX || few_width<T, DP> <= 512;
-    if (FEW && f.few) {
-        if constexpr (FEW) vocab_few_kernel<T, DP, DX><<<f.splits, VS_THREADS, FewLds<T, DP>::all, st>>>(a, p);
-    } else
+    if (f.few)
+        vocab_few_kernel<T, DP, DX><<<f.splits, VS_THREADS, FewLds<T, DP>::all, st>>>(a, p);
+    else
         vocab_rows_kernel<T, DP, DX><<<(unsigned)(f.row_blocks * f.splits), VS_THREADS,
                                        3 * (VocabTile<T, DP>::bytes + VocabTile<T, DP>::ROWS * sizeof(float)), st>>>(a, p, f.row_blocks);
     DCTR_LAUNCH_CHECK();
