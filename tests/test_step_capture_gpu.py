@@ -1,0 +1,52 @@
+"""dctr_time_kernel("train_step"): the captured steps are whole steps -- grouping, weight gradients and optimizer steps of the side streams included --
+and each of the two replays advances the engine as that many eager steps would."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import deepctr_oracle as O
+from tests.util import dev_batch
+from tf_repos_amd.engine import Engine, EngineConfig
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("hint", [False, True])
+@pytest.mark.parametrize("period", [1, 8])
+@pytest.mark.parametrize("B", [256, 4096])
+def test_replayed_steps_equal_eager_steps(B, period, hint, dev):
+    """Six steps of one batch, eager or as two replays of three captured ones.  A step more or less, or one whose rows were grouped wrongly, moves the
+    variables by about lr = 5e-4 each; the order of the float atomics moves single elements, the mean by far less than 1e-6."""
+    F, V, K = 39, 50_000, 16
+    kw = dict(model="deepfm", field_size=F, feature_size=V, embedding_size=K, deep_layers=(400, 400), dropout=(0.5, 0.5), l2_reg=1e-4, learning_rate=5e-4,
+              optimizer="Adam", max_batch=B, seed=3, use_graph=False, table_sweep_period=period)
+    ocfg = O.Config(model="deepfm", field_size=F, feature_size=V, embedding_size=K, deep_layers=(400, 400), dropout=(0.5, 0.5))
+    params = O.init_params(ocfg, seed=4, scale=0.01)
+    batches = [O.synth_batch(B, F, V, seed=90 + i) for i in range(3)]
+    states = []
+    for captured in (False, True):
+        eng = Engine(EngineConfig(**kw))
+        eng.set_params(params)
+        slots = []
+        for i, b in enumerate(batches):
+            slots.append(tuple(x[:B] for x in eng.input_slot(i)))
+            for to, of in zip(slots[i], dev_batch(*b, dev)):
+                to.copy_(of)
+        for i in range(3):
+            eng.train_step(*slots[i], want_loss=False)
+        if hint:
+            eng.prefetch_ids(slots[2][0])                   # the batch of the steps that follow: grouped ahead
+        if captured:
+            assert eng.time_stage("train_step", iters=3) > 0.0
+        else:
+            for i in range(6):
+                eng.train_step(*slots[2], want_loss=False)
+        assert eng.global_step == 9
+        eng.prefetch_ids(slots[0][0])
+        loss = eng.train_step(*slots[0])                    # ... and the engine goes on
+        eng.check_ids()
+        states.append((loss, dict(eng.get_params())))
+        eng.close()
+    assert abs(states[0][0] - states[1][0]) <= 1e-4 * abs(states[0][0])
+    for k, v in states[0][1].items():
+        assert np.abs(v - states[1][1][k]).mean() <= 1e-6, k

@@ -50,12 +50,14 @@ int fork(dctr_engine* E, hipStream_t from, hipStream_t to) {
 //     stop_arm(E);  <enqueue the op whose LAST kernel the fork depends on>;  stop_fork(E, st, to)  /  stop_record(E, st, &ev)
 // If the op's launch site took the armed event (the direct GEMM kernels and the fused head do), the event completes with that
 // kernel and no barrier packet is enqueued on `st`; otherwise it is recorded the ordinary way.  A/B knob DCTR_STOP_EVENTS=0.
+// Never while a step is captured: the capture does not see such a record.  A stream that waits for it stays outside the capture, its kernels run
+// at once, and what is captured waits for them without an edge -- groupings then count over slot words that no replay has cleared.
 static bool stop_events_on() {
     static const bool off = [] { const char* v = getenv("DCTR_STOP_EVENTS"); return v != nullptr && v[0] == '0'; }();
     return !off;
 }
 void stop_arm(dctr_engine* E) {
-    if (!stop_events_on() || E->cfg.use_graph) { E->armed_ev = nullptr; return; }
+    if (!stop_events_on() || E->cfg.use_graph || E->capturing) { E->armed_ev = nullptr; return; }
     E->armed_ev = E->events[E->ev_next++ % E->events.size()];
     arm_stop_event(E->armed_ev);
 }
@@ -668,7 +670,7 @@ int forward_rest(dctr_engine* E, int B, bool train, hipStream_t st, const std::f
         // relu(x W + b) [-> batch_norm] -> dropout (DeepFM.py:156-162): without BN the dropout rides in the GEMM epilogue
         // (every 32nd step only: a timed step costs ~15 us more -- event records, or launches with completion signals -- which the
         //  bench's `value` should not carry: 0.5 us per step on average)
-        if (i == 0) E->timer_step = E->timer_on && train && (E->timer_tick++ % 32) == 3;      // (not the very first step after the enable: it fills the pipeline)
+        if (i == 0) E->timer_step = E->timer_on && train && !E->capturing && (E->timer_tick++ % 32) == 3;      // (not the very first step after the enable: it fills the pipeline)
         const bool room = E->timer_n + 2 <= E->timer_ev.size();
         const bool timed = E->timer_step && room && E->timer_mode == 1 && i == 0;
         // mode 2: the launch carries its own start / stop events (common.h arm_timer_events) -- the interval is the dispatch alone
@@ -1140,7 +1142,7 @@ int record_train(dctr_engine* E, int B, hipStream_t st) {
     // dependency -- two cross-queue hops of ~10 us each, measured 0.374 -> 0.351 ms/step.  DCTR_STATE_ON_SIDE=1 is the old placement
     static const bool state_on_main = getenv("DCTR_STATE_ON_SIDE") == nullptr;
     // ids grouped ahead (dctr_prefetch_ids, during the tail of the previous step)
-    const bool pregrouped = E->pre_valid && E->pre_ids == E->ids && E->pre_B == B && E->group_alt != nullptr && !E->cfg.use_graph &&
+    const bool pregrouped = E->pre_valid && E->pre_ids == E->ids && E->pre_B == B && E->group_alt != nullptr && !E->cfg.use_graph && !E->capturing &&
                             E->pre_gen == E->slot_gen[E->pre_slot].load();     // (the slot still holds what was grouped)
     if (E->x_in_alt != nullptr && !E->cfg.use_graph) {       // (engine.h ev_dense: the step before may still be reading its x_in on the side stream)
         const bool e_is_x = E->e == E->x_in;
@@ -1283,7 +1285,7 @@ int record_train(dctr_engine* E, int B, hipStream_t st) {
     if (!fused_opt || (serial && sw != st)) DCTR_TRY(fork(E, st, sw));
     // where a prefetched grouping of the next batch may start (beside scatter + table step): the record of that last st -> sw
     // fork serves -- one more record here is one more barrier packet (~5 us) in front of the scatter
-    if (!E->cfg.use_graph && E->last_fork_ev != nullptr) { E->ev_tail = E->last_fork_ev; E->have_tail = true; }
+    if (!E->cfg.use_graph && !E->capturing && E->last_fork_ev != nullptr) { E->ev_tail = E->last_fork_ev; E->have_tail = true; }
     if (fused_opt) {
         // what is left of the dense arena: cross_w / cross_b (DCN), and the output layer + bias if they were not stepped above --
         // neighbours in the arena in one launch (c3: cross_w, cross_b were two 6-us launches at the very end of the step)
@@ -1317,12 +1319,13 @@ int record_train(dctr_engine* E, int B, hipStream_t st) {
     // A/B knob DCTR_PREGROUP_WAIT=end: the next batch's grouping (dctr_prefetch_ids) starts BEHIND the table step -- beside the next gather and
     // first forward product -- instead of beside it: one more record on st (in front of the next gather)
     static const bool pregroup_end = [] { const char* v = getenv("DCTR_PREGROUP_WAIT"); return v != nullptr && strcmp(v, "end") == 0; }();
-    if (pregroup_end && !E->cfg.use_graph) {
+    if (pregroup_end && !E->cfg.use_graph && !E->capturing) {
         hipEvent_t ev_end = nullptr;
         DCTR_TRY(record_on(E, st, &ev_end));
         E->ev_tail = ev_end; E->have_tail = true;
     }
-    if (!E->cfg.use_graph && !no_state_ahead && sw != st) {
+    // (a captured step advances the one state in place: prepared states change roles, which a replay cannot)
+    if (!E->cfg.use_graph && !E->capturing && !no_state_ahead && sw != st) {
         // the next step's state (global_step + 1, Adam's lr_t, dropout seed, zeroed loss scalars) into the second StepState, on
         // the weight-gradient stream beside scatter / table step: it only READS the live state, and the join below orders it
         // (state_early: already enqueued on the grouping stream, in front of the record the table step waited for)
@@ -2524,16 +2527,27 @@ int dctr_time_kernel(dctr_handle E, const char* kernel, int iters, float* h_ms_p
         set_error("unknown stage '%s'", kernel);
         return DCTR_ERR_NOT_FOUND;
     };
+    if (s == "train_step") {        // (every captured step groups its ids and advances the state by itself)
+        E->pre_valid = false;
+        E->state_ready = false;
+    }
     hipGraph_t graph = nullptr;
     hipStream_t cs = nullptr;
     DCTR_HIP_CHECK(hipStreamCreateWithFlags(&cs, hipStreamNonBlocking));
+    // (the capture's own events: the steps' hold records that eager streams may still wait for)
+    std::vector<hipEvent_t> own(E->events.size(), nullptr);
+    for (auto& ev : own) DCTR_HIP_CHECK(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
     DCTR_HIP_CHECK(hipStreamBeginCapture(cs, hipStreamCaptureModeThreadLocal));
     int rc = DCTR_OK;
+    std::swap(E->events, own);
     E->capturing = true;
     for (int i = 0; i < iters && rc == DCTR_OK; ++i) rc = stage(cs);
     E->capturing = false;
+    std::swap(E->events, own);
+    E->last_fork_ev = nullptr;
     hipError_t e = hipStreamEndCapture(cs, &graph);
     hipStreamDestroy(cs);
+    for (auto& ev : own) hipEventDestroy(ev);
     E->lag_suspended = false;
     if (rc != DCTR_OK) { if (graph) hipGraphDestroy(graph); return rc; }
     if (e != hipSuccess) { set_error("hipStreamEndCapture: %s", hipGetErrorString(e)); return DCTR_ERR_HIP; }
@@ -2554,8 +2568,10 @@ int dctr_time_kernel(dctr_handle E, const char* kernel, int iters, float* h_ms_p
     hipEventDestroy(e0); hipEventDestroy(e1);
     hipGraphExecDestroy(exec);
     *h_ms_per_launch = ms / (float)iters;
-    if (E->lag_period > 1) {        // whatever the stages did to the tables: every row counts as current from here on
-        DCTR_TRY(lag_stamp(E->row_ts, E->rows, E->state, st));
+    if (E->lag_period > 1) {
+        // (captured steps have left the tables as steps do; whatever a single stage did to them: every row counts as current from here on)
+        if (s == "train_step") DCTR_TRY(lag_flush_tables(E, st, 0, false));
+        else DCTR_TRY(lag_stamp(E->row_ts, E->rows, E->state, st));
         DCTR_HIP_CHECK(hipStreamSynchronize(st));
         E->lag_dirty = false;
     }

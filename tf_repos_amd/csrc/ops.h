@@ -35,8 +35,8 @@ struct OptBlockMeta {
     float l2;             // l2_reg coefficient if this variable is in the loss via l2_loss (DCN.py:199), else 0
 };
 
-// n 32-bit words cleared by a kernel.  What a step may record into a graph is cleared with this and not with hipMemsetAsync: replays after the first have
-// found the memory of such a node uncleared (a grouping then counts on from the last replay's distinct ids, past the end of its lists).
+// n 32-bit words cleared by a kernel.  What a step may record into a graph is cleared with this and not with hipMemsetAsync: replays after the first can
+// find the memory of such a node uncleared.
 int zero_words(void* p, size_t n, hipStream_t st);
 
 // ---- K8 grouping state (group.hip)
