@@ -546,7 +546,9 @@ int dctr_input_slot(dctr_handle h, int slot, int32_t** d_ids, float** d_vals, fl
  * The hint is tied to the slot's GENERATION: dctr_input_slot_rewrite(slot) -- which an input pipeline calls before it refills a
  * slot -- and the engine's own staging copies advance it, and a step whose slot has moved on since the hint groups the ids
  * itself instead of using a stale grouping.  dctr_prefetch_cancel drops a pending hint (end of a training loop: the announced
- * batch will not be trained).  dctr_input_slot_rewrite is safe to call from the input pipeline's thread. */
+ * batch will not be trained).  dctr_input_slot_rewrite is safe to call from the input pipeline's thread.  A grouping that is dropped may
+ * still be reading the slot: rewrite, fill and cancel wait for it (and only then), a staging copy is ordered behind it.  Announced ids
+ * that are rewritten without any of these are not grouped (nothing is written out of range). */
 int dctr_prefetch_ids(dctr_handle h, const int32_t* d_ids_next, int B);
 int dctr_prefetch_cancel(dctr_handle h);
 /* time-blocked table sweep (dctr_config.table_sweep_period > 1): advances every lagging table row to global_step, on `stream`.

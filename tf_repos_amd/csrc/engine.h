@@ -102,6 +102,7 @@ struct dctr_engine {
     bool pre_valid = false;
     int pre_slot = 0;               // ... of input slot `pre_slot` at generation `pre_gen`: a slot rewritten since (dctr_input_slot_rewrite,
     uint32_t pre_gen = 0;           // or a staging copy into it) no longer matches and the hint is dropped
+    std::atomic<int> slot_grouping[DCTR_INPUT_SLOTS] = {};    // a prefetched grouping that no step has taken over may still be reading the slot's ids
     std::atomic<uint32_t> slot_gen[DCTR_INPUT_SLOTS] = {};
     // dctr_input_slot_fill / acquire / release: the library's own H2D leg (created on first use)
     int device = 0;

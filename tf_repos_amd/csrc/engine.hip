@@ -1186,7 +1186,10 @@ int record_train(dctr_engine* E, int B, hipStream_t st) {
     // the id grouping (and the background table pass behind it) on the grouping stream
     // ids grouped ahead (dctr_prefetch_ids, during the tail of the previous step): the two grouping states change roles
     E->pre_valid = false;
-    if (pregrouped) std::swap(E->group, E->group_alt);
+    if (pregrouped) {
+        std::swap(E->group, E->group_alt);
+        E->slot_grouping[E->pre_slot].store(0, std::memory_order_release);      // (whoever rewrites the slot waits for this step)
+    }
     const int group_after = group_after_env >= 0 ? group_after_env
                             : E->mlp.empty() ? 0
                             : pregrouped ? (int)E->mlp.size()
@@ -1394,6 +1397,7 @@ int stage_inputs(dctr_engine* E, const int32_t* ids, const float* vals, const fl
     E->ids = E->slot_ids[slot]; E->vals = E->slot_vals[slot]; E->labels = E->slot_labels[slot];
     if (ids != E->ids) {
         E->slot_gen[slot]++;                // the staging copy rewrites the slot: a grouping prefetched from it is stale
+        if (E->slot_grouping[slot].exchange(0)) DCTR_TRY(fork(E, E->s_group, st));       // (and may still be reading it)
         DCTR_HIP_CHECK(hipMemcpyAsync(E->ids, ids, n * 4, hipMemcpyDeviceToDevice, st));
     }
     if (vals != E->vals) DCTR_HIP_CHECK(hipMemcpyAsync(E->vals, vals, n * 4, hipMemcpyDeviceToDevice, st));
@@ -1787,6 +1791,7 @@ int dctr_prefetch_ids(dctr_handle E, const int32_t* d_ids_next, int B) {
     if (E->have_tail && wait_mode != 0) DCTR_HIP_CHECK(hipStreamWaitEvent(sh, E->ev_tail, 0));
     // (a slot filled by dctr_input_slot_fill whose copies may still be in flight: the grouping stream waits for them on the device)
     if (E->slot_fill_pending[slot].load(std::memory_order_acquire)) DCTR_HIP_CHECK(hipStreamWaitEvent(sh, E->slot_filled[slot], 0));
+    E->slot_grouping[slot].store(1, std::memory_order_release);
     DCTR_TRY(group_ids(E->group_alt, d_ids_next, B, E->F, sh, !tail_fused(E)));
     E->pre_ids = d_ids_next; E->pre_B = B; E->pre_valid = true;
     E->pre_slot = slot; E->pre_gen = E->slot_gen[slot].load();
@@ -1798,16 +1803,24 @@ int dctr_tables_sync(dctr_handle E, void* stream) {
     return lag_flush_tables(E, as_stream(stream), 0, false);
 }
 
+// A dropped grouping is still on its way and reads its slot's ids twice; ids that change in between would be filled into segments that were never
+// counted.  Before a slot is rewritten without the step that was announced, its grouping is waited for.
+static int slot_grouping_done(dctr_engine* E, int slot) {
+    if (E->slot_grouping[slot].exchange(0)) DCTR_HIP_CHECK(hipStreamSynchronize(E->s_group));
+    return DCTR_OK;
+}
+
 int dctr_prefetch_cancel(dctr_handle E) {
     DCTR_REQUIRE(E, "null argument");
     E->pre_valid = false;
+    for (int k = 0; k < DCTR_INPUT_SLOTS; ++k) DCTR_TRY(slot_grouping_done(E, k));
     return DCTR_OK;
 }
 
 int dctr_input_slot_rewrite(dctr_handle E, int slot) {
     DCTR_REQUIRE(E && slot >= 0 && slot < DCTR_INPUT_SLOTS, "input slot %d outside [0, %d)", slot, DCTR_INPUT_SLOTS);
     E->slot_gen[slot]++;                    // (atomic: the input pipeline's thread calls this while the training thread enqueues steps)
-    return DCTR_OK;
+    return slot_grouping_done(E, slot);
 }
 
 // ---- the H2D leg of the input pipeline (see the header): events and the copy stream are made on first use, under a lock -- the input
@@ -1846,6 +1859,7 @@ int dctr_input_slot_fill(dctr_handle E, int slot, const int32_t* h_ids, const fl
     DCTR_TRY(slot_feed_init(E));
     DCTR_HIP_CHECK(hipSetDevice(E->device));                       // (the input thread's current device is its own affair)
     E->slot_gen[slot]++;                                           // a grouping prefetched from the slot's old contents is stale from here on
+    DCTR_TRY(slot_grouping_done(E, slot));
     const size_t n = (size_t)B * E->F;
     // a whole batch laid out like the slot ([ids | vals | labels], the first two padded to a multiple of 64 elements) is ONE copy: every host-to-device copy
     // brings its own system-scope acquire, and the step running beside it pays for each

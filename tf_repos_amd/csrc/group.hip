@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void group_fill_hash_kernel(const int32_t* __r
     for (int h = tid; h < HSIZE; h += 256)
         if (hkey[h] >= 0) {
             const int u = slot[hkey[h]] - 1;
-            hbase[h] = atomicAdd(&cursor[u], hcnt[h]);  // this block's run inside the id's segment
+            hbase[h] = u >= 0 ? atomicAdd(&cursor[u], hcnt[h]) : n;             // this block's run inside the id's segment (see group_fill_kernel)
             hkey[h] = u;
         }
     __syncthreads();
@@ -205,8 +205,10 @@ __global__ __launch_bounds__(256) void group_fill_hash_kernel(const int32_t* __r
     for (int k = 0; k < HCHUNK / 256; ++k)
         if (myh[k] >= 0) {
             const int pos = hbase[myh[k]] + myrank[k];
-            perm[pos] = base + k * 256 + tid;
-            seg_of[pos] = hkey[myh[k]];
+            if (pos < n) {
+                perm[pos] = base + k * 256 + tid;
+                seg_of[pos] = hkey[myh[k]];
+            }
         }
 }
 
@@ -305,10 +307,11 @@ __global__ __launch_bounds__(256) void group_fill_kernel(const int32_t* __restri
     const WaveGroup g = wave_group(id, valid, lane);
     int u = 0, base = 0;
     if (valid) u = slot[id] - 1;
-    if (valid && g.leader == lane) base = atomicAdd(&cursor[u], g.count);
+    if (valid && u >= 0 && g.leader == lane) base = atomicAdd(&cursor[u], g.count);
     base = __shfl(base, g.leader);
-    if (valid) {
-        const int pos = base + g.rank;
+    const int pos = base + g.rank;
+    // (an id that was not counted, or more often than now: the caller has rewritten ids that it had announced.  Nothing is written out of range.)
+    if (valid && u >= 0 && pos < n) {
         perm[pos] = i;
         seg_of[pos] = u;
     }
@@ -404,10 +407,10 @@ __global__ __launch_bounds__(GROUP_BLOCK) void group_one_block_kernel(const int3
         const WaveGroup g = wave_group(id, valid, lane);
         int u = 0, pos0 = 0;
         if (valid) u = slot[id] - 1;
-        if (valid && g.leader == lane) pos0 = atomicAdd(&cursor[u], g.count);
+        if (u >= 0 && valid && g.leader == lane) pos0 = atomicAdd(&cursor[u], g.count);
         pos0 = __shfl(pos0, g.leader);
-        if (valid) {
-            const int pos = pos0 + g.rank;
+        const int pos = pos0 + g.rank;
+        if (valid && u >= 0 && pos < n) {            // (see group_fill_kernel)
             perm[pos] = i;
             seg_of[pos] = u;
         }
