@@ -13,8 +13,10 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("how", ["rewrite", "fill", "cancel", "staging_copy", "predict"])
 @pytest.mark.parametrize("B", [256, 4096])
 def test_a_slot_rewritten_under_a_dropped_grouping(how, B, dev):
-    """Against the same steps without the announcement.  The optimizer is Adagrad: a step with wrong rows moves them by about lr = 1e-2, the order of the float
-    atomics the mean of a variable by far less than 1e-6."""
+    """Against the same steps without the announcement, by the mean over each variable.  The optimizer is Adagrad with lr = 1e-2: after 20 steps a step is about
+    lr / sqrt(20) = 2e-3, so one with wrong rows moves the rows' mean by 1e-4 and more.  The order of the float atomics moves an activation by 1e-7 of its
+    scale, which turns the ReLU decision of about 1e-6 of the 4096 x 96 x 21 = 8e6 units computed; each turned one adds or takes one of some 2000 examples
+    of random sign, 1 / sqrt(2000) of a step, in one column of 64: 2e-3 / 45 / 64 = 7e-7 of the mean, 6e-6 for all of them; 2e-5 leaves three times that."""
     F, V = 39, 60_000
     b = [O.synth_batch(B, F, V, seed=300 + i) for i in range(3)]
     b[2] = ((b[2][0] + V // 2) % V,) + b[2][1:]                 # other ids than those announced
@@ -58,4 +60,4 @@ def test_a_slot_rewritten_under_a_dropped_grouping(how, B, dev):
         runs.append(dict(eng.get_params()))
         eng.close()
     for k, v in runs[0].items():
-        assert np.abs(v - runs[1][k]).mean() <= 1e-6, k
+        assert np.abs(v - runs[1][k]).mean() <= 2e-5, k

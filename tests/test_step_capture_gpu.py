@@ -15,8 +15,10 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("period", [1, 8])
 @pytest.mark.parametrize("B", [256, 4096])
 def test_replayed_steps_equal_eager_steps(B, period, hint, dev):
-    """Six steps of one batch, eager or as two replays of three captured ones.  A step more or less, or one whose rows were grouped wrongly, moves the
-    variables by about lr = 5e-4 each; the order of the float atomics moves single elements, the mean by far less than 1e-6."""
+    """Six steps of one batch, eager or as two replays of three captured ones, by the mean over each variable.  A step more or less, or one whose rows were
+    grouped wrongly, moves the variables by about lr = 5e-4 each.  The order of the float atomics moves an activation by 1e-7 of its scale, which turns the
+    ReLU decision of about 1e-6 of the 4096 x 800 x 10 = 3e7 units computed; each turned one is 1 / sqrt(2000) of a step in one column of 400: 3e-8 of the
+    mean, 1e-6 for all of them; 1e-5 leaves ten times that."""
     F, V, K = 39, 50_000, 16
     kw = dict(model="deepfm", field_size=F, feature_size=V, embedding_size=K, deep_layers=(400, 400), dropout=(0.5, 0.5), l2_reg=1e-4, learning_rate=5e-4,
               optimizer="Adam", max_batch=B, seed=3, use_graph=False, table_sweep_period=period)
@@ -49,4 +51,4 @@ def test_replayed_steps_equal_eager_steps(B, period, hint, dev):
         eng.close()
     assert abs(states[0][0] - states[1][0]) <= 1e-4 * abs(states[0][0])
     for k, v in states[0][1].items():
-        assert np.abs(v - states[1][1][k]).mean() <= 1e-6, k
+        assert np.abs(v - states[1][1][k]).mean() <= 1e-5, k
