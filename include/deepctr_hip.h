@@ -574,7 +574,7 @@ int dctr_input_slot_acquire(dctr_handle h, int slot, void* stream);
 int dctr_input_slot_release(dctr_handle h, int slot, void* stream);
 int dctr_input_slot_wait_released(dctr_handle h, int slot);
 int dctr_input_slot_ready(dctr_handle h, int slot, int* ready);
-/* a non-blocking stream owned by the handle (created on first call, destroyed with it) for the caller's step calls: pass it as `stream`
+/* a non-blocking stream of the library's (one a device, shared by its handles, never destroyed) for the caller's step calls: pass it as `stream`
  * instead of the legacy default stream (0), on which every event of the step and of the slot handshake costs more.  The caller orders
  * its own work against it (hipStreamSynchronize / events) as with any stream. */
 int dctr_main_stream(dctr_handle h, void** stream);

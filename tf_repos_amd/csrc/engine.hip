@@ -132,6 +132,28 @@ int dropout_inplace(float* x, int64_t n, int width, float keep, const uint64_t* 
     return DCTR_OK;
 }
 
+// The streams beside the caller's: id grouping / routing, weight gradients + dense update, the handles' own main stream and the input copies.
+// All at the default priority: kernels of streams of different priorities can wait for each other on this chip without end, and priorities never moved a
+// step's time (weight gradients at high / normal / low: 0.2600 / 0.2598 / 0.2603 ms).  The runtime spreads streams over 4 hardware queues, and two that
+// share one run one behind the other: one set serves every handle of a device, made with the first and never destroyed, so that a second handle's streams
+// do not land on the queue of the stream it is called on (0.277 -> 0.328 ms a step).  Waits only ever look back in enqueueing order, so handles
+// that are used at the same time hold each other up at most.  Captures take streams of their own (CaptureStreams).
+struct SideStreams { hipStream_t group, wgrad, main, copy; };
+int side_streams(int device, SideStreams* out) {
+    static std::mutex mu;
+    static std::map<int, SideStreams> made;
+    std::lock_guard<std::mutex> lk(mu);
+    auto it = made.find(device);
+    if (it == made.end()) {
+        SideStreams s{};
+        DCTR_HIP_CHECK(hipSetDevice(device));
+        for (hipStream_t* p : {&s.group, &s.wgrad, &s.main, &s.copy}) DCTR_HIP_CHECK(hipStreamCreateWithFlags(p, hipStreamNonBlocking));
+        it = made.emplace(device, s).first;
+    }
+    *out = it->second;
+    return DCTR_OK;
+}
+
 int build(dctr_engine* E) {
     const dctr_config& c = E->cfg;
     DCTR_REQUIRE(c.model >= DCTR_MODEL_DEEPFM && c.model <= DCTR_MODEL_ESMM, "unknown model %d", c.model);
@@ -414,22 +436,12 @@ int build(dctr_engine* E) {
     }
 
     {
-        // The runtime multiplexes streams onto 4 hardware queues PER PRIORITY LEVEL, and which queue a stream lands on depends on
-        // how many other streams the process (torch, RCCL) has touched before: side streams that share the main stream's queue
-        // silently serialise behind it.  Giving each side stream its own priority level gives it a queue of its own:
-        // grouping / routing = low (background work hidden under the GEMMs), weight gradients + dense update = high.
-        int least = 0, greatest = 0;
-        DCTR_HIP_CHECK(hipDeviceGetStreamPriorityRange(&least, &greatest));
-        auto prio = [&](const char* env, int dflt) {
-            const char* v = getenv(env);
-            if (v == nullptr) return dflt;
-            return v[0] == 'h' ? greatest : (v[0] == 'l' ? least : 0);
-        };
-        // (use_graph: a graph captured across streams of different priorities replays 2.7x slower -- measured on c1 -- so the
-        //  graph mode keeps plain streams)
-        DCTR_HIP_CHECK(hipStreamCreateWithPriority(&E->s_group, hipStreamNonBlocking, c.use_graph ? 0 : prio("DCTR_PRIO_GROUP", least)));
-        DCTR_HIP_CHECK(hipStreamCreateWithPriority(&E->s_wgrad, hipStreamNonBlocking, c.use_graph ? 0 : prio("DCTR_PRIO_WGRAD", greatest)));
-        DCTR_HIP_CHECK(hipStreamCreateWithPriority(&E->s_opt, hipStreamNonBlocking, c.use_graph ? 0 : prio("DCTR_PRIO_OPT", least)));
+        SideStreams side;
+        DCTR_TRY(side_streams(E->device, &side));
+        E->s_group = side.group;
+        E->s_wgrad = side.wgrad;
+        if (getenv("DCTR_WGRAD_LATE") != nullptr || getenv("DCTR_OPT_SIDE") != nullptr)
+            DCTR_HIP_CHECK(hipStreamCreateWithFlags(&E->s_opt, hipStreamNonBlocking));
     }
     E->events.resize(64);
     {
@@ -1363,18 +1375,36 @@ int record_predict(dctr_engine* E, int B, hipStream_t st) {
     return DCTR_OK;
 }
 
+// While it lives the engine's side streams are streams of the capture's own: what other handles enqueue on the shared ones is theirs.
+struct CaptureStreams {
+    dctr_engine* E;
+    hipStream_t own[3] = {}, kept[3] = {};
+    explicit CaptureStreams(dctr_engine* e) : E(e) {}
+    int make() {
+        for (hipStream_t& s : own) DCTR_HIP_CHECK(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
+        kept[0] = E->s_group, kept[1] = E->s_wgrad;
+        E->s_group = own[0], E->s_wgrad = own[1];
+        return DCTR_OK;
+    }
+    hipStream_t origin() const { return own[2]; }
+    ~CaptureStreams() {
+        if (kept[0] != nullptr) E->s_group = kept[0], E->s_wgrad = kept[1];
+        for (hipStream_t s : own) if (s != nullptr) hipStreamDestroy(s);
+    }
+};
+
 int run_graph(dctr_engine* E, std::map<int, hipGraphExec_t>& cache, int B, bool train, hipStream_t st) {
     if (!E->cfg.use_graph) return train ? record_train(E, B, st) : record_predict(E, B, st);
     const int key = B * DCTR_INPUT_SLOTS + E->cur_slot;        // input pointers are baked into the graph
     auto it = cache.find(key);
     if (it == cache.end()) {
         hipGraph_t graph = nullptr;
-        hipStream_t cs = nullptr;
-        DCTR_HIP_CHECK(hipStreamCreateWithFlags(&cs, hipStreamNonBlocking));
+        CaptureStreams streams(E);
+        DCTR_TRY(streams.make());
+        const hipStream_t cs = streams.origin();
         DCTR_HIP_CHECK(hipStreamBeginCapture(cs, hipStreamCaptureModeThreadLocal));
         int rc = train ? record_train(E, B, cs) : record_predict(E, B, cs);
         hipError_t e = hipStreamEndCapture(cs, &graph);
-        hipStreamDestroy(cs);
         if (rc != DCTR_OK) { if (graph) hipGraphDestroy(graph); return rc; }
         if (e != hipSuccess) { set_error("hipStreamEndCapture: %s", hipGetErrorString(e)); return DCTR_ERR_HIP; }
         hipGraphExec_t exec = nullptr;
@@ -1553,8 +1583,8 @@ int dctr_destroy(dctr_handle E) {
     if (E->entry_goff) hipFree(E->entry_goff);
     if (E->pair_ad) hipFree(E->pair_ad);
     { float* f3[] = {E->x_att, E->att_sc, E->att_w}; for (float* p : f3) if (p) hipFree(p); }
-    if (E->s_copy) { hipStreamSynchronize(E->s_copy); hipStreamDestroy(E->s_copy); }
-    if (E->s_main) { hipStreamSynchronize(E->s_main); hipStreamDestroy(E->s_main); }
+    if (E->s_copy) hipStreamSynchronize(E->s_copy);
+    if (E->s_main) hipStreamSynchronize(E->s_main);
     for (int k = 0; k < DCTR_INPUT_SLOTS; ++k) { if (E->slot_filled[k]) hipEventDestroy(E->slot_filled[k]); if (E->slot_released[k]) hipEventDestroy(E->slot_released[k]); }
     for (int k = 0; k < DCTR_INPUT_SLOTS; ++k) if (E->slot_ids[k]) hipFree(E->slot_ids[k]);       // (vals and labels live in the same block)
     if (E->status) hipFree(E->status);
@@ -1581,8 +1611,6 @@ int dctr_destroy(dctr_handle E) {
     for (auto& ev : E->events) if (ev) hipEventDestroy(ev);
     if (E->ev_dense) hipEventDestroy(E->ev_dense);
     if (E->x_in_alt) hipFree(E->x_in_alt);
-    if (E->s_group) hipStreamDestroy(E->s_group);
-    if (E->s_wgrad) hipStreamDestroy(E->s_wgrad);
     if (E->s_opt) hipStreamDestroy(E->s_opt);
     delete E;
     return DCTR_OK;
@@ -1831,15 +1859,9 @@ static int slot_feed_init(dctr_engine* E) {
     std::lock_guard<std::mutex> lk(mu);
     if (E->slot_feed_ready.load(std::memory_order_acquire)) return DCTR_OK;
     DCTR_HIP_CHECK(hipSetDevice(E->device));
-    {
-        // the copy stream at the LOW priority level (with the grouping stream): streams share 4 hardware queues per priority level, and a
-        // copy stream that lands on the training stream's queue serialises the H2D copies with the steps (A/B knob DCTR_PRIO_COPY)
-        int least = 0, greatest = 0;
-        DCTR_HIP_CHECK(hipDeviceGetStreamPriorityRange(&least, &greatest));
-        const char* v = getenv("DCTR_PRIO_COPY");
-        const int pr = v == nullptr ? least : (v[0] == 'h' ? greatest : (v[0] == 'l' ? least : 0));
-        DCTR_HIP_CHECK(hipStreamCreateWithPriority(&E->s_copy, hipStreamNonBlocking, pr));
-    }
+    SideStreams side;
+    DCTR_TRY(side_streams(E->device, &side));
+    E->s_copy = side.copy;
     // no system-scope fence on either record: "filled" orders a copy before kernels of the same device, "released" tells the host
     // that kernels have finished READING -- nothing they wrote is for the host to see.  (A plain event's record writes the L2s
     // back: with the tables' dirty lines in them that was worth 60 us per step through the feeder.)
@@ -1898,14 +1920,15 @@ int dctr_input_slot_wait_released(dctr_handle E, int slot) {
     return DCTR_OK;
 }
 
-// A stream of the engine's own for the caller's step calls.  Why: the legacy default stream (what a Python caller that never thinks about
+// A stream of the library's for the caller's step calls (side_streams).  Why: the legacy default stream (what a Python caller that never thinks about
 // streams passes) pays for every cross-stream record / wait of the step and of the input slots' handshake -- the feeder-driven loop
 // ran 312 us per step there against 272 us on a stream of its own (tools/feeder_breakdown.py); the Estimator trains on this one.
 int dctr_main_stream(dctr_handle E, void** stream) {
     DCTR_REQUIRE(E && stream, "null argument");
     if (E->s_main == nullptr) {
-        DCTR_HIP_CHECK(hipSetDevice(E->device));
-        DCTR_HIP_CHECK(hipStreamCreateWithFlags(&E->s_main, hipStreamNonBlocking));
+        SideStreams side;
+        DCTR_TRY(side_streams(E->device, &side));
+        E->s_main = side.main;
     }
     *stream = reinterpret_cast<void*>(E->s_main);
     return DCTR_OK;
@@ -2546,8 +2569,9 @@ int dctr_time_kernel(dctr_handle E, const char* kernel, int iters, float* h_ms_p
         E->state_ready = false;
     }
     hipGraph_t graph = nullptr;
-    hipStream_t cs = nullptr;
-    DCTR_HIP_CHECK(hipStreamCreateWithFlags(&cs, hipStreamNonBlocking));
+    CaptureStreams streams(E);
+    DCTR_TRY(streams.make());
+    const hipStream_t cs = streams.origin();
     // (the capture's own events: the steps' hold records that eager streams may still wait for)
     std::vector<hipEvent_t> own(E->events.size(), nullptr);
     for (auto& ev : own) DCTR_HIP_CHECK(hipEventCreateWithFlags(&ev, hipEventDisableTiming));
@@ -2560,7 +2584,6 @@ int dctr_time_kernel(dctr_handle E, const char* kernel, int iters, float* h_ms_p
     std::swap(E->events, own);
     E->last_fork_ev = nullptr;
     hipError_t e = hipStreamEndCapture(cs, &graph);
-    hipStreamDestroy(cs);
     for (auto& ev : own) hipEventDestroy(ev);
     E->lag_suspended = false;
     if (rc != DCTR_OK) { if (graph) hipGraphDestroy(graph); return rc; }

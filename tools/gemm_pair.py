@@ -29,7 +29,7 @@ def run(fns, streams):
 
 
 def main():
-    s1, s2 = torch.cuda.Stream(priority=0), torch.cuda.Stream(priority=-1)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
     for (M, K, N) in [(4096, 624, 400), (4096, 400, 400)]:
         x = torch.randn(M, K, device=dev); w = torch.randn(K, N, device=dev) * 0.05
         y = torch.randn(M, N, device=dev).relu(); dy = torch.randn(M, N, device=dev); dx = torch.empty(M, K, device=dev)
