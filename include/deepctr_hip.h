@@ -439,7 +439,8 @@ typedef struct dctr_attention {
     int32_t n_seg;                     /* examples: segment b = rows [q_offsets[b], q_offsets[b+1]) x [k_offsets[b], k_offsets[b+1]) */
     int32_t heads, kv_heads;           /* query head h reads key head h / (heads / kv_heads)                                  */
     int32_t head_dim;                  /* a multiple of 8, 8..128; head h of a row is columns [h*head_dim, (h+1)*head_dim)     */
-    int32_t max_q, max_k;              /* no segment has more rows (the launches are sized by them); at most DCTR_MAX_POSITION  */
+    int32_t max_q, max_k;              /* no segment has more rows; at most DCTR_MAX_POSITION.  The launches are sized by them: a call that
+                                        * needs 2^24 blocks or more is refused (n_seg x heads x ceil(max / 32) below that always fits) */
     int32_t causal;                    /* 1: a query sees the keys at positions <= its own only                               */
     int64_t total_q, total_k;          /* rows of the q / k, v arrays: offsets stay within them                               */
     float   scale;                     /* of the scores, e.g. 1/sqrt(head_dim)                                                */
@@ -472,7 +473,7 @@ int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld,
                              void* d_workspace, size_t workspace_bytes, void* stream);
 /* Softmax cross entropy of N rows against a vocabulary's table, without the [N, V] logits: z = x w^T + b (d_b f32 [V] or null),
  *     d_loss[n] = lse_n - z[n, label_n]      d_lse[n] = log sum_v exp(z_nv) (may be null)
- * N <= 2^30, V < 2^31.  d_labels int32 [N]; a negative label = a row without one: loss 0, no gradient; one >= V is treated the same and flagged in d_status
+ * N <= 2^30, V < 2^31 (bwd_weights: V <= 2^31 - 128).  d_labels int32 [N]; a negative label = a row without one: loss 0, no gradient; one >= V is treated the same and flagged in d_status
  * (int32[2] or null: [0] = 1, [1] = the label).  Gradients are of  sum_n scale * d_row_scale[n] * loss_n  (d_row_scale f32 [N] or null = 1;
  * scale = 1/batch for a mean).  d_x [N, D], d_w [V, D] and the gradients in `dtype`, rows 16-byte aligned, D a multiple of 8, 8..256.
  *   fwd: loss, lse and, d_dx not null, dL/dx [N, dx_ld] from the same pass over the table

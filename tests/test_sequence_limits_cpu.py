@@ -1,0 +1,53 @@
+"""Sizes at the edge of what a launch can hold (fewer than 2^32 threads in a grid's dimension): refused before the first launch, no GPU needed."""
+import ctypes as C
+
+import pytest
+
+from tf_repos_amd import capi, errors
+from tests.test_sequence_ops_cpu import A, attention, bwd, fwd, vbwd, vfwd
+
+
+@pytest.mark.parametrize("other", [dict(n_seg=65536, heads=16, kv_heads=16, max_q=2048, max_k=128, total_q=1 << 27, total_k=1 << 23),
+                                   dict(n_seg=1 << 24, heads=4, kv_heads=4, max_q=8, max_k=600, total_q=1 << 27, total_k=1 << 30),
+                                   dict(n_seg=1, heads=1024, kv_heads=1024, max_q=1 << 28, max_k=1, total_q=1 << 28, total_k=1),
+                                   dict(n_seg=(1 << 26) + 1, heads=1, kv_heads=1, max_q=1, max_k=1, total_q=1, total_k=1),
+                                   dict(n_seg=1 << 26, heads=1024, kv_heads=1024, max_q=1 << 28, max_k=1 << 28, total_q=1 << 30, total_k=1 << 30, n_buckets=128)])
+def test_attention_of_too_many_blocks_refused(other):
+    a, size = attention(**other), C.c_int64()
+    for i in range(a.n_buckets - 1):
+        a.boundaries[i] = i
+    ld = 16 * a.heads
+    for call in (lambda: fwd(a, q_ld=ld, k_ld=ld, v_ld=ld, out_ld=ld, bias=A if a.n_buckets else None),
+                 lambda: capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), 0, C.byref(size))):
+        with pytest.raises(errors.InvalidArgumentError, match="blocks in one launch|segments"):
+            capi.check(call())
+
+
+@pytest.mark.parametrize("other", [dict(n_seg=1 << 23, max_q=0, max_k=600, total_q=0, total_k=1 << 30), dict(n_seg=1 << 21, max_q=1, max_k=4096, total_q=1 << 21, total_k=1 << 30)])
+def test_a_backward_whose_second_launch_does_not_fit_refused_before_the_first(other):
+    a = attention(heads=1, kv_heads=1, **other)
+    size = C.c_int64()
+    capi.check(capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), 0, C.byref(size)))        # (the forward fits)
+    with pytest.raises(errors.InvalidArgumentError, match="blocks in one launch"):
+        capi.check(capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), 1, C.byref(size)))
+    with pytest.raises(errors.InvalidArgumentError, match="blocks in one launch"):
+        capi.check(bwd(a))
+
+
+def test_workspace_of_the_largest_call_that_fits():
+    a, size = attention(n_seg=1 << 13, heads=16, kv_heads=16, max_q=4096, max_k=4096, total_q=1 << 25, total_k=1 << 25, n_buckets=128), C.c_int64()
+    for i in range(127):
+        a.boundaries[i] = 8 * i
+    capi.check(capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), 1, C.byref(size)))
+    assert size.value >= 4 * ((1 << 25) * 16 + (1 << 13) * 16 * 32 * 128)
+
+
+def test_a_vocabulary_of_more_table_blocks_than_a_launch_holds_refused():
+    for v in ((1 << 31) - 1, (1 << 31) - 127):
+        with pytest.raises(errors.InvalidArgumentError, match="vocabulary"):
+            capi.check(vbwd(v=v, size=1 << 62))
+    for v in ((1 << 31) - 128, 10):                                      # (refused for something else: the size is fine)
+        with pytest.raises(errors.InvalidArgumentError, match="dw"):
+            capi.check(vbwd(v=v, dw=None, size=1 << 62))
+    with pytest.raises(errors.InvalidArgumentError, match="loss"):
+        capi.check(vfwd(v=(1 << 31) - 1, loss=None, size=1 << 62))

@@ -137,6 +137,7 @@ inline bool attn_solo(const dctr_attention* a, int64_t items) {
 // chunks: no more pairs of segment and cut than these.
 struct AttnSplit { int row_blocks, splits, each, chunks; bool solo; };
 AttnSplit attn_split(const dctr_attention* a);
+int64_t attn_fwd_blocks(const dctr_attention* a);         // of the call's largest launch
 int64_t attn_fwd_workspace(const dctr_attention* a);      // bytes
 int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st);
 
@@ -149,6 +150,7 @@ struct AttnGrads {
     void* dv; int64_t dv_ld;
     float* dbias;                                       // may be null
 };
+int64_t attn_bwd_blocks(const dctr_attention* a);
 int64_t attn_bwd_workspace(const dctr_attention* a);
 int attn_bwd(const dctr_attention* a, const AttnView& v, const AttnGrads& x, float* ws, hipStream_t st);
 

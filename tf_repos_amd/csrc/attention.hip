@@ -19,6 +19,7 @@ __global__ void fill_zero_kernel(float* x, int n) {
 static int check_attention(const dctr_attention* a) {
     DCTR_REQUIRE(a != nullptr, "null attention description");
     DCTR_REQUIRE(a->dtype == DCTR_TYPE_F32 || a->dtype == DCTR_TYPE_BF16, "attention: unknown element type %d", a->dtype);
+    DCTR_REQUIRE(a->n_seg <= 1 << 26, "attention: %d segments (at most 2^26)", a->n_seg);       // (products of sizes stay within 64 bits)
     DCTR_REQUIRE(a->n_seg >= 0 && a->max_q >= 0 && a->max_k >= 0 && a->total_q >= 0 && a->total_k >= 0, "attention: negative size");
     DCTR_REQUIRE(a->total_q <= INT32_MAX && a->total_k <= INT32_MAX, "attention: more rows than int32 offsets reach");
     DCTR_REQUIRE(a->max_q <= DCTR_MAX_POSITION && a->max_k <= DCTR_MAX_POSITION, "attention: segments of %d x %d rows (at most %d)", a->max_q, a->max_k,
@@ -64,11 +65,20 @@ static int make_view(const dctr_attention* a, const void* q, int q_ld, const voi
     return DCTR_OK;
 }
 
+// Every launch of a call, before the first one.
+static int check_launches(const dctr_attention* a, int backward) {
+    const int64_t blocks = std::max(attn_fwd_blocks(a), backward ? attn_bwd_blocks(a) : 0);
+    DCTR_REQUIRE(blocks <= MAX_BLOCKS, "attention: %lld blocks in one launch (at most %lld): too many segments, heads or rows a segment", (long long)blocks,
+                 (long long)MAX_BLOCKS);
+    return DCTR_OK;
+}
+
 static int64_t workspace_bytes(const dctr_attention* a, int backward) {
     return std::max(attn_fwd_workspace(a), backward ? attn_bwd_workspace(a) : 0);
 }
 
 static int check_workspace(const dctr_attention* a, int backward, const void* ws, size_t bytes) {
+    DCTR_TRY(check_launches(a, backward));
     const int64_t need = workspace_bytes(a, backward);
     DCTR_REQUIRE(need == 0 || (ws != nullptr && (int64_t)bytes >= need), "attention: workspace of %lld bytes needed, %lld given", (long long)need,
                  ws != nullptr ? (long long)bytes : 0ll);
@@ -85,6 +95,7 @@ extern "C" {
 int dctr_cross_attention_workspace_bytes(const dctr_attention* a, int backward, int64_t* bytes) {
     DCTR_REQUIRE(bytes != nullptr, "null out pointer");
     DCTR_TRY(check_attention(a));
+    DCTR_TRY(check_launches(a, backward));
     *bytes = workspace_bytes(a, backward);
     return DCTR_OK;
 }

@@ -645,6 +645,12 @@ static int key_form(const dctr_attention* a) {
 }
 static int row_blocks_of(const dctr_attention* a) { return ceil_div(a->max_q, query_form(a) == ROWS ? 128 : 32); }
 
+int64_t attn_bwd_blocks(const dctr_attention* a) {
+    const int keys = key_form(a);
+    const int64_t q = (int64_t)row_blocks_of(a) * a->heads * a->n_seg, k = (int64_t)ceil_div(a->max_k, keys == KEY_ROWS ? 128 : 32) * a->kv_heads * a->n_seg;
+    return std::max(query_form(a) == SOLO ? (q + 3) / 4 : q, (keys == KEY_SOLO ? (k + 3) / 4 : k) + a->heads);
+}
+
 // delta, then the bias gradient's shares
 int64_t attn_bwd_workspace(const dctr_attention* a) {
     return 4 * (round_up(a->total_q * a->heads, 4) + (int64_t)a->heads * a->n_seg * row_blocks_of(a) * a->n_buckets);
@@ -654,7 +660,6 @@ template <typename T, int DP, int FORM>
 static int launch_q(const dctr_attention* a, const AttnView& v, const AttnGrads& x, float* delta, float* part, hipStream_t st) {
     const int row_blocks = row_blocks_of(a);
     const int64_t items = (int64_t)row_blocks * a->heads * a->n_seg, blocks = FORM == SOLO ? (items + 3) / 4 : items;
-    DCTR_REQUIRE(items <= INT32_MAX, "attention: too many blocks for one launch");
     if (blocks == 0) return DCTR_OK;
     const size_t lds = QuerySide<T, DP, FORM>::first + sizeof(float) * (QuerySide<T, DP, FORM>::HIDDEN + 4 * SKEW + (FORM == SOLO ? 8 : 5) * rel_reach(a) + 8);
     attn_bwd_q_kernel<T, DP, FORM><<<(unsigned)blocks, BWD_THREADS, lds, st>>>(v, (const T*)x.out, x.out_ld, x.lse, (const T*)x.dout, x.dout_ld, (T*)x.dq, x.dq_ld,
@@ -668,7 +673,6 @@ static int launch_kv(const dctr_attention* a, const AttnView& v, const AttnGrads
     using Kd = KeySide<T, DP, FORM>;
     const int key_blocks = ceil_div(a->max_k, Kd::OWN ? 32 : 128), sums = part != nullptr ? a->heads : 0;
     const int64_t items = (int64_t)key_blocks * a->kv_heads * a->n_seg, blocks = FORM == KEY_SOLO ? (items + 3) / 4 : items;
-    DCTR_REQUIRE(items + a->heads <= INT32_MAX, "attention: too many blocks for one launch");
     if (blocks + sums == 0) return DCTR_OK;
     const size_t lds = std::max(Kd::tiles + Kd::stats + sizeof(float) * (Kd::OWN ? 8 : 2) * rel_reach(a), BWD_THREADS * sizeof(float));
     attn_bwd_kv_kernel<T, DP, FORM><<<(unsigned)(blocks + sums), BWD_THREADS, lds, st>>>(

@@ -419,14 +419,12 @@ static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int
     if (cut.splits == 0) {
         const int row_blocks = ceil_div(a->max_q, 128);
         const int64_t blocks = (int64_t)row_blocks * a->heads * a->n_seg;
-        DCTR_REQUIRE(blocks <= INT32_MAX, "attention: too many blocks for one launch");
         const size_t lds = 4 * rows_keys<T, DP> * attn_width<T, DP> + (2 * rows_keys<T, DP> + rel_reach(a)) * sizeof(float);
         attn_rows_kernel<T, DP><<<(unsigned)blocks, ROWS_THREADS, lds, st>>>(v, (T*)out, out_ld, lse, status, row_blocks);
         DCTR_LAUNCH_CHECK();
         return DCTR_OK;
     }
     const int64_t items = (int64_t)cut.row_blocks * a->kv_heads * a->n_seg;
-    DCTR_REQUIRE(items * 8 <= INT32_MAX, "attention: too many blocks for one launch");
     if (items == 0) return DCTR_OK;
     using L = SplitLds<T, DP>;
     if (cut.solo)
@@ -448,6 +446,13 @@ static int by_width(const dctr_attention* a, const AttnView& v, void* out, int64
         case 64: return launch_fwd<T, 64>(a, v, out, out_ld, lse, status, ws, st);
         default: return launch_fwd<T, 128>(a, v, out, out_ld, lse, status, ws, st);
     }
+}
+
+int64_t attn_fwd_blocks(const dctr_attention* a) {
+    const AttnSplit cut = attn_split(a);
+    if (cut.splits == 0) return (int64_t)ceil_div(a->max_q, 128) * a->heads * a->n_seg;
+    const int64_t items = (int64_t)cut.row_blocks * a->kv_heads * a->n_seg;
+    return cut.solo ? (items + 3) / 4 : cut.splits > 1 ? std::max((int64_t)cut.row_blocks * a->kv_heads * cut.chunks, items * 8) : items;
 }
 
 int64_t attn_fwd_workspace(const dctr_attention* a) {

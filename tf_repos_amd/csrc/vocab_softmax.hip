@@ -238,12 +238,11 @@ __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 ? 2 : 1
     p.e[(int64_t)sp * a.N + threadIdx.x] = sum;
 }
 
-// Joins the splits and adds the label's column: one block a row, thread = (4 columns, slice of the splits) for dx.
+// Joins the splits and adds the label's column: one block a row (and every gridDim.x-th one behind it), thread = (4 columns, slice of the splits) for dx.
+constexpr int JOIN_BLOCKS = 1 << 22;                    // of the launch: there are more rows than one can have blocks
 template <typename T, int DP, bool DX>
-__global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, VocabParts p, float* loss, float* lse, T* dx, int64_t dx_ld, int32_t* status) {
-    __shared__ float red[3][4];
-    __shared__ f32x4 cols[VS_THREADS];
-    const int64_t n = blockIdx.x;
+__device__ __forceinline__ void vocab_join_row(const VocabView& a, const VocabParts& p, float* loss, float* lse, T* dx, int64_t dx_ld, int32_t* status, int64_t n,
+                                               float (&red)[3][4], f32x4 (&cols)[VS_THREADS]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int label = a.labels[n];
     const bool on = label >= 0 && label < a.V;
@@ -286,6 +285,15 @@ __global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, Voc
 #pragma unroll
     for (int d = 0; d < 4; ++d) to[d] = on ? c * (acc[d] - e * to_f32(w[col + d])) / all : 0.f;
     Mma<T>::store4(dx + n * dx_ld + col, to[0], to[1], to[2], to[3]);
+}
+template <typename T, int DP, bool DX>
+__global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, VocabParts p, float* loss, float* lse, T* dx, int64_t dx_ld, int32_t* status) {
+    __shared__ float red[3][4];
+    __shared__ f32x4 cols[VS_THREADS];
+    for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x) {
+        vocab_join_row<T, DP, DX>(a, p, loss, lse, dx, dx_ld, status, n, red, cols);
+        __syncthreads();                                                // (the next row's sums go where this one's are read)
+    }
 }
 
 // ---- dw, db: 32 table rows a wave, over the rows of x ---------------------------------------------------------------------------------
@@ -465,14 +473,13 @@ static int launch_fwd(const VocabView& a, float* loss, float* lse, void* dx, int
     const VocabPlan f = plan_fwd(a.N, a.V);
     const int64_t rows = (int64_t)f.splits * a.N;
     const VocabParts p{ws, ws + rows, ws + round_up(2 * rows, 4), f.splits, f.each};
-    DCTR_REQUIRE((int64_t)f.row_blocks * f.splits <= INT32_MAX, "vocab softmax: too many blocks for one launch");
     if (f.few)
         vocab_few_kernel<T, DP, DX><<<f.splits, VS_THREADS, FewLds<T, DP>::all, st>>>(a, p);
     else
         vocab_rows_kernel<T, DP, DX><<<(unsigned)(f.row_blocks * f.splits), VS_THREADS,
                                        3 * (VocabTile<T, DP>::bytes + VocabTile<T, DP>::ROWS * sizeof(float)), st>>>(a, p, f.row_blocks);
     DCTR_LAUNCH_CHECK();
-    vocab_join_kernel<T, DP, DX><<<a.N, VS_THREADS, 0, st>>>(a, p, loss, lse, (T*)dx, dx_ld, status);
+    vocab_join_kernel<T, DP, DX><<<std::min(a.N, JOIN_BLOCKS), VS_THREADS, 0, st>>>(a, p, loss, lse, (T*)dx, dx_ld, status);
     DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
@@ -481,7 +488,6 @@ template <typename T, int DP>
 static int launch_dw(const VocabView& a, const float* lse, void* dw, int64_t dw_ld, float* db, float* ws, hipStream_t st) {
     const VocabWPlan w = plan_dw(a.N, a.V);
     float *part = ws, *part_b = ws + (int64_t)w.splits * a.V * DP;
-    DCTR_REQUIRE((int64_t)w.table_blocks * w.splits <= INT32_MAX, "vocab softmax: too many blocks for one launch");
     const size_t lds = 2 * (VocabTile<T, DP>::bytes + 3 * VocabTile<T, DP>::ROWS * sizeof(float));
     vocab_dw_kernel<T, DP><<<(unsigned)(w.table_blocks * w.splits), VS_THREADS, lds, st>>>(a, lse, (T*)dw, dw_ld, db, part, part_b, w.splits, w.each,
                                                                                            w.table_blocks);
@@ -573,6 +579,7 @@ int dctr_vocab_softmax_bwd_weights(int dtype, const void* d_x, int x_ld, const v
     VocabView a;
     DCTR_TRY(make_view(dtype, d_x, x_ld, d_w, w_ld, d_b, d_labels, N, V, D, d_row_scale, scale, 1, d_workspace, workspace_bytes, &a));
     DCTR_REQUIRE(N == 0 || d_lse != nullptr, "vocab softmax: lse is null");
+    DCTR_REQUIRE(V <= 128 * MAX_BLOCKS, "vocab softmax: vocabulary of %lld (gradients: at most %lld)", (long long)V, (long long)(128 * MAX_BLOCKS));   // (a block 128 rows)
     DCTR_TRY(check_rows("dw", d_dw, dw_ld, D, dtype == DCTR_TYPE_F32 ? 4 : 2));
     hipStream_t st = as_stream(stream);
     float* ws = (float*)d_workspace;
