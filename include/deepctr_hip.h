@@ -432,7 +432,7 @@ int dctr_dcn_cross_bwd(const float* d_xs, const float* d_xlw, const float* d_w, 
  * sums, softmax statistics, biases, their gradients and losses in f32. */
 enum { DCTR_TYPE_F32 = 0, DCTR_TYPE_BF16 = 1 };
 #define DCTR_MAX_REL_BUCKETS 128
-#define DCTR_MAX_REL_SPAN 1024         /* last boundary - first boundary */
+#define DCTR_MAX_REL_SPAN 1025         /* last boundary - first boundary: steps of up to 512 on either side, -512 .. 513 */
 #define DCTR_MAX_POSITION (1 << 28)
 typedef struct dctr_attention {
     int32_t dtype;                     /* DCTR_TYPE_* of q, k, v, out and their gradients                                     */

@@ -34,6 +34,18 @@ def test_a_backward_whose_second_launch_does_not_fit_refused_before_the_first(ot
         capi.check(bwd(a))
 
 
+@pytest.mark.parametrize("edges,fits", [((-512, 513), True), ((-512, 514), False), ((0, 1025), True), ((-2000, -975), True), ((-2000, -974), False)])
+def test_boundaries_reach_512_steps_to_either_side(edges, fits):
+    a, size = attention(n_buckets=3), C.c_int64()
+    a.boundaries[0], a.boundaries[1] = edges
+    call = lambda: capi.check(capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), 1, C.byref(size)))      # noqa: E731
+    if fits:
+        call()
+    else:
+        with pytest.raises(errors.InvalidArgumentError, match="boundaries span"):
+            call()
+
+
 def test_workspace_of_the_largest_call_that_fits():
     a, size = attention(n_seg=1 << 13, heads=16, kv_heads=16, max_q=4096, max_k=4096, total_q=1 << 25, total_k=1 << 25, n_buckets=128), C.c_int64()
     for i in range(127):
