@@ -455,7 +455,8 @@ typedef struct dctr_attention {
  *   d_q [total_q, heads * head_dim], d_k / d_v [total_k, kv_heads * head_dim]; row strides *_ld in elements; rows 16-byte aligned
  *   d_q_offsets / d_k_offsets int32 [n_seg + 1]; d_q_start int32 [n_seg] or null; d_rel_bias f32 [n_buckets, heads]
  *   d_status int32[2] or null: [0] = 1, [1] = b if segment b's offsets leave the arrays, descend, or hold more than max_q / max_k rows
- *              (or its q_start is beyond +-DCTR_MAX_POSITION): such a segment is cut to what is within
+ *              (or its q_start is beyond +-DCTR_MAX_POSITION): such a segment is cut to what is within.  Only set: the caller clears it.  Offsets that
+ *              descend can make segments share rows; of those rows' outputs and gradients one segment's stay
  *   d_workspace: dctr_cross_attention_workspace_bytes(a, backward) bytes (0: the forward's; 1: enough for the forward and the backward), 16-byte
  *              aligned, overwritten; calls that may run at the same time (streams, captured graphs) need one each.  A handful of queries per segment (serving) splits long histories over blocks. */
 int dctr_cross_attention_workspace_bytes(const dctr_attention* a, int backward, int64_t* bytes);

@@ -46,3 +46,35 @@ def test_boundaries_at_the_widest_span(dtype, heads, kv_heads, dim, q, k, dev):
     torch.cuda.synchronize()
     assert d["status"].tolist() == [0, 0]
     case.check(d, ("out", "lse", "dq", "dk", "dv", "db"))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n_seg", [5, 150])
+def test_overlapping_segments_of_descending_offsets_in_the_split_form(dtype, n_seg, dev):
+    """k_offsets 0, T, 0, T, ..: every other segment descends (flagged) and those between all hold the same T keys, more cuts than disjoint segments could have.
+    The workspace is filled with NaN bytes; each such segment gives what it gives alone."""
+    T, H, D = 9001, 4, 32
+    case = AttentionCase(dtype, [1] * n_seg, [T] + [0] * (n_seg - 1), H, 2, D, causal=True, boundaries=[-64, -8, 0], q_start=[T - 1] * n_seg, seed=52)
+    d = case.to(dev)
+    d["ko"] = torch.tensor([T * (i % 2) for i in range(n_seg + 1)], dtype=torch.int32, device=dev)
+    a = case.describe()
+    size = C.c_int64()
+    capi.check(capi.lib().dctr_cross_attention_workspace_bytes(C.byref(a), 0, C.byref(size)))
+    assert size.value > 0                                                # (the keys are split)
+    capi.check(case.forward(d))
+    capi.check(case.backward(d))
+    torch.cuda.synchronize()
+    assert d["status"][0].item() == 1 and d["status"][1].item() % 2 == 1
+    for b in range(0, n_seg, 2):
+        alone = AttentionCase(dtype, [1], [T], H, 2, D, causal=True, boundaries=[-64, -8, 0], q_start=[T - 1], seed=1)
+        alone.q, alone.do, alone.k, alone.v, alone.bias = case.q[b:b + 4], case.do[b:b + 4], case.k, case.v, case.bias
+        want = alone.reference() if b in (0, 2, n_seg - 1) else None
+        if want is None:
+            continue
+        got = {n: d[n][b:b + 1].clone() for n in ("out", "lse", "dq")}
+        for n in got:
+            ref, bound = want[n]
+            off = (got[n].cpu().double().view(ref.shape) - ref).abs() - bound
+            assert not (off > 0).any(), (n, b, float(off.max()))
+    assert torch.isfinite(d["out"][:n_seg:2].float()).all() and torch.isfinite(d["lse"][:n_seg:2]).all()
+    assert not d["out"][1:n_seg:2].any() and torch.isinf(d["lse"][1:n_seg:2]).all()

@@ -134,7 +134,7 @@ inline bool attn_solo(const dctr_attention* a, int64_t items) {
 
 // ---- launchers (attention_fwd.hip, attention_bwd.hip): DP = 32, 64 or 128 by head_dim
 // The forward's form for few query rows a key head (splits = 0: the other form).  An item's keys are cut every `each` tiles, into `splits` at most;
-// chunks: no more pairs of segment and cut than these.
+// chunks: no more pairs of segment and cut than these, of segments that do not overlap.
 struct AttnSplit { int row_blocks, splits, each, chunks; bool solo; };
 AttnSplit attn_split(const dctr_attention* a);
 int64_t attn_fwd_blocks(const dctr_attention* a);         // of the call's largest launch

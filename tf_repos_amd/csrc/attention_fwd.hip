@@ -179,11 +179,21 @@ __device__ __forceinline__ int item_tiles(const AttnView& a, const Segment& s, i
 
 // Which segment and which of its cuts chunk c is: a wave counts the segments' cuts, 64 segments at a time.  (A grid of segments x cuts of the
 // longest one would mostly start blocks without work: 3072 for 340 of work in a batch of 48 histories of 1..16384 keys, 57 us against 24.)
-__device__ __forceinline__ bool find_chunk(const AttnView& a, const AttnSplit& cut, int c, int* b, int* sp) {
+// Offsets that descend make segments overlap, and the grid's chunks would not do for all of their cuts: from such a place on, a segment is one cut
+// (each: tiles of a cut).
+__device__ __forceinline__ bool find_chunk(const AttnView& a, const AttnSplit& cut, int c, int* b, int* sp, int* each) {
     const int lane = threadIdx.x & 63;
     int before = 0;
+    bool broken = false;
     for (int b0 = 0; b0 < a.n_seg; b0 += 64) {
-        const int mine = b0 + lane < a.n_seg ? max(1, (segment_keys(a, b0 + lane) + cut.each * SPLIT_KEYS - 1) / (cut.each * SPLIT_KEYS)) : 0;
+        int mine = 0;
+        bool descends = false;
+        if (b0 + lane < a.n_seg) {
+            mine = max(1, (segment_keys(a, b0 + lane) + cut.each * SPLIT_KEYS - 1) / (cut.each * SPLIT_KEYS));
+            descends = a.k_off[b0 + lane + 1] < a.k_off[b0 + lane];
+        }
+        const uint64_t down = __ballot(descends), upto_me = ~0ull >> (63 - lane);
+        if (mine > 0 && (broken || (down & upto_me) != 0)) mine = 1;
         int upto = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -195,14 +205,16 @@ __device__ __forceinline__ bool find_chunk(const AttnView& a, const AttnSplit& c
             const int at = __ffsll((unsigned long long)past) - 1;
             *b = b0 + at;
             *sp = c - before - __shfl(upto - mine, at);
+            *each = broken || (down & (~0ull >> (63 - at))) != 0 ? 1 << 24 : cut.each;         // (> the tiles of DCTR_MAX_POSITION keys)
             return true;
         }
         before += __shfl(upto, 63);
+        broken = broken || down != 0;
     }
     return false;
 }
 
-// part: [item][split][32][DP + 2] (weighted sum, maximum, sum); not used when there is one split, nor of splits behind the item's last tile
+// part: [item][split][32][DP + 2] (weighted sum, maximum, sum), then [item] how many of an item's are written; not used when there is one split
 template <typename T, int DP, bool SOLO>
 __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, DP> <= 192 ? 2 : 1)) void attn_split_kernel(AttnView a, T* out, int64_t out_ld, float* lse, int32_t* status, float* part,
                                                                                               AttnSplit cut) {
@@ -217,7 +229,7 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
     float* stats = reinterpret_cast<float*>(lds + L::first);
     float* hidden = stats + wave * 64;                                  // (in the statistics' place)
     const int64_t items = (int64_t)cut.row_blocks * kv_heads * a.n_seg, at_item = SOLO ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-    int rb, g, b, sp = 0, item;
+    int rb, g, b, sp = 0, item, each = cut.each;
     if (SOLO) {                                                         // (row block slowest: a block's waves are alike long)
         item = (int)min(at_item, items - 1);
         const Item it = item_of(item, kv_heads, a.n_seg);
@@ -227,15 +239,17 @@ __global__ __launch_bounds__(256, (attn_width<T, DP> <= 128 ? 3 : attn_width<T, 
         rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
     } else {
         rb = blockIdx.x % cut.row_blocks, g = blockIdx.x / cut.row_blocks % kv_heads;
-        if (!find_chunk(a, cut, blockIdx.x / cut.row_blocks / kv_heads, &b, &sp)) return;
+        if (!find_chunk(a, cut, blockIdx.x / cut.row_blocks / kv_heads, &b, &sp, &each)) return;
         item = (b * kv_heads + g) * cut.row_blocks + rb;
     }
     const Segment s = load_segment(a, b);
     if (rb == 0 && g == 0 && sp == 0 && (SOLO ? lane : tid) == 0) flag_segment(a, b, status);
     const int rows = s.nq * a.group, r0 = rb * 32;
-    const int tiles = item_tiles(a, s, rb), t0 = sp * cut.each, t1 = cut.splits == 1 ? tiles : min(tiles, t0 + cut.each);
+    const int tiles = item_tiles(a, s, rb), t0 = sp * each, t1 = cut.splits == 1 ? tiles : min(tiles, t0 + each);
     const bool none = r0 >= rows || (SOLO && at_item >= items);
     if (!SOLO && (none || (sp > 0 && t0 >= tiles))) return;
+    if (!SOLO && cut.splits > 1 && sp == 0 && tid == 0)
+        reinterpret_cast<int32_t*>(part + items * cut.splits * 32 * (DP + 2))[item] = max(1, (tiles + each - 1) / each);
     const int r = r0 + (lane & 31), i = r / a.group, hg = r % a.group, h = g * a.group + hg;
     const int chunks = a.dim / Tile<M, DP>::PER;
     const float scale = fabsf(a.scale) * LOG2E;
@@ -338,10 +352,10 @@ template <typename T, int DP>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnView a, T* out, int64_t out_ld, float* lse, const float* part, AttnSplit cut) {
     const int lane = threadIdx.x & 63, kv_heads = a.heads / a.group, item = blockIdx.x >> 3, r = (blockIdx.x & 7) * 4 + (threadIdx.x >> 6);
     const int rb = item % cut.row_blocks, g = item / cut.row_blocks % kv_heads, b = item / cut.row_blocks / kv_heads;
+    const int splits = reinterpret_cast<const int32_t*>(part + (int64_t)cut.row_blocks * kv_heads * a.n_seg * cut.splits * 32 * (DP + 2))[item];
     const Segment s = load_segment(a, b);
     const int mine = rb * 32 + r;
     if (mine >= s.nq * a.group) return;
-    const int splits = max(1, (item_tiles(a, s, rb) + cut.each - 1) / cut.each);                                 // that have left a part
     const int64_t step = 32 * (DP + 2);
     const float* p = part + ((int64_t)item * cut.splits * 32 + r) * (DP + 2);
     float m = -INFINITY;
@@ -403,7 +417,8 @@ AttnSplit attn_split(const dctr_attention* a) {
     const int64_t items = (int64_t)c.row_blocks * a->kv_heads * a->n_seg, tiles = (a->max_k + SPLIT_KEYS - 1) / SPLIT_KEYS;
     c.solo = attn_solo(a, items);
     if (c.solo || items == 0 || items > 4096) return c;
-    // cuts of 512 keys (4 tiles a wave: about 1 us each, after 5 us for a block's start and its join), longer ones where the parts would pass 64 MB
+    // cuts of 512 keys (4 tiles a wave: about 1 us each, after 5 us for a block's start and its join), longer ones where there would be more than 8192
+    // parts (136 MB of heads of 128, 69 of 64, 36 of 32)
     const int64_t most = std::min<int64_t>((tiles + SPLIT_TILES - 1) / SPLIT_TILES, std::max<int64_t>(1, 8192 / items));
     if (most <= 1) return c;
     c.each = (int)((tiles + most - 1) / most);
@@ -457,7 +472,7 @@ int64_t attn_fwd_blocks(const dctr_attention* a) {
 
 int64_t attn_fwd_workspace(const dctr_attention* a) {
     const AttnSplit cut = attn_split(a);
-    return cut.splits > 1 ? (int64_t)cut.row_blocks * a->kv_heads * a->n_seg * cut.splits * 32 * (padded(a->head_dim) + 2) * (int64_t)sizeof(float) : 0;
+    return cut.splits > 1 ? (int64_t)cut.row_blocks * a->kv_heads * a->n_seg * (cut.splits * 32 * (padded(a->head_dim) + 2) + 1) * (int64_t)sizeof(float) : 0;
 }
 
 int attn_fwd(const dctr_attention* a, const AttnView& v, void* out, int64_t out_ld, float* lse, int32_t* status, float* ws, hipStream_t st) {
