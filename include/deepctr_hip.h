@@ -451,7 +451,8 @@ typedef struct dctr_attention {
 /* Key j of a segment is at position j, query i at d_q_start[b] + i (d_q_start null: at i).  Scores
  *     s_ij = scale <q_i, k_j> + d_rel_bias[bucket(j - q_start - i), h]      over the keys with d_key_keep[row] != 0 (null: all) that a causal
  * query sees; out_i = sum_j softmax(s)_ij v_j, d_lse[row, h] = log sum_j exp(s_ij) (may be null).  A query that sees no key: out 0, lse -inf.
- * Rows outside every segment are neither read nor written; what a key that is not kept holds (inf, NaN) reaches nothing.
+ * Rows outside every segment are neither read nor written; what a key that is not kept holds (inf, NaN) reaches nothing.  A bias of -inf, or below what f32
+ * holds times log2(e) (-2.3e38: the type's lowest value is), hides its bucket's keys from that head.
  *   d_q [total_q, heads * head_dim], d_k / d_v [total_k, kv_heads * head_dim]; row strides *_ld in elements; rows 16-byte aligned
  *   d_q_offsets / d_k_offsets int32 [n_seg + 1]; d_q_start int32 [n_seg] or null; d_rel_bias f32 [n_buckets, heads]
  *   d_status int32[2] or null: [0] = 1, [1] = b if segment b's offsets leave the arrays, descend, or hold more than max_q / max_k rows
@@ -466,7 +467,8 @@ int dctr_cross_attention_fwd(const dctr_attention* a, const void* d_q, int q_ld,
                              void* d_workspace, size_t workspace_bytes, void* stream);
 /* gradients of the same call: d_dout = dL/dout in; dL/dq, dL/dk, dL/dv (shared key heads: summed over their query heads) and dL/d rel_bias
  * [n_buckets, heads] f32 (null: not wanted) overwritten -- 0 where nothing contributes.  d_out, d_lse: the forward's.  d_dout has
- * to be finite in every row of a segment, also where the query saw no key.  Sums run in a fixed order: the same call gives the same bits. */
+ * to be finite in every row of a segment, also where the query saw no key.  The weights are formed again from d_lse, as exactly as f32 holds scores of its
+ * size (2^-24 |lse|); a query with lse < -1e7 -- it sees only keys whose bias is a mask like -1e9 -- passes on no gradient.  Sums run in a fixed order: the same call gives the same bits. */
 int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld, const void* d_k, int k_ld, const void* d_v, int v_ld,
                              const int32_t* d_q_offsets, const int32_t* d_k_offsets, const int32_t* d_q_start, const uint8_t* d_key_keep,
                              const float* d_rel_bias, const void* d_out, int out_ld, const float* d_lse, const void* d_dout,

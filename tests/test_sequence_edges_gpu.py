@@ -1,5 +1,6 @@
 """The sequence operators at the edges of what their calls allow."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -78,3 +79,34 @@ def test_overlapping_segments_of_descending_offsets_in_the_split_form(dtype, n_s
             assert not (off > 0).any(), (n, b, float(off.max()))
     assert torch.isfinite(d["out"][:n_seg:2].float()).all() and torch.isfinite(d["lse"][:n_seg:2]).all()
     assert not d["out"][1:n_seg:2].any() and torch.isinf(d["lse"][1:n_seg:2]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("mask", [-math.inf, torch.finfo(torch.float32).min, -1e38, -1e9, -1e8])
+@pytest.mark.parametrize("n_seg,q,k,heads,dim", [(3, 40, 90, 2, 32), (20, 200, 300, 8, 64), (20, 200, 300, 8, 128), (300, 20, 40, 4, 16)])
+def test_biases_that_mask_a_bucket(dtype, mask, n_seg, q, k, heads, dim, dev):
+    """Buckets of one head whose bias is -inf, the type's lowest value or a large negative number, and queries that see nothing else: every gradient is that
+    of the buckets hidden, finite, and none comes from the queries that see nothing."""
+    lens = [max(1, q - 7 * i % q) for i in range(n_seg)], [max(1, k - 11 * i % k) for i in range(n_seg)]
+    case = AttentionCase(dtype, *lens, heads, heads, dim, boundaries=[-20, 5], q_start=[10 if i % 3 else k + 100 for i in range(n_seg)], seed=53)
+    case.bias[0, 1] = -math.inf                                         # (of the reference; the queries of every third segment see bucket 0 only)
+    ref = case.reference()
+    case.bias[0, 1] = mask
+    d = case.to(dev)
+    capi.check(case.forward(d))
+    hidden = torch.zeros(case.nq, heads, dtype=torch.bool)
+    hidden[:, 1] = torch.isinf(ref["lse"][0][:, 1])
+    assert hidden.any() and not hidden[:, 1].all()
+    lse, out = d["lse"][:case.nq].cpu(), d["out"][:case.nq, :heads * dim].float().cpu().view(case.nq, heads, dim)
+    assert torch.isfinite(out).all() and not torch.isnan(lse).any()
+    if mask < -2.4e38:
+        assert torch.isinf(lse[hidden]).all() and not out[hidden].any()
+    else:                                                               # (such a query sees keys of one and the same bias: lse is that bias, to f32's place)
+        assert ((lse[hidden] / mask - 1).abs() < 1e-6).all()
+        d["lse"][:case.nq][hidden.to(dev)] = -math.inf                  # (for the comparison of the others)
+        d["out"][:case.nq, :heads * dim].view(case.nq, heads, dim)[hidden.to(dev)] = 0.0
+    case.check(d, ("out", "lse"), ref)
+    capi.check(case.forward(d))
+    capi.check(case.backward(d))
+    torch.cuda.synchronize()
+    case.check(d, ("dq", "dk", "dv", "db"), ref)

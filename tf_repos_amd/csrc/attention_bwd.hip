@@ -15,6 +15,12 @@ namespace dctr {
 
 constexpr int BWD_THREADS = 256;
 
+// -log2(e) lse, the addend of a row's exponents: -inf where there is nothing to form again.  A row that saw nothing has lse = -inf.  One that saw only keys of
+// biases like -1e9 has an lse whose last place is worth more than its weights (2^-24 of 1e7 is 0.6): exponents off by whole units, up to
+// infinite weights, would reach the gradients of every key it sees, so it passes on none.
+constexpr float LEAST_LSE = -1e7f;
+__device__ __forceinline__ float minus_log2(float lse) { return lse < LEAST_LSE ? -INFINITY : -LOG2E * lse; }
+
 // Query-side forms: ROWS a block's waves take 32 rows each and share 64-key tiles; SPLIT the waves take 32-key tiles of their own of the same 32
 // rows and add up at the end; SOLO a wave has 32 rows to itself.
 enum { ROWS = 0, SPLIT = 1, SOLO = 2 };
@@ -130,8 +136,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
         dl = both_sum(dl);
         if (!ROUNDED && (lane & 1)) go.negate();
         if (row < s.nq) {
-            const float L = lse[(s.q0 + row) * a.heads + h];
-            if (L != -INFINITY) minus_lse = -LOG2E * L;
+            minus_lse = minus_log2(lse[(s.q0 + row) * a.heads + h]);
             if (!ROUNDED && (FORM != SPLIT || wave == 0) && half == 0) delta[(s.q0 + row) * a.heads + h] = dl;
         }
     }
@@ -506,7 +511,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
         qs.land(qt + buf * TILE, loader, first_rows(s.nq - i0));
         gs.land(gt + buf * TILE, loader, first_rows(s.nq - i0));
         if (loader < QT) {
-            stats[buf * 2 * QT + loader] = lv == -INFINITY ? -INFINITY : -LOG2E * lv;        // p = 2^-inf = 0 for a row that saw nothing, and behind the last row
+            stats[buf * 2 * QT + loader] = minus_log2(lv);              // p = 2^-inf = 0 for a row that saw nothing, and behind the last row
             stats[buf * 2 * QT + QT + loader] = dv_;
         }
     };
