@@ -429,7 +429,11 @@ int dctr_dcn_cross_bwd(const float* d_xs, const float* d_xlw, const float* d_w, 
  * Beyond DIN's sigmoid-scored pooling of a behaviour list (DIN.py:152-172) and the binary loss heads: multi-head softmax attention of any
  * number of queries per example (candidate ads, a sequence's own steps, one new event) over that example's history, with a learned bias per
  * bucket of the distance between them, and the cross entropy of rows against every row of an item table.  Types: F32, or BF16 with all
- * sums, softmax statistics, biases, their gradients and losses in f32. */
+ * sums, softmax statistics, biases, their gradients and losses in f32; for BF16 the matrix unit's second operands are rounded to it (half a step, 2^-8 of
+ * each): the weights before they meet v, k or dout, the scores' gradients before k and q, the loss's weights before x and the table.
+ * Elements that take part are finite, in F32 at most 3.38e38 (bfloat16's largest: F32 arrays go through the matrix unit in bfloat16 planes, which makes NaN
+ * of more).  An infinite or NaN element of a query's row stays with that query's outputs; one of a key's row reaches the queries of its segment,
+ * also those before it in causal order; what is masked (keys not kept, rows without a label) may hold anything. */
 enum { DCTR_TYPE_F32 = 0, DCTR_TYPE_BF16 = 1 };
 #define DCTR_MAX_REL_BUCKETS 128
 #define DCTR_MAX_REL_SPAN 1025         /* last boundary - first boundary: steps of up to 512 on either side, -512 .. 513 */
@@ -480,7 +484,8 @@ int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld,
  * (int32[2] or null: [0] = 1, [1] = the label).  Gradients are of  sum_n scale * d_row_scale[n] * loss_n  (d_row_scale f32 [N] or null = 1;
  * scale = 1/batch for a mean).  d_x [N, D], d_w [V, D] and the gradients in `dtype`, rows 16-byte aligned, D a multiple of 8, 8..256.
  *   fwd: loss, lse and, d_dx not null, dL/dx [N, dx_ld] from the same pass over the table
- *   bwd_weights: dL/dw [V, dw_ld] and (may be null) dL/db f32 [V], overwritten; d_lse: the forward's
+ *   bwd_weights: dL/dw [V, dw_ld] and (may be null) dL/db f32 [V], overwritten; d_lse: the forward's.  The label's 1 - p is taken from d_lse here: off by
+ *                about 2^-23 |lse|, where loss and dx keep its leading digits however sure the model is
  * d_workspace: dctr_vocab_softmax_workspace_bytes(dtype, N, V, D, train) bytes (0: fwd without dx; 1: enough for all three), as above. */
 int dctr_vocab_softmax_workspace_bytes(int dtype, int N, int64_t V, int D, int train, int64_t* bytes);
 int dctr_vocab_softmax_fwd(int dtype, const void* d_x, int x_ld, const void* d_w, int w_ld, const float* d_b, const int32_t* d_labels, int N,

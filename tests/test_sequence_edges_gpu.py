@@ -110,3 +110,71 @@ def test_biases_that_mask_a_bucket(dtype, mask, n_seg, q, k, heads, dim, dev):
     capi.check(case.backward(d))
     torch.cuda.synchronize()
     case.check(d, ("dq", "dk", "dv", "db"), ref)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n_seg,q,k,heads,dim", [(3, 40, 90, 2, 32), (20, 200, 300, 8, 64), (20, 200, 300, 8, 128), (300, 20, 40, 4, 16), (4, 1, 900, 2, 64)])
+def test_infinities_stay_where_they_are_seen(dtype, n_seg, q, k, heads, dim, dev):
+    """One query's row holds inf and one other segment's key row NaN: the outputs of every other query, and the gradients of every other segment, are the
+    bits they were."""
+    lens = [max(1, q - 7 * i % q) for i in range(n_seg)], [max(1, k - 11 * i % k) for i in range(n_seg)]
+    case = AttentionCase(dtype, *lens, heads, heads, dim, boundaries=[-20, 5], q_start=[5] * n_seg, seed=54)
+    clean, spoilt = case.to(dev), case.to(dev)
+    qo, ko = clean["qo"].tolist(), clean["ko"].tolist()
+    row, col = qo[1], slice(dim, 2 * dim)                               # the first query of segment 1, its second head
+    spoilt["q"][row, col] = math.inf
+    spoilt["k"][ko[2] + 1, col] = math.nan
+    spoilt["v"][ko[2] + 1, col] = math.inf
+    for d in (clean, spoilt):
+        capi.check(case.forward(d))
+        capi.check(case.backward(d))
+    torch.cuda.synchronize()
+    away = torch.ones(case.nq, dtype=torch.bool, device=dev)
+    away[row] = False
+    away[qo[2]:qo[3]] = False
+    for n in ("out", "lse", "dq"):
+        assert torch.equal(clean[n][:case.nq][away], spoilt[n][:case.nq][away]), n
+    other = torch.ones(case.nk, dtype=torch.bool, device=dev)
+    other[ko[1]:ko[3]] = False
+    for n in ("dk", "dv"):
+        assert torch.equal(clean[n][:case.nk][other], spoilt[n][:case.nk][other]), n
+    for n in ("out", "dq", "dk", "dv"):                                  # ... and the other head's columns anywhere
+        assert torch.equal(clean[n][:, :dim], spoilt[n][:, :dim]), n
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,dim", [(20, 500, 32), (150, 700, 64), (150, 700, 200), (9, 40000, 128)])
+def test_rows_without_a_label_may_hold_anything(dtype, rows, vocab, dim, dev):
+    case = VocabCase(dtype, rows, vocab, dim, row_scale=True, unlabelled=0.3, seed=55)
+    none = case.labels < 0
+    assert none.any() and not none.all()
+    clean, spoilt = case.to(dev), case.to(dev)
+    at = none.nonzero().flatten().to(dev)
+    spoilt["x"][at[0::2]], spoilt["x"][at[1::2]] = math.inf, math.nan
+    spoilt["row_scale"][at] = math.nan
+    for d in (clean, spoilt):
+        capi.check(case.forward(d))
+        capi.check(case.backward(d))
+    torch.cuda.synchronize()
+    case.check(clean, ("loss", "lse", "dx", "dw", "db"))
+    for n in ("loss", "dx", "dw", "db"):
+        assert torch.equal(clean[n], spoilt[n]), n
+    assert torch.equal(clean["lse"][:rows][~none.to(dev)], spoilt["lse"][:rows][~none.to(dev)])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [5, 150])
+def test_without_the_bias_gradient_and_lse(dtype, rows, dev):
+    """A bias without its gradient, a forward without lse: the rest is the same, bit by bit."""
+    case = VocabCase(dtype, rows, 3000, 40, seed=56)
+    full, part = case.to(dev), case.to(dev)
+    capi.check(case.forward(full))
+    capi.check(case.backward(full))
+    p = capi.ptr
+    capi.check(capi.lib().dctr_vocab_softmax_fwd(*case.ins(part), p(part["loss"]), None, p(part["dx"]), case.ld, None, p(part["ws1"]), part["bytes1"],
+                                                 capi.current_stream()))
+    capi.check(capi.lib().dctr_vocab_softmax_bwd_weights(*case.ins(part), p(full["lse"]), p(part["dw"]), case.ld, None, p(part["ws1"]), part["bytes1"],
+                                                         capi.current_stream()))
+    torch.cuda.synchronize()
+    for n in ("loss", "dx", "dw"):
+        assert torch.equal(full[n], part[n]), n
