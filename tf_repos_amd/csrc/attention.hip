@@ -2,17 +2,13 @@
 #include <cmath>
 
 #include "attention.h"
+#include "ops.h"
 
 namespace dctr {
 
 __global__ void attn_check_kernel(AttnView a, int32_t* status) {
     const int b = blockIdx.x * 256 + threadIdx.x;
     if (b < a.n_seg) flag_segment(a, b, status);
-}
-
-__global__ void fill_zero_kernel(float* x, int n) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n) x[i] = 0.f;
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------------
@@ -137,8 +133,7 @@ int dctr_cross_attention_bwd(const dctr_attention* a, const void* d_q, int q_ld,
     DCTR_TRY(check_workspace(a, 1, d_workspace, workspace_bytes));
     hipStream_t st = as_stream(stream);
     if (a->n_buckets > 0 && d_drel_bias != nullptr && (a->n_seg == 0 || a->total_q == 0 || a->max_q == 0)) {
-        fill_zero_kernel<<<ceil_div(a->n_buckets * a->heads, 256), 256, 0, st>>>(d_drel_bias, a->n_buckets * a->heads);
-        DCTR_LAUNCH_CHECK();
+        DCTR_TRY(zero_words(d_drel_bias, (size_t)a->n_buckets * a->heads, st));
         d_drel_bias = nullptr;
     }
     if (a->n_seg == 0) return DCTR_OK;

@@ -442,8 +442,9 @@ static int launch_fwd(const dctr_attention* a, const AttnView& v, void* out, int
     const int64_t items = (int64_t)cut.row_blocks * a->kv_heads * a->n_seg;
     if (items == 0) return DCTR_OK;
     using L = SplitLds<T, DP>;
+    constexpr bool wide = sizeof(T) == 4 && DP > 64;                    // (attn_solo: never)
     if (cut.solo)
-        attn_split_kernel<T, DP, true><<<ceil_div(items, 4), 256, L::first + L::stats + lut + 4 * table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
+        attn_split_kernel<T, DP, !wide><<<ceil_div(items, 4), 256, L::first + L::stats + lut + 4 * table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     else
         attn_split_kernel<T, DP, false><<<(unsigned)(cut.splits > 1 ? items / a->n_seg * cut.chunks : items), 256, L::first + L::stats + lut + table, st>>>(v, (T*)out, out_ld, lse, status, ws, cut);
     DCTR_LAUNCH_CHECK();
