@@ -40,6 +40,17 @@ int zero_words(void* p, size_t n, hipStream_t st) {
 
 using namespace dctr;
 
+// 16-byte stores between the first and the last aligned address, bytes at the ends
+__global__ __launch_bounds__(256) void fill_bytes_kernel(uint8_t* p, uint8_t value, size_t n) {
+    const size_t head = min((size_t)(-reinterpret_cast<uintptr_t>(p) & 15), n), mid = (n - head) / 16, tail = head + 16 * mid;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, step = (size_t)gridDim.x * 256;
+    const uint32_t w = value * 0x01010101u;
+    uint4* q = reinterpret_cast<uint4*>(p + head);
+    for (size_t k = i; k < mid; k += step) q[k] = make_uint4(w, w, w, w);
+    if (i < head) p[i] = value;
+    if (i < n - tail) p[tail + i] = value;
+}
+
 // streaming float4 copy: the "measured HBM roofline" the gather / optimizer fractions are quoted against
 // (one float4 per lane and a grid that covers the buffer: measured 6.2 TB/s; grid-stride variants of the same copy reach 4.4)
 __global__ __launch_bounds__(256) void copy_f4_kernel(const float4* __restrict__ src, float4* __restrict__ dst, size_t n4) {
@@ -113,8 +124,12 @@ int dctr_memcpy_d2h(void* h_dst, const void* d_src, size_t nbytes, void* stream)
     DCTR_HIP_CHECK(hipStreamSynchronize(as_stream(stream)));
     return DCTR_OK;
 }
-int dctr_memset(void* d_dst, int value, size_t nbytes, void* stream) {
-    DCTR_HIP_CHECK(hipMemsetAsync(d_dst, value, nbytes, as_stream(stream)));
+int dctr_memset(void* d_dst, int value, size_t nbytes, void* stream) {         // (a kernel: the caller may capture it, see zero_words)
+    if (nbytes == 0) return DCTR_OK;
+    DCTR_REQUIRE(d_dst != nullptr, "null pointer");
+    const size_t blocks = nbytes / 4096 + 1;
+    fill_bytes_kernel<<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, as_stream(stream)>>>(static_cast<uint8_t*>(d_dst), (uint8_t)value, nbytes);
+    DCTR_LAUNCH_CHECK();
     return DCTR_OK;
 }
 int dctr_stream_sync(void* stream) {

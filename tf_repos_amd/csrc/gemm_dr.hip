@@ -404,7 +404,7 @@ int opnn_outer_wgrad(const float* e, int e_ld, int B, int F, int K, const int* p
     DCTR_REQUIRE(opnn_fused_ok(F, K, H) && al16(e) && al16(dy) && al16(dw_outer) && (e_ld & 3) == 0 && (lddy & 3) == 0 && fits31(B, e_ld) && fits31(B, lddy),
                  "opnn_outer_wgrad: unsupported shape / alignment");
     const int L = F * (F - 1) / 2 * K * K;
-    if (B <= 0) { DCTR_HIP_CHECK(hipMemsetAsync(dw_outer, 0, (size_t)L * H * sizeof(float), st)); return DCTR_OK; }
+    if (B <= 0) return zero_words(dw_outer, (size_t)L * H, st);
     DrOuter og{e, e_ld, B, pairs, 31 - __builtin_clz((unsigned)K)};
     const int R = (int)round_up(B, 64);
     if (H > 208) return dr_launch_outer<16, DR_AGEN_OUTER_WGRAD>(og, dy, lddy, dw_outer, H, L, H, R, 1, 0, st);
