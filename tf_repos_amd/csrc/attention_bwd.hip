@@ -4,8 +4,8 @@
 //               the bias gradient's sums over a tile's diagonals
 //   key side    S = Q K^T and dP = dO V^T by 32 keys a wave, over the queries of every head of the group: dV^T += dO^T P, dK^T += Q^T dS
 // p and ds are rounded to bf16 for the second products of bf16 arrays, half a step each, as the results are; everything that is summed is f32.
-// Measured on 16 segments of 1024 x 1024, 8 heads, bf16: query side 91 us at 64 wide (755 TF/s of its four products) and 242 at 128 (567), key side 97
-// (712) and 248 (554): at 128 the accumulators leave one wave a SIMD, whose exponents then run beside nothing.  f32 in planes at 64: 272 and 429 us.
+// Measured on 16 segments of 1024 x 1024, 8 heads, bf16: query side 92 us at 64 wide (747 TF/s of its four products) and 235 at 128 (584), key side 98
+// (703) and 240 (573): at 128 the accumulators leave one wave a SIMD, whose exponents then run beside nothing.  f32 in planes at 64: 272 and 428 us.
 // 512 segments of up to 40 x 200, 4 heads of 16, f32 with a bias: 37 and 35 us, the latency of each wave's few tiles and of its bias tables.
 #include <cmath>
 

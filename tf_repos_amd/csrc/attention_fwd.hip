@@ -27,8 +27,8 @@ __device__ __forceinline__ void write_rows(const AttnView& a, const Softmax<M, D
 
 // ---- row form ------------------------------------------------------------------------------------------------------------------------
 // 32 rows a wave, 128 a block, whose waves share the tiles of K and V (two buffers, loaded straight into shared memory).  Bound by the softmax's vector
-// work and the power that it and the matrix unit draw together: 16 segments of 1024 x 1024, 8 heads, bf16: 687 TF/s at 128 wide (99 us), 551 at 64
-// (62 us); f32 in planes at 64 173 TF/s (199 us), f32 instructions at 128 98 (700 us).  Of few and uneven segments the longest list's chain of tiles is
+// work and the power that it and the matrix unit draw together: 16 segments of 1024 x 1024, 8 heads, bf16: 713 TF/s at 128 wide (96 us), 538 at 64
+// (64 us); f32 in planes at 64 170 TF/s (202 us), f32 instructions at 128 98 (704 us).  Of few and uneven segments the longest list's chain of tiles is
 // what takes the time: 2.2 us a tile of 64 keys at 128 wide.
 constexpr int ROWS_THREADS = 256;
 template <typename T, int DP>
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(ROWS_THREADS, (attn_width<T, DP> <= 384 ? 2 : 1)) v
 // ---- split form, solo form -----------------------------------------------------------------------------------------------------------
 // An item is 32 (query, head of the group) rows of a segment and key head.  Split: the block's waves, and the blocks of an item, share its keys.
 // Solo: a wave has an item to itself, nothing to join and nobody to wait for -- for short lists in number.
-// One query an item (serving) reads each key once: 48 histories of up to 16384 keys, 64 MB, 20 us (3.2 TB/s) and 5.5 for the join, the rest the launch
+// One query an item (serving) reads each key once: 48 histories of up to 16384 keys, 64 MB, 21 us (3.0 TB/s) and 5.3 for the join, the rest the launch
 // and the first loads; a single short item takes 6 us, which is the latency of four dependent reads and the code's own first fetch.
 constexpr int SPLIT_KEYS = 32, SPLIT_TILES = 16;                       // keys of a wave's tile, tiles below which an item is not split
 // shared memory: 4 waves' K and V tiles, in whose place the waves' results meet (rows of DP + 4 floats: no two rows start at the same bank)

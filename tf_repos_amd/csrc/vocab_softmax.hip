@@ -42,7 +42,7 @@ struct VocabTile {
     using M = VocabKind<T, DP>;
     static constexpr int WIDTH = Mma<M>::BYTES * DP, ROWS = WIDTH <= 384 ? 64 : 32, NB = ROWS / 32, SIZE = ROWS * Tile<M, DP>::STRIDE;
     static constexpr size_t bytes = (size_t)ROWS * WIDTH;
-    static constexpr bool LEAD = WIDTH == 512;                          // bf16 of 256, a wave a SIMD (rows of 2048 x 100000: 445 us, 430 with; f32 the same)
+    static constexpr bool LEAD = WIDTH == 512;                          // bf16 of 256, a wave a SIMD (rows of 2048 x 100000: 3 % longer without; f32 the same)
 };
 
 // Bias and hidden columns (behind the table, the row's label) of a wave's 32 rows' scores against NB * 32 table rows from v0 on; returns the factor
@@ -90,9 +90,9 @@ __device__ __forceinline__ void write_parts(const VocabParts& p, int sp, int N, 
 }
 
 // 4 waves of 32 rows share the table's tiles, three buffers: while a tile is weighed, the scores of the next one are formed under its exponents and
-// the one after that is on its way.  Bound by the matrix unit and the exponents beside it: bf16 2048 x 1000000 x 64 with dx 749 us (700 TF/s of its two
-// products), 2048 x 100000 x 256 430 us (490: one wave a SIMD); f32 in planes 4096 x 117581 x 64 without dx, the whole call: 373 us (165 TF/s; a large
-// f32 matrix product of the library runs at 154).
+// the one after that is on its way.  Bound by the matrix unit and the exponents beside it: bf16 2048 x 1000000 x 64 with dx 697 us (752 TF/s of its two
+// products), 2048 x 100000 x 256 342 us (613: one wave a SIMD); f32 in planes 4096 x 117581 x 64 without dx, the whole call: 379 us (163 TF/s; a large
+// f32 matrix product of the library runs at 153).
 template <typename T, int DP, bool DX>
 __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= (DX ? 384 : 512) ? 2 : 1)) void vocab_rows_kernel(VocabView a, VocabParts p, int row_blocks) {
     extern __shared__ __attribute__((aligned(TILE_ALIGN))) char lds[];
@@ -297,9 +297,9 @@ __global__ __launch_bounds__(VS_THREADS) void vocab_join_kernel(VocabView a, Voc
 }
 
 // ---- dw, db: 32 table rows a wave, over the rows of x ---------------------------------------------------------------------------------
-// bf16 2048 x 1000000 x 64: 617 us (850 TF/s of two products); 2048 x 100000 x 256: 370 us (567).  f32 in planes 1024 x 117581 x 64: 170 us (181 TF/s).
+// bf16 2048 x 1000000 x 64: 600 us (874 TF/s of two products); 2048 x 100000 x 256: 352 us (596).  f32 in planes 1024 x 117581 x 64: 178 us (173 TF/s).
 // With more than one split (a short vocabulary): part [splits][V][DP], part_b [splits][V], joined by vocab_dw_join_kernel.
-// (bf16 of 256: two waves a SIMD at the price of 13 spilled registers, 2048 x 100000: 510 us -> 370; the rows kernel would spill 110: 430 -> 514)
+// (bf16 of 256: two waves a SIMD at the price of 13 spilled registers take 2048 x 100000 in 0.73 of the time; the rows kernel would spill 110 and take 1.2 times its)
 template <typename T, int DP>
 __global__ __launch_bounds__(VS_THREADS, (VocabTile<T, DP>::WIDTH <= 256 || VocabTile<T, DP>::WIDTH == 512 ? 2 : 1)) void vocab_dw_kernel(VocabView a, const float* lse, T* dw, int64_t dw_ld, float* db, float* part, float* part_b,
                                                               int splits, int each, int table_blocks) {
