@@ -126,7 +126,13 @@ int dctr_memcpy_d2h(void* h_dst, const void* d_src, size_t nbytes, void* stream)
 }
 int dctr_memset(void* d_dst, int value, size_t nbytes, void* stream) {         // (a kernel: the caller may capture it, see zero_words)
     if (nbytes == 0) return DCTR_OK;
-    DCTR_REQUIRE(d_dst != nullptr, "null pointer");
+    hipDeviceptr_t base = nullptr;
+    size_t size = 0;
+    if (hipMemGetAddressRange(&base, &size, d_dst) != hipSuccess || static_cast<char*>(d_dst) + nbytes > static_cast<char*>(base) + size) {
+        (void)hipGetLastError();                                        // not within one device allocation: the runtime knows what it is
+        DCTR_HIP_CHECK(hipMemsetAsync(d_dst, value, nbytes, as_stream(stream)));
+        return DCTR_OK;
+    }
     const size_t blocks = nbytes / 4096 + 1;
     fill_bytes_kernel<<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, as_stream(stream)>>>(static_cast<uint8_t*>(d_dst), (uint8_t)value, nbytes);
     DCTR_LAUNCH_CHECK();
