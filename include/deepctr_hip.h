@@ -539,7 +539,8 @@ int dctr_get_global_step(dctr_handle h, int64_t* step);
 
 /* one optimizer step on one batch: forward, loss, backward, optimizer (DeepFM.py:125-213).
  * d_ids/d_vals/d_labels are device pointers ([B,F] i32, [B,F] f32, [B] f32).  h_loss (may be NULL)
- * receives the full loss of DeepFM.py:188-190 evaluated BEFORE the update; passing it forces a sync. */
+ * receives the full loss of DeepFM.py:188-190 evaluated BEFORE the update; passing it forces a sync.  A stream that is being captured is
+ * refused (dctr_config.use_graph replays steps from graphs of the handle's own). */
 int dctr_train_step(dctr_handle h, const int32_t* d_ids, const float* d_vals, const float* d_labels,
                     int B, float* h_loss, void* stream);
 /* Engine-owned input staging: DCTR_INPUT_SLOTS sets of ([max_batch,F] i32, [max_batch,F] f32, [max_batch] f32) device

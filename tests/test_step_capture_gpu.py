@@ -52,3 +52,31 @@ def test_replayed_steps_equal_eager_steps(B, period, hint, dev):
     assert abs(states[0][0] - states[1][0]) <= 1e-4 * abs(states[0][0])
     for k, v in states[0][1].items():
         assert np.abs(v - states[1][1][k]).mean() <= 1e-5, k
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_a_step_in_a_callers_capture_is_refused(use_graph, dev):
+    """... with an error, and the handle goes on as if it had not been asked."""
+    from tests.util import make_pair
+    from tf_repos_amd import errors
+    B, F, V = 128, 39, 3000
+    runs = []
+    for ask in (False, True):
+        _, _, eng = make_pair("deepfm", B=B, F=F, V=V, opt="Adam", seed=5, use_graph=use_graph)
+        batch = dev_batch(*O.synth_batch(B, F, V, seed=8), dev)
+        losses = [eng.train_step(*batch)]
+        if ask:
+            s, g, x = torch.cuda.Stream(), torch.cuda.CUDAGraph(), torch.zeros(4, device=dev)
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g, stream=s):
+                x.add_(1.0)
+                with pytest.raises(errors.InvalidArgumentError, match="captured"):
+                    eng.train_step(*batch, want_loss=False)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.all(x == 1.0)
+        losses.append(eng.train_step(*batch))
+        assert eng.global_step == 2
+        runs.append(losses)
+        eng.close()
+    assert np.allclose(runs[0], runs[1], rtol=0, atol=1e-6)

@@ -1785,10 +1785,19 @@ int dctr_get_global_step(dctr_handle E, int64_t* step) {
     return DCTR_OK;
 }
 
+// A step takes side streams, records that ride on launches and host-side state along, none of which a caller's capture records.
+static int refuse_capture(hipStream_t st) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (st != nullptr && hipStreamIsCapturing(st, &status) == hipSuccess)
+        DCTR_REQUIRE(status == hipStreamCaptureStatusNone, "a training step cannot be captured by its caller (dctr_config.use_graph captures it)");
+    return DCTR_OK;
+}
+
 int dctr_train_step(dctr_handle E, const int32_t* d_ids, const float* d_vals, const float* d_labels, int B, float* h_loss,
                     void* stream) {
     DCTR_REQUIRE(E && d_ids && d_vals && d_labels, "null argument");
     DCTR_REQUIRE(!E->csr, "this handle's model takes CSR batches (dctr_train_step_csr)");
+    DCTR_TRY(refuse_capture(as_stream(stream)));
     hipStream_t st = as_stream(stream);
     DCTR_TRY(stage_inputs(E, d_ids, d_vals, d_labels, B, st));
     E->want_loss = h_loss != nullptr;
@@ -2035,6 +2044,7 @@ extern "C" {
 int dctr_train_step_csr(dctr_handle E, const int32_t* d_offsets, const int32_t* d_ids, const float* d_weights, int nnz,
                         const float* d_y, const float* d_z, int B, float* h_loss, void* stream) {
     DCTR_TRY(csr_check(E, d_offsets, d_ids, nnz, B));
+    DCTR_TRY(refuse_capture(as_stream(stream)));
     const dctr_config& c = E->cfg;
     const bool esmm = c.model == DCTR_MODEL_ESMM;
     DCTR_REQUIRE(d_y != nullptr && (!esmm || d_z != nullptr), "labels missing (ESMM takes y and z)");
