@@ -430,7 +430,8 @@ int dctr_dcn_cross_bwd(const float* d_xs, const float* d_xlw, const float* d_w, 
  * number of queries per example (candidate ads, a sequence's own steps, one new event) over that example's history, with a learned bias per
  * bucket of the distance between them, and the cross entropy of rows against every row of an item table.  Types: F32, or BF16 with all
  * sums, softmax statistics, biases, their gradients and losses in f32; for BF16 the matrix unit's second operands are rounded to it (half a step, 2^-8 of
- * each): the weights before they meet v, k or dout, the scores' gradients before k and q, the loss's weights before x and the table.
+ * each): the weights before they meet v, k or dout, the scores' gradients before k and q, the loss's weights before x and the table (the attention's gradients
+ * of few or short lists and heads up to 64 keep what is rounded off).
  * Elements that take part are finite, in F32 at most 3.38e38 (bfloat16's largest: F32 arrays go through the matrix unit in bfloat16 planes, which makes NaN
  * of more).  An infinite or NaN element of a query's row stays with that query's outputs; one of a key's row reaches the queries of its segment,
  * also those before it in causal order; what is masked (keys not kept, rows without a label) may hold anything. */

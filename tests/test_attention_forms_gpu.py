@@ -109,3 +109,22 @@ def test_two_calls_at_once(dtype, dev):
     for x, y in zip(alone, both):
         for n in ALL:
             assert torch.equal(x[n], y[n]), n
+
+
+@pytest.mark.parametrize("dim", [24, 64])
+@pytest.mark.parametrize("form", ["split", "solo"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_small_gradients_are_rounded_once(form, dim, causal, dev):
+    """bf16 gradients of few or short lists are as far off as their own rounding makes them: an error spread over a step of 2^-7 of the power of two below a
+    value has the root mean square 2^-7 / sqrt(12) = 0.00226 of that, and less of the value (0.0017 of normal ones).  Weights rounded before them make
+    sqrt(2) times the 0.0017, 0.00235."""
+    n, q, k, heads = FORMS[form]
+    q, k = lengths(n + dim, n, q, k)
+    case = AttentionCase("bf16", q, k, heads, heads, dim, causal=causal, boundaries=[-5, 0], q_start=[max(0, b - a) for a, b in zip(q, k)], seed=70)
+    d, ref = case.to(dev), case.reference()
+    capi.check(case.forward(d))
+    capi.check(case.backward(d))
+    for name, rows in (("dq", case.nq), ("dk", case.nk), ("dv", case.nk)):
+        got = d[name][:rows, :heads * dim].cpu().double().view(rows, heads, dim)
+        off = ((got - ref[name][0]).norm() / ref[name][0].norm()).item()
+        assert off <= 2.0 ** -7 / 12 ** 0.5, (name, off)

@@ -3,7 +3,10 @@
 //   query side  S^T = K Q^T and dP^T = V dO^T by 32 queries a wave, dQ^T += K^T dS^T; delta = <do, out> on the way, kept for the key side;
 //               the bias gradient's sums over a tile's diagonals
 //   key side    S = Q K^T and dP = dO V^T by 32 keys a wave, over the queries of every head of the group: dV^T += dO^T P, dK^T += Q^T dS
-// p and ds are rounded to bf16 for the second products of bf16 arrays, half a step each, as the results are; everything that is summed is f32.
+// p and ds are rounded to bf16 for the second products of bf16 arrays, half a step each, as the results are; everything that is summed is f32.  Where a
+// wave has items or tiles of its own and heads are up to 64 wide, ds (and p on the key side) keep what is rounded off as a second plane (FINE): rounding them
+// makes sqrt(2) times the error of rounding the results, and small calls scatter above that, but wait for latencies more than for the matrix unit (bf16
+// with gradients, 512 x (<= 40 x 200), 4 heads of 16: 70 -> 72 us; 300 x (<= 40 x 90), 8 heads of 64: 66 -> 71; wider heads would spill).
 // Measured on 16 segments of 1024 x 1024, 8 heads, bf16: query side 92 us at 64 wide (747 TF/s of its four products) and 235 at 128 (584), key side 98
 // (703) and 240 (573): at 128 the accumulators leave one wave a SIMD, whose exponents then run beside nothing.  f32 in planes at 64: 272 and 428 us.
 // 512 segments of up to 40 x 200, 4 heads of 16, f32 with a bias: 37 and 35 us, the latency of each wave's few tiles and of its bias tables.
@@ -82,6 +85,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
     using S = typename Mma<M>::Store;
     constexpr bool ROUNDED = Mma<M>::ROUNDS;
     constexpr bool OWN = FORM != ROWS;                                  // tiles of a wave's own
+    constexpr bool FINE = ROUNDED && OWN && DP <= 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
     S* kt = reinterpret_cast<S*>(lds) + (OWN ? wave * 2 * Q::BUFS * TILE : 0);
     S* vt = kt + Q::BUFS * TILE;
@@ -298,6 +302,11 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 || (FORM == 
                             }
                         }
                         const auto w = Mma<M>::pack(p[k]);
+                        if constexpr (FINE) {
+                            const auto rest = Mma<M>::pack_rest(p[k], w);
+#pragma unroll
+                            for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(kb, 32 * k, 32 * d, rest, acc[d]);
+                        }
 #pragma unroll
                         for (int d = 0; d < DP / 32; ++d) acc[d] = Mma<M>::template weigh<DP>(kb, 32 * k, 32 * d, w, acc[d]);
                     }
@@ -452,7 +461,7 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
     using M = AttnKind<T, DP>;
     using S = typename Mma<M>::Store;
     constexpr int QT = Kd::QT, TILE = Kd::TILE, BUFS = Kd::BUFS, STEP = FORM == KEY_SPLIT ? 4 : 1;
-    constexpr bool OWN = Kd::OWN;
+    constexpr bool OWN = Kd::OWN, FINE = Mma<M>::ROUNDS && OWN && DP <= 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, kv_heads = a.heads / a.group, loader = OWN ? lane : tid;
     S* qt = reinterpret_cast<S*>(lds) + (OWN ? wave * 2 * BUFS * TILE : 0);
     S* gt = qt + BUFS * TILE;
@@ -566,12 +575,26 @@ __global__ __launch_bounds__(BWD_THREADS, (attn_width<T, DP> <= 192 ? 2 : 1)) vo
                         for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(fmaf(p[r], scale, far + ml[r >> 2][r & 3]));
                     }
                     const auto wp = Mma<M>::pack(p);
+                    if constexpr (FINE) {
+                        const auto rest = Mma<M>::pack_rest(p, wp);
+#pragma unroll
+                        for (int d = 0; d < DP / 32; ++d) {
+                            av[d] = Mma<M>::template weigh<DP>(gb, 32 * n, 32 * d, rest, av[d]);
+                            av[d] = Mma<M>::template weigh<DP>(gb, 32 * n, 32 * d, wp, av[d]);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);              // (p's planes are done with before ds's are made: registers)
+                    }
 #pragma unroll
                     for (int r = 0; r < 16; ++r) p[r] *= dp[r] - dl[r >> 2][r & 3];
                     const auto wd = Mma<M>::pack(p);
+                    if constexpr (FINE) {
+                        const auto rest = Mma<M>::pack_rest(p, wd);
+#pragma unroll
+                        for (int d = 0; d < DP / 32; ++d) ak[d] = Mma<M>::template weigh<DP>(qb, 32 * n, 32 * d, rest, ak[d]);
+                    }
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) {
-                        av[d] = Mma<M>::template weigh<DP>(gb, 32 * n, 32 * d, wp, av[d]);
+                        if constexpr (!FINE) av[d] = Mma<M>::template weigh<DP>(gb, 32 * n, 32 * d, wp, av[d]);
                         ak[d] = Mma<M>::template weigh<DP>(qb, 32 * n, 32 * d, wd, ak[d]);
                     }
                 }

@@ -122,6 +122,11 @@ template <> struct Mma<__bf16> {
         for (int i = 0; i < 16; ++i) r.w[i >> 3][i & 7] = (__bf16)p[i];
         return r;
     }
+    static __device__ __forceinline__ Weights pack_rest(f32x16 p, const Weights& first) {       // what pack has rounded off, exact to 2^-17 of a weight
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] -= (float)first.w[i >> 3][i & 7];
+        return pack(p);
+    }
     template <int DP>
     static __device__ __forceinline__ f32x16 weigh(const __bf16* tile, int row0, int col0, const Weights& p, f32x16 acc) {
         const int l = tile_lane<DP>(), row = row0 + 4 * (l >> 5) + ((l & 15) >> 2), col = col0 + 16 * ((l >> 4) & 1) + 4 * (l & 3);
