@@ -1559,6 +1559,7 @@ int dctr_create(const dctr_config* cfg, dctr_handle* h) {
 
 int dctr_destroy(dctr_handle E) {
     if (!E) return DCTR_OK;
+    (void)hipDeviceSynchronize();            // (the side streams outlive the handle: nothing on them may still use what is freed here)
     for (auto& kv : E->train_graphs) hipGraphExecDestroy(kv.second);
     for (auto& kv : E->predict_graphs) hipGraphExecDestroy(kv.second);
     if (E->table_rec != nullptr) {          // row records: the six table pointers are views into this one buffer

@@ -313,7 +313,7 @@ class Engine:
         return out_prob
 
     def main_stream(self):
-        """torch view (ExternalStream) of the engine-owned stream for step calls (dctr_main_stream)."""
+        """torch view (ExternalStream) of the library's stream for step calls (dctr_main_stream; one a device, shared by its engines)."""
         import torch
         p = C.c_void_p()
         capi.check(self._lib.dctr_main_stream(self._h, C.byref(p)))
